@@ -388,6 +388,86 @@ void skl_cvt_f8e5m2_bf16_gfx950(skl_bf16_t *dst, const uint8_t *src, size_t n);
  * source byte, low nibble first. */
 void skl_cvt_f4e2m1_f8e4m3_gfx950(uint8_t *dst, const uint8_t *src, size_t n);
 
+/* ======================================================================== */
+/* Microscaled 4-bit values (OCP MXFP4): conversions and products            */
+/* ======================================================================== */
+
+/* An MXFP4 matrix has rows of E2M1 values (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives), two to a byte, the first in
+ * the low half (the packing ref/cvt/cvt_ofp4.c:59-68 reads), and one E8M0 byte per 32 consecutive values of a row: value
+ * (i, p) is 4-bit number i * ld + p of the codes, times 2^(scales[i * lds + p / 32] - 127); a scale byte of 255 makes a NaN of
+ * each of its 32 values. The last block of a row holds k % 32 values where that is not zero. Rows begin on bytes: ld is
+ * even (for one row it does not count). The reference has no notion of block scales; the rules here are those of the OCP
+ * microscaling formats.
+ *
+ * Quantisation: element (i, p) of the source at src[i * rs + p * cs], both strides free, so that rs = 1 quantises the
+ * columns of a row-major matrix - the transposed operand that a layer's gradients multiply. With a the largest magnitude of
+ * a block, its scale is 2^s, s = max(floor(log2 a) - 2, -126), and a value x becomes the E2M1 value nearest to x / 2^s,
+ * ties to the even code, 6 in magnitude at most, the sign of a zero kept. A block of zeros has s = -126; one that holds a NaN or an infinity
+ * gets the scale byte 255 and codes 0. Every scale byte written otherwise lies in [1, 252]. With an odd k the half byte behind a
+ * row's last value is written as 0; nothing else outside the m x k values and their scales is written. */
+void skl_cvt_f32rc_mxf4e2m1_gfx950(size_t m, size_t k, const float *src, size_t rs, size_t cs, uint8_t *dst, size_t ldd,
+                                   uint8_t *scales, size_t lds);
+void skl_cvt_bf16rc_mxf4e2m1_gfx950(size_t m, size_t k, const skl_bf16_t *src, size_t rs, size_t cs, uint8_t *dst, size_t ldd,
+                                    uint8_t *scales, size_t lds);
+/* The way back, exact for every scale byte: f32 and bf16 hold each of these values (the smallest is 2^-128, subnormal in both).
+ * Element (i, p) of the result at dst[i * rs + p * cs]. */
+void skl_cvt_mxf4e2m1_f32rc_gfx950(size_t m, size_t k, const uint8_t *src, size_t ldsrc, const uint8_t *scales, size_t lds,
+                                   float *dst, size_t rs, size_t cs);
+void skl_cvt_mxf4e2m1_bf16rc_gfx950(size_t m, size_t k, const uint8_t *src, size_t ldsrc, const uint8_t *scales, size_t lds,
+                                    skl_bf16_t *dst, size_t rs, size_t cs);
+
+/* C = alpha * A * B + beta * C of two MXFP4 operands: A's rows and B's columns are K-contiguous (B is stored column by column,
+ * as a linear layer's [out][in] weight is), n columns of B as rows of an MXFP4 matrix. alpha, beta, C and the empty cases as in
+ * skl_gemm_f32rc_f32rc_f32rc_gfx950. Products are exact, sums are in fp32 on the matrix cores, in an order that depends on the sizes
+ * and layouts alone; the result is that of ref/gemm/gemm_f32rc_f32rc_f32rc.h:44 on the decoded operands, inside its error bound.
+ * A block whose scale byte is 255 makes NaN of what it enters; every other byte is a scale, 0 (2^-127) included.
+ * A layer in training multiplies three times, each operand quantised along the axis that the product sums over:
+ *   y (m x n)  = A B            A: x by rows,        B: W by rows
+ *   dx (m x k) = dy W           A: dy by rows,       B: W by columns   (rs = 1)
+ *   dW (n x k) = dy^T x         A: dy by columns,    B: x by columns
+ * and the gradients pass the quantisers as they are. */
+void skl_gemm_mxf4e2m1r_mxf4e2m1c_f32rc_gfx950(size_t m, size_t n, size_t k, float alpha, const uint8_t *a, size_t lda,
+                                               const uint8_t *scales_a, size_t lsa, const uint8_t *b, size_t ldb,
+                                               const uint8_t *scales_b, size_t lsb, float beta, float *c, size_t rsc,
+                                               size_t csc);
+
+/* ======================================================================== */
+/* A mixture-of-experts layer over MXFP4 weights                             */
+/* ======================================================================== */
+
+/* For each of `tokens` rows x of X (bf16, row t at x + t * ldx):
+ *   l_e = sum_p x_p * router[e][p]                                        for the `experts` rows of the router
+ *   the top_k largest l_e, in descending order, ties by the lower e; NaN counts as the lowest
+ *   w_j = exp(l_j - max l) / sum exp(l - max l), the sum over the chosen ones (normalise != 0) or over all experts
+ *   h_j = act(x gate_j^T) * (x up_j^T)                                    `inter` values, gate and up of expert j: inter x hidden
+ *   y   = beta * residual + sum_j w_j * (h_j down_j^T)                    `hidden` values, down: hidden x inter
+ * X, the logits' and all further products and sums are exact products summed in fp32; h, times its w, is held as the sum of two bf16
+ * values (16 bits of significand, the error of a sum of a few hundred fp32 products), nothing else is rounded to fewer bits. Every sum's order depends
+ * on the sizes and on who was chosen alone: the same call gives the same bits.
+ * residual may be y (each with its own row distance), or NULL with beta == 0, where it is not read. Made for a few tokens: the weights are read once for up to 64
+ * tokens, and again for each further 64.
+ * hidden and inter are multiples of 32; experts <= 1024, top_k <= experts, top_k <= 64; every row of weights and of X begins on a
+ * 16-byte boundary (pointers and distances); anything else is SKL_HIP_ERR_BAD_ARGUMENT, and nothing is done. */
+typedef struct skl_gfx950_moe {
+  size_t hidden, inter, experts, top_k;
+  const skl_bf16_t *router; /* experts x hidden, rows ld_router apart */
+  size_t ld_router;
+  const uint8_t *gate, *up; /* MXFP4, per expert inter x hidden: rows ld_in values apart, experts expert_in values apart */
+  size_t ld_in, expert_in;
+  const uint8_t *gate_scales, *up_scales; /* rows ld_in_scales bytes apart, experts expert_in_scales */
+  size_t ld_in_scales, expert_in_scales;
+  const uint8_t *down; /* MXFP4, per expert hidden x inter */
+  size_t ld_down, expert_down;
+  const uint8_t *down_scales;
+  size_t ld_down_scales, expert_down_scales;
+  int activation;  /* SKL_GFX950_ACT_*, on the gate */
+  int normalise;
+  int32_t *ids;    /* tokens x top_k, the chosen experts; NULL: not wanted */
+  float *weights;  /* tokens x top_k, their weights; NULL: not wanted */
+} skl_gfx950_moe_t;
+void skl_moe_bf16_mxf4e2m1_f32_gfx950(const skl_gfx950_moe_t *layer, size_t tokens, const skl_bf16_t *x, size_t ldx, float beta,
+                                      const float *residual, size_t ld_residual, float *y, size_t ldy);
+
 #ifdef __cplusplus
 }
 #endif

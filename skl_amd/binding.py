@@ -74,9 +74,26 @@ class Epilogue:
                                          _as_pointer(self.q_scale), int(self.q_format))
 
 
+class MoeLayer:
+    """A mixture-of-experts layer (`skl_gfx950_moe_t`, every member by its name there) for `skl_moe_bf16_mxf4e2m1_f32`. Pointers are
+    DeviceBuffers, numpy arrays, integer addresses or None; what they refer to is kept as long as the layer is. The C descriptor is
+    made once."""
+
+    def __init__(self, **members):
+        fields = dict(signatures.MoeStruct._fields_)
+        unknown = set(members) - set(fields)
+        if unknown:
+            raise TypeError(f"skl_gfx950_moe_t has no member {sorted(unknown)[0]}")
+        self.members = members
+        self._struct = signatures.MoeStruct(**{name: _as_pointer(v) if fields[name] is ctypes.c_void_p else int(v) for name, v in members.items()})
+
+    def as_struct(self):
+        return self._struct
+
+
 def _wrap(raw, sig):
     ptr_positions = [i for i, ch in enumerate(sig) if ch == "p"]
-    epilogue_positions = [i for i, ch in enumerate(sig) if ch == "E"]
+    epilogue_positions = [i for i, ch in enumerate(sig) if ch in "EM"]
 
     def call(*args):
         if len(args) != len(sig):

@@ -17,6 +17,7 @@
 #include <string.h>
 
 #include "../../include/skl-gfx950.h"
+#include "skl_host.h"
 #include "skl_launch.h"
 
 #define SKL_TE 64u
@@ -48,29 +49,8 @@ static size_t span4(size_t d0, size_t s0, size_t d1, size_t s1, size_t d2, size_
 /* Classifies up to three pointers (NULL entries are skipped).
  * Returns 1 all device, 0 all host, -1 mixed (error recorded). */
 static int classify(const void *p0, const void *p1, const void *p2, const char *who) {
-  const void *p[3];
-  int n = 0, dev = 0;
-  if (p0) p[n++] = p0;
-  if (p1) p[n++] = p1;
-  if (p2) p[n++] = p2;
-  if (skl_hip_get_pointer_mode() == SKL_HIP_POINTERS_DEVICE) return 1;
-  for (int i = 0; i < n; ++i) dev += skl_hip_pointer_is_device(p[i]) ? 1 : 0;
-  if (dev == n) return 1;
-  if (dev == 0) return 0;
-  skl_hip_record_error(SKL_HIP_ERR_MIXED_POINTERS, who);
-  return -1;
-}
-
-/* Device copy of a host span (NULL on failure or empty span). */
-static void *stage_in(const void *host, size_t bytes) {
-  void *d;
-  if (bytes == 0) return NULL;
-  d = skl_hip_malloc(bytes);
-  if (d && skl_hip_memcpy_h2d(d, host, bytes) != 0) {
-    skl_hip_free(d);
-    d = NULL;
-  }
-  return d;
+  const void *p[3] = {p0, p1, p2};
+  return skl_classify(p, 3, who);
 }
 
 /* ------------------------------------------------------------------------ */
@@ -616,12 +596,12 @@ static void gemm_run(const skl_gemm_desc *in, const char *who) {
     skl_gemm_desc dd = *d;
     const size_t esc = c_elem_size(d->ta);
     const int untouched = c_untouched(d); /* then the caller's C need not exist: a stand-in that no kernel touches */
-    void *da = stage_in(d->a, na * esa), *db = stage_in(d->b, nb * esb), *dc = untouched ? skl_hip_malloc(16) : stage_in(d->c, nc * esc);
-    void *dbias = d->bias ? stage_in(d->bias, N * esc) : NULL, *dmax = d->max ? stage_in(d->max, esc) : NULL;
+    void *da = skl_stage_in(d->a, na * esa), *db = skl_stage_in(d->b, nb * esb), *dc = untouched ? skl_hip_malloc(16) : skl_stage_in(d->c, nc * esc);
+    void *dbias = d->bias ? skl_stage_in(d->bias, N * esc) : NULL, *dmax = d->max ? skl_stage_in(d->max, esc) : NULL;
     /* the requantised copy: its whole span travels both ways, like C's */
     const size_t nq = d->rq.q ? (M - 1) * d->rq.rsq + (N - 1) * d->rq.csq + 1 : 0;
-    void *dq = d->rq.q ? stage_in(d->rq.q, nq) : NULL;
-    void *dqs = d->rq.q ? stage_in(d->rq.q_scale, (d->rq.q_per_column ? N : 1) * sizeof(float)) : NULL;
+    void *dq = d->rq.q ? skl_stage_in(d->rq.q, nq) : NULL;
+    void *dqs = d->rq.q ? skl_stage_in(d->rq.q_scale, (d->rq.q_per_column ? N : 1) * sizeof(float)) : NULL;
     if ((na && !da) || (nb && !db) || !dc || (d->bias && !dbias) || (d->max && !dmax) || (d->rq.q && (!dq || !dqs))) {
       skl_hip_free(da);
       skl_hip_free(db);
@@ -844,7 +824,7 @@ static void f4_gemm_run(size_t m, size_t n, size_t k, float alpha, const uint8_t
   {
     const size_t na = k ? (m - 1) * rsa + (k - 1) * csa + 1 : 0, nb = k ? ((n - 1) * ldb + k + 1) / 2 : 0;
     const size_t ns = (k && scales) ? (n - 1) * lds + (k + 31) / 32 : 0, nc = (m - 1) * rsc + (n - 1) * csc + 1;
-    void *da = stage_in(a, na), *db = stage_in(b, nb), *ds = stage_in(scales, ns), *dc = stage_in(c, nc * sizeof(float));
+    void *da = skl_stage_in(a, na), *db = skl_stage_in(b, nb), *ds = skl_stage_in(scales, ns), *dc = skl_stage_in(c, nc * sizeof(float));
     if ((!na || da) && (!nb || db) && (!ns || ds) && dc &&
         f4_gemm_on_device(m, n, k, alpha, (const uint8_t *)da, rsa, csa, (const uint8_t *)db, ldb, (const uint8_t *)ds, lds, beta_s,
                           (float *)dc, rsc, csc) == 0)
@@ -934,7 +914,7 @@ static void pack_run(int esize, size_t m, size_t n, const void *src, size_t rs, 
     const size_t m1 = (m + m0 - 1) / m0, n1 = (n + n0 - 1) / n0;
     const size_t ns = span4(m, rs, n, cs, 1, 0, 1, 0);
     const size_t nd = span4(m1, rs1, n1, cs1, m0, rs0, n0, cs0);
-    void *ds = stage_in(src, ns * esize), *dd = stage_in(dst, nd * esize);
+    void *ds = skl_stage_in(src, ns * esize), *dd = skl_stage_in(dst, nd * esize);
     if (ds && dd) {
       skl_hip_launch_pack(esize, m, n, ds, rs, cs, m0, n0, dd, rs0, cs0, rs1, cs1, pad);
       skl_hip_memcpy_d2h(dst, dd, nd * esize);
@@ -968,8 +948,8 @@ static void unpack_run(int esize, size_t m0, size_t n0, const void *src, size_t 
     if (m1 > 1 && (m1 - 2) * rs1 + (m0 - 1) * rs0 > max_r) max_r = (m1 - 2) * rs1 + (m0 - 1) * rs0;
     if (n1 > 1 && (n1 - 2) * cs1 + (n0 - 1) * cs0 > max_c) max_c = (n1 - 2) * cs1 + (n0 - 1) * cs0;
     ns = max_r + max_c + 1;
-    ds = stage_in(src, ns * esize);
-    dd = stage_in(dst, nd * esize);
+    ds = skl_stage_in(src, ns * esize);
+    dd = skl_stage_in(dst, nd * esize);
     if (ds && dd) {
       skl_hip_launch_unpack(esize, m0, n0, ds, rs0, cs0, rs1, cs1, m, n, dd, rs, cs);
       skl_hip_memcpy_d2h(dst, dd, nd * esize);
@@ -1039,7 +1019,7 @@ static void cvt_run(int kind, int fmt, int sat, void *dst, const void *src, floa
   src_bytes = kind == 3 ? (n + 1) / 2 : n * src_num[kind];
   dst_bytes = n * dst_size[kind];
   if (where == 0) {
-    ds = stage_in(src, src_bytes);
+    ds = skl_stage_in(src, src_bytes);
     dd = skl_hip_malloc(dst_bytes);
     if (!ds || !dd) {
       skl_hip_free(ds);

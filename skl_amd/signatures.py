@@ -3,7 +3,7 @@
 Each character is one C parameter: ``z`` size_t, ``p`` pointer, ``i`` int32_t,
 ``f`` float, ``d`` double, ``b`` uint8_t, ``h`` uint16_t, ``w`` uint32_t,
 ``B`` bool,
-``H`` a ``_Float16`` passed by value, ``E`` a pointer to a ``skl_gfx950_epilogue_t``.
+``H`` a ``_Float16`` passed by value, ``E`` a pointer to a ``skl_gfx950_epilogue_t``, ``M`` one to a ``skl_gfx950_moe_t``.
 Names are given without the implementation suffix (``_gfx950`` for the GPU
 library); the parameter order is the reference's (include/skl-gfx950.h cites
 the prototype each one mirrors).
@@ -38,6 +38,7 @@ CTYPES = {
     "B": ctypes.c_bool,
     "H": HalfByValue,
     "E": ctypes.c_void_p,
+    "M": ctypes.c_void_p,
 }
 
 
@@ -47,6 +48,17 @@ class EpilogueStruct(ctypes.Structure):
                 ("q_scale_per_column", ctypes.c_int), ("q_only", ctypes.c_int), ("q_zero", ctypes.c_int32),
                 ("q", ctypes.c_void_p), ("rsq", ctypes.c_size_t), ("csq", ctypes.c_size_t),
                 ("q_scale", ctypes.c_void_p), ("q_format", ctypes.c_int)]
+
+
+class MoeStruct(ctypes.Structure):
+    """``skl_gfx950_moe_t`` (include/skl-gfx950.h)."""
+    _fields_ = [(name, ctypes.c_size_t) for name in ("hidden", "inter", "experts", "top_k")] + [
+        ("router", ctypes.c_void_p), ("ld_router", ctypes.c_size_t),
+        ("gate", ctypes.c_void_p), ("up", ctypes.c_void_p), ("ld_in", ctypes.c_size_t), ("expert_in", ctypes.c_size_t),
+        ("gate_scales", ctypes.c_void_p), ("up_scales", ctypes.c_void_p), ("ld_in_scales", ctypes.c_size_t), ("expert_in_scales", ctypes.c_size_t),
+        ("down", ctypes.c_void_p), ("ld_down", ctypes.c_size_t), ("expert_down", ctypes.c_size_t),
+        ("down_scales", ctypes.c_void_p), ("ld_down_scales", ctypes.c_size_t), ("expert_down_scales", ctypes.c_size_t),
+        ("activation", ctypes.c_int), ("normalise", ctypes.c_int), ("ids", ctypes.c_void_p), ("weights", ctypes.c_void_p)]
 
 
 def _rc(s):      # m n k alpha a rsa csa b rsb csb beta c rsc csc
@@ -172,6 +184,11 @@ def gfx950_only():
     sigs["skl_pack_e8_e8p8x4"] = "zzpzpzb"
     sigs["skl_pack_e32_e32p4x4"] = "zzpzpzw"
     sigs["skl_unpack_e32p4x4_e32"] = "zzpzpz"                     # m n src rs1 dst rs
+    for src in ("f32", "bf16"):                                    # m k src rs cs dst ldd scales lds, and back
+        sigs[f"skl_cvt_{src}rc_mxf4e2m1"] = "zzpzzpzpz"
+        sigs[f"skl_cvt_mxf4e2m1_{src}rc"] = "zzpzpzpzz"
+    sigs["skl_gemm_mxf4e2m1r_mxf4e2m1c_f32rc"] = "zzzfpzpzpzpzfpzz"     # m n k alpha a lda sa lsa b ldb sb lsb beta c rsc csc
+    sigs["skl_moe_bf16_mxf4e2m1_f32"] = "Mzpzfpzpz"                     # layer tokens x ldx beta residual ld y ldy
     for name, sig in GEMM_FUSED.items():
         sigs[name] = sig + "E"
     for w, pad in _PAD.items():
