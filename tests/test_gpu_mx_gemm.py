@@ -58,7 +58,8 @@ def check(lib, mode, rng, m, n, k, alpha=1.0, beta=0.0, rsc=None, csc=1, **layou
 
 # whole tiles and ragged ones of every kernel, K of one value, of a block, off blocks and chunks, rows off every alignment
 SHAPES = ((1, 1, 1), (1, 33, 32), (2, 64, 64), (5, 300, 100), (16, 512, 4096), (17, 130, 513), (31, 1, 700), (33, 65, 31), (64, 64, 256), (65, 129, 288),
-          (100, 200, 1000), (128, 128, 512), (130, 257, 2049), (512, 512, 512), (300, 700, 770), (1, 4096, 2080), (48, 1024, 11008))
+          (100, 200, 1000), (128, 128, 512), (130, 257, 2049), (512, 512, 512), (300, 700, 770), (1, 4096, 2080), (48, 1024, 11008), (16, 4100, 256), (17, 8200, 544), (64, 12300, 1024), (3, 9000, 4128),
+          (40, 12000, 8192), (64, 64, 14336), (200, 190, 6000))
 
 
 @pytest.mark.parametrize("mode", MODES)
@@ -76,7 +77,7 @@ def test_distances_off_every_alignment(gpu, m, n, k, layout):
     check(gpu, "device", np.random.default_rng(k), m, n, k, **layout)
 
 
-@pytest.mark.parametrize("m,n,k", ((70, 90, 256), (8, 200, 512), (300, 260, 320)))
+@pytest.mark.parametrize("m,n,k", ((70, 90, 256), (8, 200, 512), (300, 260, 320), (1500, 1501, 256)))
 def test_c_by_columns_and_with_gaps(gpu, m, n, k):
     rng = np.random.default_rng(m)
     check(gpu, "device", rng, m, n, k, rsc=1, csc=m + 2)
@@ -84,18 +85,21 @@ def test_c_by_columns_and_with_gaps(gpu, m, n, k):
     check(gpu, "device", rng, m, n, k, rsc=2 * n + 5, csc=2)
 
 
-@pytest.mark.parametrize("m,n,k", ((2048, 2304, 512), (1300, 3400, 300), (3500, 4100, 1056)))
-def test_large_tiles_are_exact(gpu, m, n, k):
-    """One scale everywhere: every partial sum is a multiple of a quarter below 2^24 quarters."""
+@pytest.mark.parametrize("m,n,k,ld", ((2048, 2304, 512, None), (1300, 3400, 300, None), (3500, 4100, 1056, None), (1500, 1472, 257, None), (1409, 1500, 4133, None),
+                                      (2048, 4100, 31, None), (2040, 4097, 1315, None), (2049, 6300, 345, 348), (3400, 4097, 64, 66), (3329, 4100, 2049, 2056),
+                                      (1500, 1500, 1024, 1024), (2048, 4096, 1536, 1536), (3328, 4096, 512, 520), (1500, 1500, 2047, None)))
+def test_large_tiles_are_exact(gpu, m, n, k, ld):
+    """One scale everywhere: every partial sum is a multiple of a quarter below 2^24 quarters. Each tile size; K below a block, of one chunk, of several, off blocks
+    and chunks; rows that loads to LDS read and rows that are copied."""
     rng = np.random.default_rng(k)
-    a, b = operand(rng, m, k, low=127, high=128), operand(rng, n, k, low=127, high=128)
+    a, b = operand(rng, m, k, ld, low=127, high=128), operand(rng, n, k, ld, low=127, high=128)
     c = np.full(m * n, np.nan, np.float32)
     got = run(gpu, "device", a, b, k, 1.0, 0.0, c, m, n, n, 1).reshape(m, n)
     want = (mx.values(a[0], a[1]).astype(np.float32) @ mx.values(b[0], b[1]).astype(np.float32).T)  # exact in fp32 for the same reason
     assert np.array_equal(got, want)
 
 
-@pytest.mark.parametrize("m,n,k", ((16, 96, 640), (70, 40, 640), (300, 4096, 640), (2048, 2048, 640)))
+@pytest.mark.parametrize("m,n,k", ((16, 96, 640), (70, 40, 640), (300, 4096, 640), (1500, 1500, 1600), (2048, 4096, 2048), (3500, 4096, 1632)))
 def test_every_value_and_scale_is_read_back(gpu, m, n, k):
     """Rows of A with a single one read single columns of B, each value times its own block's scale; every scale byte but 255."""
     rng = np.random.default_rng(m)
@@ -115,7 +119,7 @@ def test_every_value_and_scale_is_read_back(gpu, m, n, k):
 def test_scales_of_nan(gpu):
     """A block whose scale byte is 255 makes NaN of its row of C, in A and in B, wherever in K it lies, and of nothing else."""
     rng = np.random.default_rng(4)
-    for m, n, k in ((5, 90, 352), (150, 130, 352)):
+    for m, n, k in ((5, 90, 352), (150, 130, 352), (1500, 1500, 352)):
         a, b = operand(rng, m, k), operand(rng, n, k)
         for op, row, block in ((a, 3, 10), (b, 88, 0)):
             op[1][row, block] = 255
