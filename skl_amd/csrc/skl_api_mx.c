@@ -168,7 +168,7 @@ static int moe_ok(const skl_gfx950_moe_t *l, size_t tokens, const void *x, size_
   if (l->ld_in % 32 != 0 || l->ld_in < h || l->expert_in % 32 != 0 || l->ld_down % 32 != 0 || l->ld_down < i || l->expert_down % 32 != 0) return 0;
   if (l->ld_in_scales < h / 32 || l->ld_down_scales < i / 32) return 0;
   /* a workgroup's offsets from its first row are 32-bit numbers */
-  if (h > ((size_t)1 << 24) || i > ((size_t)1 << 24) || l->ld_in > ((size_t)1 << 26) || l->ld_down > ((size_t)1 << 26)) return 0;
+  if (h > ((size_t)1 << 24) || i > ((size_t)1 << 24) || l->ld_in > ((size_t)1 << 24) || l->ld_down > ((size_t)1 << 24) || (tokens > 1 && ldx > ((size_t)1 << 23))) return 0;
   return 1;
 }
 

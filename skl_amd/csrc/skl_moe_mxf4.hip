@@ -8,10 +8,11 @@
 // The tokens of an expert are gathered: only rows of tokens that chose it are multiplied, 16 at a time. h travels as the sum of three bf16
 // values, which is all of its 24 bits: two (7.6e-6 off at most) left y 1.0e-6 off, three 3e-7, and the stream covers the third's products.
 //
-// Three launches, each with a workgroup per piece of work so that the stream finds every compute unit; what must follow all of a
-// launch's workgroups is done by the one that arrives last (a counter that is zero between calls): the choice behind the router's
-// sums, and the weighted sum over a token's experts behind the output products. Every sum has a fixed order.
+// Four launches, each with a workgroup per piece of work so that the stream finds every compute unit: the router, whose last workgroup (a counter that is zero
+// between calls) makes the choice behind everyone's sums; the two products; the weighted sum over a token's experts. Every sum has a fixed order.
 #include <hip/hip_runtime.h>
+
+#include <atomic>
 
 #include "skl_device.hpp"
 #include "skl_mx.h"
@@ -20,6 +21,7 @@
 namespace {
 
 typedef int v4i __attribute__((ext_vector_type(4)));
+typedef float v2f __attribute__((ext_vector_type(2)));
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
@@ -39,7 +41,7 @@ struct Routing {
   unsigned *place;       // [token][j], of its j-th choice
   uint16_t *h[3];        // [place][inter]: the terms
   float *out;            // [split][place][hidden], the output products
-  unsigned *counters;    // zero between launches: the router's, then one per tile of columns of y
+  unsigned *counter;     // zero between launches
   unsigned router_splits, out_splits, places;
 };
 
@@ -57,7 +59,7 @@ __device__ __forceinline__ unsigned short bf16_of(float v) { return __builtin_bi
 __device__ __forceinline__ float of_bf16(unsigned short v) { return __uint_as_float((unsigned)v << 16); }
 
 // What one workgroup leaves for another of the same launch goes past its die's cache and is read past it, value by value; a fence
-// instead writes all of that cache back, for every workgroup (the output products of 7 tokens 147 us with fences).
+// instead writes all of that cache back, for every workgroup (tens of microseconds).
 __device__ __forceinline__ void leave(float *to, float v) { __hip_atomic_store(to, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 __device__ __forceinline__ float found(const float *from) { return __hip_atomic_load(from, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 
@@ -194,7 +196,7 @@ __global__ void __launch_bounds__(kRouterThreads) moe_router_kernel(MoeArgs a) {
     for (int w = 0; w < kRouterThreads / 64; ++w) v += s.red[w][i][j];
     if (t0 + i < p.tokens && e0 + j < p.experts) leave(a.r.parts + ((size_t)blockIdx.z * p.tokens + t0 + i) * p.experts + e0 + j, v);
   }
-  if (!arrives_last(a.r.counters, gridDim.x * gridDim.y * gridDim.z, &arrived)) return;
+  if (!arrives_last(a.r.counter, gridDim.x * gridDim.y * gridDim.z, &arrived)) return;
   const unsigned top = (unsigned)p.top_k, tokens = (unsigned)p.tokens, e = threadIdx.x;
   s.c.mask[e][0] = s.c.mask[e][1] = 0;  // one thread per expert
   __syncthreads();
@@ -229,137 +231,346 @@ __global__ void __launch_bounds__(kRouterThreads) moe_router_kernel(MoeArgs a) {
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// The two products. A workgroup has CG groups of 16 rows of one expert's weights - columns of the result -, RG groups of 16 of its tokens
-// at a time, and a range of k, of which each of its four waves takes a quarter: chunks of 128, the next one requested before one is
-// multiplied. The waves' sums meet in LDS.
+// The two products. A workgroup of eight waves has 64 CG rows of one expert's weights - columns of the result - and up to 16 RG of its tokens at a time. K comes in
+// chunks of 256, a line of a row of weights and four (TERMS times) of a token, from memory to LDS without registers, whole lines at a time, a few chunks ahead. Four
+// pairs of waves have 16 CG rows of weights each; of a pair, each has its half of every chunk, so that a token is read from LDS four times and not eight.
+// 64 tokens, 2 of 8 experts of 14336 x 4096: 114 us for h (500 MB of weights, 4.4 TB/s) and 93 for the output products (250 MB and three terms of h, of which each
+// workgroup has to have all: 2.7 TB/s). Read straight into registers as the operands lie - 16 lines for 1024 bytes, and as many for every token's - the compute
+// units' address paths bound them: 193 and 205 us. 7 tokens, 3 of 20 experts of 1440 x 2080: 20 and 12 us, 1 token, 4 of 32 of 1024 x 2048: 9 and 6, most of it the
+// way to a launch's first bytes.
+// A chunk half is four steps of 32 k (8 from each lane group's block): the products of one run while the operands of the next come from LDS.
 // ---------------------------------------------------------------------------------------------------------------------
+typedef __attribute__((address_space(3))) char lds_char;
+typedef unsigned unsigned_any __attribute__((aligned(1)));
+constexpr int kWaves = 8, kThreads = kWaves * 64, kChunk = 256, kLine = 128;
+constexpr unsigned kRange = 0x7FFFFFF0u, kOutside = 0x7FFFFFF0u;  // of a buffer descriptor; an offset that loads zeros
 
-constexpr int kWaves = 4;
-
-struct Row {  // of weights: this lane's
-  const uint8_t *codes, *scales;
+template <int CG_, int RG_, int TERMS_>
+struct Shape {
+  static constexpr int CG = CG_, RG = RG_, TERMS = TERMS_;
+  static constexpr int kAll = 64 * CG;  // rows of weights
+  static constexpr int kWeightBytes = kAll * kLine, kTokenBytes = TERMS * 16 * RG * 512;  // of a chunk
+  // Two rings, that of the weights the deeper one: they come from memory, the tokens from a cache. Both for two workgroups per compute unit where two chunks of each fit.
+  static constexpr int kBudget = (2 * (kWeightBytes + kTokenBytes) <= 80 * 1024 ? 80 : 160) * 1024;
+  static constexpr int kFit = (kBudget - 2 * kTokenBytes) / kWeightBytes, kWeightStages = kFit < 4 ? kFit : 4;
+  static constexpr int kRest = (kBudget - kWeightStages * kWeightBytes) / kTokenBytes, kTokenStages = kRest < kWeightStages ? kRest : kWeightStages;
+  static constexpr int kLoads = CG + RG * TERMS;  // requests of a wave per chunk
+  // With rings of one depth a chunk's weights are requested before its tokens, else behind them: what may be under way when the next chunk has to be there.
+  static constexpr bool kTokensFirst = kWeightStages > kTokenStages;
+  static constexpr int kUnderWay = (kTokenStages - 2) * kLoads + (kTokensFirst ? CG : 0);
+  static constexpr int kTokensAt = kWeightStages * kWeightBytes, kLds = kTokensAt + kTokenStages * kTokenBytes;
+  static constexpr int kPitch = kAll + 1;  // of the sums, which meet in the rings' place
+  static_assert(kTokenStages >= 2 && 16 * RG * kPitch * 4 <= kLds && kUnderWay + kLoads < 63);
 };
 
-template <int CG, int RG, int TERMS>
-struct Chunk {
-  v4i w[CG];
-  unsigned s[CG];
-  v4i x[RG][TERMS][4];
-
-  // Blocks from `end` on are zeros with a scale of one, and so is what they meet.
-  __device__ __forceinline__ void load(const Row (&row)[CG], const uint16_t *const (&x0)[TERMS], const unsigned (&at)[RG], unsigned k, unsigned end, int g, unsigned groups) {
-    const unsigned own = k + 32u * (unsigned)g;
-    const bool in = own < end;
-    const unsigned from = in ? own : 0u;
-#pragma unroll
-    for (int c = 0; c < CG; ++c) {
-      const v4i v = *reinterpret_cast<const v4i *>(row[c].codes + from / 2);
-      const unsigned b = row[c].scales[from / 32];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) w[c][j] = in ? v[j] : 0;
-      s[c] = in ? b : 127u;
-    }
-#pragma unroll
-    for (int r = 0; r < RG; ++r)
-#pragma unroll
-      for (int t = 0; t < TERMS; ++t)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          v4i v = {0, 0, 0, 0};
-          if (r == 0 || r < (int)groups) v = *reinterpret_cast<const v4i *>(x0[t] + at[r] + from + 8 * j);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) x[r][t][j][i] = in ? v[i] : 0;
-        }
+// One step: acc[r][c] += x[r][t] b[c] over G groups of tokens, T terms and CG groups of columns, while the tokens' values of the next step come from `px` on into n - and,
+// if that is the first of a chunk, its weights from `pw` into w. The wait is the block's own: the compiler would make every read of LDS wait for all requests under way.
+#define SKL_MOE_MUL(a, x, b) "v_mfma_f32_16x16x32_bf16 %[" a "], %[" x "], %[" b "], %[" a "]\n"
+#define SKL_MOE_M1(c, t) SKL_MOE_MUL("a0" #c, "x0" #t, "b" #c)
+#define SKL_MOE_M2(c, t) SKL_MOE_M1(c, t) SKL_MOE_MUL("a1" #c, "x1" #t, "b" #c)
+#define SKL_MOE_C1(G, t) SKL_MOE_M##G(0, t)
+#define SKL_MOE_C2(G, t) SKL_MOE_C1(G, t) SKL_MOE_M##G(1, t)
+#define SKL_MOE_T1(C, G) SKL_MOE_C##C(G, 0)
+#define SKL_MOE_T3(C, G) SKL_MOE_C##C(G, 0) SKL_MOE_C##C(G, 1) SKL_MOE_C##C(G, 2)
+#define SKL_MOE_RX(r, t) "ds_read_b128 %[n" #r #t "], %[px] offset:%c[o" #r #t "]\n"
+#define SKL_MOE_RX11 SKL_MOE_RX(0, 0)
+#define SKL_MOE_RX21 SKL_MOE_RX11 SKL_MOE_RX(1, 0)
+#define SKL_MOE_RX13 SKL_MOE_RX11 SKL_MOE_RX(0, 1) SKL_MOE_RX(0, 2)
+#define SKL_MOE_RX23 SKL_MOE_RX13 SKL_MOE_RX(1, 0) SKL_MOE_RX(1, 1) SKL_MOE_RX(1, 2)
+#define SKL_MOE_RW1 "ds_read_b128 %[w0], %[pw]\n"
+#define SKL_MOE_RW2 SKL_MOE_RW1 "ds_read_b128 %[w1], %[pw] offset:2048\n"
+#define SKL_MOE_A(r, c) [a##r##c] "+v"(acc[r][c])
+#define SKL_MOE_A11 SKL_MOE_A(0, 0)
+#define SKL_MOE_A21 SKL_MOE_A11, SKL_MOE_A(0, 1)
+#define SKL_MOE_A12 SKL_MOE_A11, SKL_MOE_A(1, 0)
+#define SKL_MOE_A22 SKL_MOE_A21, SKL_MOE_A(1, 0), SKL_MOE_A(1, 1)
+#define SKL_MOE_N(r, t) [n##r##t] "=&v"(n[r][t])
+#define SKL_MOE_N11 SKL_MOE_N(0, 0)
+#define SKL_MOE_N21 SKL_MOE_N11, SKL_MOE_N(1, 0)
+#define SKL_MOE_N13 SKL_MOE_N11, SKL_MOE_N(0, 1), SKL_MOE_N(0, 2)
+#define SKL_MOE_N23 SKL_MOE_N13, SKL_MOE_N(1, 0), SKL_MOE_N(1, 1), SKL_MOE_N(1, 2)
+#define SKL_MOE_X(r, t) [x##r##t] "v"(x[r][t])
+#define SKL_MOE_X11 SKL_MOE_X(0, 0)
+#define SKL_MOE_X21 SKL_MOE_X11, SKL_MOE_X(1, 0)
+#define SKL_MOE_X13 SKL_MOE_X11, SKL_MOE_X(0, 1), SKL_MOE_X(0, 2)
+#define SKL_MOE_X23 SKL_MOE_X13, SKL_MOE_X(1, 0), SKL_MOE_X(1, 1), SKL_MOE_X(1, 2)
+#define SKL_MOE_W(c) [w##c] "=&v"(w[c])
+#define SKL_MOE_W1 SKL_MOE_W(0)
+#define SKL_MOE_W2 SKL_MOE_W1, SKL_MOE_W(1)
+#define SKL_MOE_B(c) [b##c] "v"(b[c])
+#define SKL_MOE_B1 SKL_MOE_B(0)
+#define SKL_MOE_B2 SKL_MOE_B1, SKL_MOE_B(1)
+#define SKL_MOE_OFFSETS [o00] "n"(0), [o01] "n"(TERM), [o02] "n"(2 * TERM), [o10] "n"(8192), [o11] "n"(8192 + TERM), [o12] "n"(8192 + 2 * TERM)
+#define SKL_MOE_STEP(C, G, T)                                                                                                                                          \
+  if constexpr (CG == C && GROUPS == G && TERMS == T) {                                                                                                                \
+    if constexpr (LAST)                                                                                                                                                \
+      asm volatile("s_nop 1\n" SKL_MOE_RW##C SKL_MOE_RX##G##T SKL_MOE_T##T(C, G) "s_waitcnt lgkmcnt(0)"                                                                \
+                   : SKL_MOE_A##C##G, SKL_MOE_N##G##T, SKL_MOE_W##C : SKL_MOE_X##G##T, SKL_MOE_B##C, SKL_MOE_OFFSETS, [px] "v"(px), [pw] "v"(pw) : "memory");          \
+    else                                                                                                                                                               \
+      asm volatile("s_nop 1\n" SKL_MOE_RX##G##T SKL_MOE_T##T(C, G) "s_waitcnt lgkmcnt(0)"                                                                              \
+                   : SKL_MOE_A##C##G, SKL_MOE_N##G##T : SKL_MOE_X##G##T, SKL_MOE_B##C, SKL_MOE_OFFSETS, [px] "v"(px) : "memory");                                      \
   }
-  __device__ __forceinline__ void multiply(v4f (&acc)[RG][CG], unsigned groups) const {
-#pragma unroll
-    for (int c = 0; c < CG; ++c) {
-      const float scale = __uint_as_float(s[c] << 23);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const v8bf b = widen_f4((unsigned)w[c][j], scale);
-#pragma unroll
-        for (int r = 0; r < RG; ++r)
-          if (r == 0 || r < (int)groups)
-#pragma unroll
-            for (int t = 0; t < TERMS; ++t) acc[r][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, x[r][t][j]), b, acc[r][c], 0, 0, 0);
-      }
-    }
-  }
-};
-
-// The sums of k in [first, end) into red[wave][row of tokens][column].
-template <int CG, int RG, int TERMS>
-__device__ __forceinline__ void stream(const Row (&row)[CG], const uint16_t *const (&x)[TERMS], const unsigned (&at)[RG], unsigned first, unsigned end, int wave, int lane,
-                                       unsigned groups, float (*red)[RG * 16][16 * CG + 1]) {
-  const int l = lane & 15, g = lane >> 4;
-  const unsigned chunks = (end - first + 127) / 128, share = (chunks + kWaves - 1) / kWaves;
-  const unsigned begin = first + 128 * share * (unsigned)wave;
-  unsigned stop = begin + 128 * share;
-  stop = stop < end ? stop : end;
-  v4f acc[RG][CG];
-#pragma unroll
-  for (int r = 0; r < RG; ++r)
-#pragma unroll
-    for (int c = 0; c < CG; ++c) acc[r][c] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-  if (begin < stop) {
-    Chunk<CG, RG, TERMS> one, two;
-    one.load(row, x, at, begin, stop, g, groups);
-    for (unsigned k = begin; k < stop; k += 256) {
-      two.load(row, x, at, k + 128, stop, g, groups);
-      one.multiply(acc, groups);
-      one.load(row, x, at, k + 256, stop, g, groups);
-      two.multiply(acc, groups);
-    }
-  }
-#pragma unroll
-  for (int r = 0; r < RG; ++r)
-#pragma unroll
-    for (int c = 0; c < CG; ++c)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) red[wave][16 * r + 4 * g + i][16 * c + l] = acc[r][c][i];
+#define SKL_MOE_READ(C, G, T)                                                                                                                                          \
+  if constexpr (CG == C && GROUPS == G && TERMS == T)                                                                                                                  \
+    asm volatile(SKL_MOE_RW##C SKL_MOE_RX##G##T "s_waitcnt lgkmcnt(0)" : SKL_MOE_N##G##T, SKL_MOE_W##C : SKL_MOE_OFFSETS, [px] "v"(px), [pw] "v"(pw) : "memory");
+#define SKL_MOE_EACH(F) \
+  F(1, 1, 1) F(2, 1, 1) F(1, 2, 1) F(2, 2, 1) F(1, 1, 3) F(2, 1, 3) F(1, 2, 3) F(2, 2, 3)
+template <int CG, int RG, int TERMS, int GROUPS, bool LAST>
+__device__ __forceinline__ void step(v4f (&acc)[RG][CG], const v4i (&x)[GROUPS][TERMS], const v8bf (&b)[CG], v4i (&n)[GROUPS][TERMS], v4i (&w)[CG], unsigned px, unsigned pw) {
+  constexpr int TERM = 16 * RG * 512;
+  SKL_MOE_EACH(SKL_MOE_STEP)
+}
+template <int CG, int RG, int TERMS, int GROUPS>
+__device__ __forceinline__ void read_first(v4i (&n)[GROUPS][TERMS], v4i (&w)[CG], unsigned px, unsigned pw) {
+  constexpr int TERM = 16 * RG * 512;
+  SKL_MOE_EACH(SKL_MOE_READ)
 }
 
-// h of 8 CG inner columns of one expert (blockIdx.y: its slot): CG / 2 groups of gate, as many of up.
+// What a wave's lanes hold of weights and tokens while they stream.
+template <class S>
+struct Operands {
+  const uint8_t *codes;          // the first row of weights that the wave requests
+  unsigned off[S::CG];           // the lane's offsets from there, requests of eight lines
+  const uint8_t *scales[S::CG];  // of the rows of weights that the lane multiplies
+  const uint16_t *tokens[S::TERMS];
+  unsigned at[S::RG];            // the lane's offsets from there: of request i, the pieces of row 2 (RG wave + i) + lane / 32
+};
+
+// The place of a token's 16-byte piece in its row of 32: reads of 16 rows with the same pieces meet in no bank (they are served rows 0 to 3 and 12 to 15 of one lane
+// group with rows 4 to 11 of the next).
+__device__ __forceinline__ unsigned turn_of(unsigned row) { return (row + 12u) & 15u; }
+template <class S>
+__device__ __forceinline__ unsigned row_of(int i, int wave, int lane) { return 2u * ((unsigned)wave * S::RG + i) + ((unsigned)lane >> 5); }
+__device__ __forceinline__ unsigned piece_of(unsigned row, int lane) { return ((unsigned)lane & 16u) | (((unsigned)lane ^ turn_of(row)) & 15u); }
+
+// acc[r][c] of the wave's rows of weights and its halves of the chunks in [begin, stop), `total` values in a row.
+template <class S, int GROUPS>
+__device__ __forceinline__ void multiply(const Operands<S> &o, v4f (&acc)[S::RG][S::CG], unsigned begin, unsigned stop, unsigned total, int wave, int lane, lds_char *stages) {
+  constexpr int CG = S::CG, RG = S::RG, TERMS = S::TERMS;
+  const int l = lane & 15, g = lane >> 4, pair = wave & 3, half = wave >> 2;
+  const unsigned per_row = total / 32, base = (unsigned)(uintptr_t)stages;
+  const unsigned piece = ((unsigned)lane & 7u) ^ ((unsigned)lane >> 3);  // of a line of weights: slot s of row r holds piece s ^ (r % 8)
+  const auto request_weights = [&](unsigned chunk) __attribute__((always_inline)) {
+    lds_char *const to = stages + (chunk - begin) % S::kWeightStages * S::kWeightBytes;
+    const unsigned byte = chunk * kLine;
+    const bool in = chunk < stop && byte + piece * 16u < total / 2;
+    const __amdgpu_buffer_rsrc_t w = __builtin_amdgcn_make_buffer_rsrc((void *)(o.codes + byte), 0, (int)kRange, 0x00027000);
+#pragma unroll
+    for (int i = 0; i < CG; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(w, (__attribute__((address_space(3))) void *)(to + (wave * CG + i) * 8 * kLine), 16, (int)(in ? o.off[i] : kOutside), 0, 0, 2);
+  };
+  const auto request_tokens = [&](unsigned chunk) __attribute__((always_inline)) {
+    lds_char *const to = stages + S::kTokensAt + (chunk - begin) % S::kTokenStages * S::kTokenBytes;
+#pragma unroll
+    for (int t = 0; t < TERMS; ++t) {
+      const __amdgpu_buffer_rsrc_t x = __builtin_amdgcn_make_buffer_rsrc((void *)(o.tokens[t] + chunk * kChunk), 0, (int)kRange, 0x00027000);
+#pragma unroll
+      for (int i = 0; i < RG; ++i) {
+        const bool there = chunk < stop && chunk * kChunk + 8u * piece_of(row_of<S>(i, wave, lane), lane) < total;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(x, (__attribute__((address_space(3))) void *)(to + t * (S::kTokenBytes / TERMS) + (wave * RG + i) * 1024), 16,
+                                                 (int)(there ? o.at[i] : kOutside), 0, 0, 0);
+      }
+    }
+  };
+  const auto request = [&](int chunk) __attribute__((always_inline)) {  // when chunk `chunk` has been read, counted from the first
+    if constexpr (S::kTokensFirst) request_tokens(begin + (unsigned)(chunk + S::kTokenStages));
+    request_weights(begin + (unsigned)(chunk + S::kWeightStages));
+    if constexpr (!S::kTokensFirst) request_tokens(begin + (unsigned)(chunk + S::kTokenStages));
+  };
+  // A row has four scale bytes in the half of a chunk. Lane group g loads those of the g-th of four chunks to come, from further down where the row ends - past its end they
+  // become zeros, like the codes. They are moved into place late: a use waits for the load.
+  const auto want_of = [&](unsigned chunk) { return (chunk + (unsigned)g) * 8u + 4u * (unsigned)half; };
+  const uint8_t *from[CG];
+  const auto load_scales = [&](unsigned (&s)[CG], unsigned chunk) __attribute__((always_inline)) {
+    const unsigned want = want_of(chunk), at = per_row < 4 ? 0u : want + 4 <= per_row ? want : per_row - 4;
+#pragma unroll
+    for (int c = 0; c < CG; ++c) s[c] = *(const __attribute__((address_space(1))) unsigned_any *)(from[c] + at);  // (not through a flat load, which a wait for LDS waits for)
+  };
+  const auto place_scales = [&](unsigned (&s)[CG], const unsigned (&v)[CG], unsigned chunk) __attribute__((always_inline)) {
+    const unsigned want = want_of(chunk), over = per_row < 4 || want + 4 <= per_row ? 0u : want >= per_row ? 32u : 8u * (want + 4 - per_row);
+#pragma unroll
+    for (int c = 0; c < CG; ++c) s[c] = over > 31 ? 0u : v[c] >> over;
+  };
+  unsigned raw[CG], ahead[CG], four[CG];  // scales of four chunks, of the next four
+#pragma unroll
+  for (int c = 0; c < CG; ++c) from[c] = o.scales[c];
+  if (per_row >= 4) {
+    load_scales(raw, begin);
+  } else {  // a row of one chunk, which is shorter than a load; what is loaded ahead of others is not used
+#pragma unroll
+    for (int c = 0; c < CG; ++c) {
+      raw[c] = 0;
+      for (unsigned i = 0; want_of(0) + i < per_row; ++i) raw[c] |= (unsigned)o.scales[c][want_of(0) + i] << (8 * i);
+      from[c] = o.codes;
+    }
+  }
+  load_scales(ahead, begin + 4);
+#pragma unroll
+  for (int c = 0; c < S::kWeightStages - S::kTokenStages; ++c) request_weights(begin + (unsigned)c);
+#pragma unroll
+  for (int c = 0; c < S::kTokenStages; ++c) request(c - S::kTokenStages);
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(S::kUnderWay + S::kLoads) : "memory");
+  __builtin_amdgcn_s_barrier();
+  const unsigned at_w = base + (pair * CG * 16 + l) * kLine + (unsigned)((4 * half + g) ^ (l & 7)) * 16u;
+  const unsigned at_x = base + S::kTokensAt + l * 512 + 256 * half + ((4u * g) ^ turn_of(l)) * 16u;
+  place_scales(four, raw, begin);
+  v4i w[CG], x0[GROUPS][TERMS], x1[GROUPS][TERMS];
+  read_first<CG, RG, TERMS, GROUPS>(x0, w, at_x, at_w);
+  unsigned at = 0, stage = 0;  // where the chunk's weights and tokens are in their rings
+#pragma unroll 1
+  for (unsigned chunk = begin; chunk < stop; ++chunk) {
+    const unsigned of = (chunk - begin) & 3u;
+    float f[CG];
+#pragma unroll
+    for (int c = 0; c < CG; ++c) {
+      const unsigned s = (unsigned)__builtin_amdgcn_ds_bpermute((int)(4 * l + 64 * of), (int)four[c]);  // the lane group's that has this chunk
+      f[c] = __uint_as_float(__builtin_amdgcn_ubfe(s, 8u * (unsigned)g, 8u) << 23);
+    }
+    const auto widen = [&](v8bf (&b)[CG], int j) __attribute__((always_inline)) {
+#pragma unroll
+      for (int c = 0; c < CG; ++c) b[c] = widen_f4((unsigned)w[c][j], f[c]);
+    };
+    v8bf b[CG];
+    v4i none[CG];
+    widen(b, 0);
+    step<CG, RG, TERMS, GROUPS, false>(acc, x0, b, x1, none, (at_x ^ 16u) + stage, 0);
+    widen(b, 1);
+    step<CG, RG, TERMS, GROUPS, false>(acc, x1, b, x0, none, (at_x ^ 32u) + stage, 0);
+    widen(b, 2);
+    step<CG, RG, TERMS, GROUPS, false>(acc, x0, b, x1, none, (at_x ^ 48u) + stage, 0);
+    widen(b, 3);
+    // Every wave has read all of this chunk; the next one is there once the requests of all waves for it are. Then this one's stage is free.
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(S::kUnderWay) : "memory");
+    __builtin_amdgcn_s_barrier();
+    if (of == 3) {
+      place_scales(four, ahead, chunk + 1);
+      load_scales(ahead, chunk + 5);
+    }
+    request((int)(chunk - begin));
+    __builtin_amdgcn_sched_barrier(0);
+    at = at == (S::kWeightStages - 1) * S::kWeightBytes ? 0 : at + S::kWeightBytes;
+    stage = stage == (S::kTokenStages - 1) * S::kTokenBytes ? 0 : stage + S::kTokenBytes;
+    step<CG, RG, TERMS, GROUPS, true>(acc, x1, b, x0, w, at_x + stage, at_w + at);
+  }
+#pragma unroll
+  for (int r = 0; r < GROUPS; ++r)
+#pragma unroll
+    for (int c = 0; c < CG; ++c) asm volatile("s_nop 15" : "+v"(acc[r][c]));  // the last products' results, before anything but a product reads them
+}
+
+// red[row of tokens][row of weights] = their products over k in [first, end), first a multiple of 256, `total` values in all.
+template <class S>
+__device__ __forceinline__ void stream(const Operands<S> &o, unsigned first, unsigned end, unsigned total, int wave, int lane, unsigned groups, char *lds) {
+  const int l = lane & 15, g = lane >> 4, pair = wave & 3, half = wave >> 2;
+  const unsigned begin = first / kChunk, stop = (end + kChunk - 1) / kChunk;
+  v4f acc[S::RG][S::CG];
+#pragma unroll
+  for (int r = 0; r < S::RG; ++r)
+#pragma unroll
+    for (int c = 0; c < S::CG; ++c) acc[r][c] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+  if (begin < stop) {  // the same for every wave
+    if (S::RG == 2 && groups > 1) multiply<S, S::RG>(o, acc, begin, stop, total, wave, lane, (lds_char *)lds);
+    else multiply<S, 1>(o, acc, begin, stop, total, wave, lane, (lds_char *)lds);
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the requests behind the last chunk write zeros into the rings
+  __syncthreads();
+  float(*red)[S::kPitch] = reinterpret_cast<float(*)[S::kPitch]>(lds);
+#pragma unroll
+  for (int turn = 0; turn < 2; ++turn) {
+    if (half == turn) {
+#pragma unroll
+      for (int r = 0; r < S::RG; ++r)
+#pragma unroll
+        for (int c = 0; c < S::CG; ++c)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float &to = red[16 * r + 4 * g + i][(pair * S::CG + c) * 16 + l];
+            to = turn ? to + acc[r][c][i] : acc[r][c][i];
+          }
+    }
+    __syncthreads();
+  }
+}
+
+// Rows of weights of one matrix from `row0` on, of which `rows` exist (others are the last one again: computed, not used): those that the lane requests, from `mine` on, and
+// those that it multiplies, from `part` on.
+template <class S>
+__device__ __forceinline__ void set_codes(Operands<S> &o, const skl_mx_operand &op, size_t expert, size_t row0, int rows, int mine, int lane) {
+  const int from = mine < rows ? mine : rows - 1;
+  const unsigned long long at = (unsigned long long)(uintptr_t)(op.codes + (expert + (row0 + from) * op.ld) / 2);
+  // spelled out as a scalar: a descriptor in vector registers costs a loop over the lanes per load
+  o.codes = (const uint8_t *)(uintptr_t)(((unsigned long long)(unsigned)__builtin_amdgcn_readfirstlane((int)(at >> 32)) << 32) | (unsigned)__builtin_amdgcn_readfirstlane((int)at));
+#pragma unroll
+  for (int i = 0; i < S::CG; ++i) {
+    const int r = mine + 8 * i + (lane >> 3);
+    o.off[i] = (unsigned)((r < rows ? r : rows - 1) - from) * (unsigned)(op.ld / 2) + (((unsigned)lane & 7u) ^ ((unsigned)lane >> 3)) * 16u;
+  }
+}
+template <class S>
+__device__ __forceinline__ void set_scales(Operands<S> &o, const skl_mx_operand &op, size_t expert, size_t row0, int rows, int part, int lane) {
+#pragma unroll
+  for (int c = 0; c < S::CG; ++c) {
+    const int r = part + 16 * c + (lane & 15);
+    o.scales[c] = op.scales + expert + (row0 + (r < rows ? r : rows - 1)) * op.lds;
+  }
+}
+// The lane's pieces of the rows of tokens that it requests: row n at of(i, n) elements from the first; rows from `count` on are not requested.
+template <class S, class F>
+__device__ __forceinline__ void set_tokens(Operands<S> &o, unsigned count, int wave, int lane, F of) {
+#pragma unroll
+  for (int i = 0; i < S::RG; ++i) {
+    const unsigned row = row_of<S>(i, wave, lane);
+    o.at[i] = row < count ? 2u * of(i, row) + 16u * piece_of(row, lane) : kOutside;
+  }
+}
+
+__device__ __forceinline__ Slot scalar(Slot s) {
+  return Slot{(unsigned)__builtin_amdgcn_readfirstlane((int)s.expert), (unsigned)__builtin_amdgcn_readfirstlane((int)s.first), (unsigned)__builtin_amdgcn_readfirstlane((int)s.count), 0};
+}
+
+// h of 32 CG inner columns of one expert (blockIdx.y: its slot): half of the rows of weights are rows of gate, half of up.
 template <int CG, int RG>
-__global__ void __launch_bounds__(kWaves * 64) moe_in_kernel(MoeArgs a) {
-  constexpr int kCols = 8 * CG;
-  __shared__ float red[kWaves][RG * 16][16 * CG + 1];
+__global__ void __launch_bounds__(kThreads) moe_in_kernel(MoeArgs a) {
+  using S = Shape<CG, RG, 1>;
+  constexpr int kCols = 32 * CG;
+  extern __shared__ __attribute__((aligned(1024))) char moe_lds[];
   const skl_moe_problem &p = a.p;
   const unsigned slot = blockIdx.y;
-  const Slot own = a.r.slots[slot];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const Slot own = scalar(a.r.slots[slot]);
   const unsigned active = *a.r.active;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, l = lane & 15;
+  unsigned token[RG];  // of the rows that the lane requests, in the first pass: asked for with the slot, not behind it
+#pragma unroll
+  for (int i = 0; i < RG; ++i) token[i] = a.r.tokens[slot * kMaxTokens + row_of<S>(i, wave, lane)];
   if (slot >= active) return;
-  Row row[CG];
-#pragma unroll
-  for (int c = 0; c < CG; ++c) {
-    const skl_mx_operand &op = c < CG / 2 ? p.gate : p.up;
-    const size_t col = (size_t)blockIdx.x * kCols + 16 * (c % (CG / 2)) + l;
-    row[c] = {op.codes + (own.expert * p.expert_in + col * op.ld) / 2, op.scales + own.expert * p.expert_in_scales + col * op.lds};
-  }
-  const uint16_t *const x[1] = {p.x};
+  const unsigned col0 = blockIdx.x * kCols, inter = (unsigned)p.inter, cols = inter - col0 < (unsigned)kCols ? inter - col0 : kCols;
+  Operands<S> o;
+  set_codes(o, wave < 4 ? p.gate : p.up, own.expert * p.expert_in, col0, (int)cols, wave % 4 * 8 * CG, lane);
+  set_scales(o, wave % 4 < 2 ? p.gate : p.up, own.expert * p.expert_in_scales, col0, (int)cols, wave % 2 * 16 * CG, lane);
+  o.tokens[0] = p.x;
   for (unsigned done = 0; done < own.count; done += RG * 16) {  // more tokens than a pass takes: the weights again
-    const unsigned left = own.count - done, here = left < RG * 16 ? left : RG * 16, groups = (here + 15) / 16;
-    unsigned at[RG];
+    const unsigned left = own.count - done, here = left < RG * 16 ? left : RG * 16;
+    if (done != 0) {
 #pragma unroll
-    for (int r = 0; r < RG; ++r) {
-      const unsigned i = 16u * r + l;
-      at[r] = (unsigned)(a.r.tokens[slot * kMaxTokens + done + (i < here ? i : here - 1)] * p.ldx);
+      for (int i = 0; i < RG; ++i) {
+        const unsigned row = row_of<S>(i, wave, lane);
+        token[i] = a.r.tokens[slot * kMaxTokens + done + (row < here ? row : 0)];
+      }
     }
-    stream<CG, RG, 1>(row, x, at, 0, (unsigned)p.hidden, wave, lane, groups, red);
-    __syncthreads();
-    for (unsigned n = threadIdx.x; n < here * kCols; n += kWaves * 64) {
+    set_tokens(o, here, wave, lane, [&](int i, unsigned) { return token[i] * (unsigned)p.ldx; });
+    stream<S>(o, 0, (unsigned)p.hidden, (unsigned)p.hidden, wave, lane, (here + 15) / 16, moe_lds);
+    const float(*red)[S::kPitch] = reinterpret_cast<const float(*)[S::kPitch]>(moe_lds);
+    for (unsigned n = threadIdx.x; n < here * kCols; n += kThreads) {
       const unsigned i = n / kCols, j = n % kCols;
-      float gv = red[0][i][j], uv = red[0][i][kCols + j];
-#pragma unroll
-      for (int w = 1; w < kWaves; ++w) gv += red[w][i][j], uv += red[w][i][kCols + j];
+      if (j >= cols) continue;
       const unsigned place = own.first + done + i;
-      const float h = skl_activate(gv, p.activation) * uv * a.r.weight[place];
+      const float h = skl_activate(red[i][j], p.activation) * red[i][kCols + j] * a.r.weight[place];
       const unsigned short t0 = bf16_of(h);
       const float rest = h - of_bf16(t0);
       const unsigned short t1 = bf16_of(rest);
-      const size_t to = (size_t)place * p.inter + (size_t)blockIdx.x * kCols + j;
+      const size_t to = (size_t)place * p.inter + col0 + j;
       a.r.h[0][to] = t0;
       a.r.h[1][to] = t1;
       a.r.h[2][to] = bf16_of(rest - of_bf16(t1));
@@ -368,69 +579,77 @@ __global__ void __launch_bounds__(kWaves * 64) moe_in_kernel(MoeArgs a) {
   }
 }
 
-// The output products of 64 columns, one expert (blockIdx.y) and a part of its inner columns (blockIdx.z); behind the last of a tile of columns
-// their sum for each token, in the order of its choices.
-constexpr int kOutCols = 64;
-template <int RG>
-__global__ void __launch_bounds__(kWaves * 64) moe_out_kernel(MoeArgs a) {
-  constexpr int CG = kOutCols / 16;
-  __shared__ float red[kWaves][RG * 16][kOutCols + 1];
-  __shared__ unsigned arrived;
+// The output products of 64 CG columns, one expert and one part of K.
+template <int CG, int RG>
+__global__ void __launch_bounds__(kThreads) moe_out_kernel(MoeArgs a) {
+  using S = Shape<CG, RG, 3>;
+  constexpr int kCols = S::kAll;
+  extern __shared__ __attribute__((aligned(1024))) char moe_lds[];
   const skl_moe_problem &p = a.p;
   const unsigned slot = blockIdx.y, split = blockIdx.z;
-  const Slot own = a.r.slots[slot];
+  const Slot own = scalar(a.r.slots[slot]);
   const unsigned active = *a.r.active;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, l = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   if (slot >= active) return;
-  const unsigned hidden = (unsigned)p.hidden, inter = (unsigned)p.inter, col0 = blockIdx.x * kOutCols;
-  const unsigned cols = hidden - col0 < kOutCols ? hidden - col0 : kOutCols;  // 32 or 64
-  const unsigned part = ((inter + a.r.out_splits - 1) / a.r.out_splits + 127) / 128 * 128;
-  const unsigned begin = split * part < inter ? split * part : inter, end = begin + part < inter ? begin + part : inter;
-  Row row[CG];
-#pragma unroll
-  for (int c = 0; c < CG; ++c) {
-    const unsigned j = 16u * c + l;
-    const size_t col = col0 + (j < cols ? j : cols - 1);
-    row[c] = {p.down.codes + (own.expert * p.expert_down + col * p.down.ld) / 2, p.down.scales + own.expert * p.expert_down_scales + col * p.down.lds};
-  }
+  const unsigned hidden = (unsigned)p.hidden, inter = (unsigned)p.inter, col0 = blockIdx.x * kCols, cols = hidden - col0 < (unsigned)kCols ? hidden - col0 : kCols;
+  const unsigned chunks = (inter + kChunk - 1) / kChunk;
+  const unsigned begin = chunks * split / a.r.out_splits * kChunk, stop = chunks * (split + 1) / a.r.out_splits * kChunk, end = stop < inter ? stop : inter;
+  Operands<S> o;
+  set_codes(o, p.down, own.expert * p.expert_down, col0, (int)cols, wave * 8 * CG, lane);
+  set_scales(o, p.down, own.expert * p.expert_down_scales, col0, (int)cols, wave % 4 * 16 * CG, lane);
   for (unsigned done = 0; done < own.count; done += RG * 16) {
-    const unsigned left = own.count - done, here = left < RG * 16 ? left : RG * 16, groups = (here + 15) / 16;
+    const unsigned left = own.count - done, here = left < RG * 16 ? left : RG * 16;
     const size_t place = own.first + done;
-    const uint16_t *const x[3] = {a.r.h[0] + place * inter, a.r.h[1] + place * inter, a.r.h[2] + place * inter};
-    unsigned at[RG];
 #pragma unroll
-    for (int r = 0; r < RG; ++r) at[r] = (16u * r + l < here ? 16u * r + l : here - 1) * inter;
-    stream<CG, RG, 3>(row, x, at, begin, end, wave, lane, groups, red);
-    __syncthreads();
-    for (unsigned n = threadIdx.x; n < here * kOutCols; n += kWaves * 64) {
-      const unsigned i = n / kOutCols, j = n % kOutCols;
-      float v = red[0][i][j];
-#pragma unroll
-      for (int w = 1; w < kWaves; ++w) v += red[w][i][j];
-      if (j < cols) leave(a.r.out + ((size_t)split * a.r.places + place + i) * hidden + col0 + j, v);
+    for (int t = 0; t < 3; ++t) o.tokens[t] = a.r.h[t] + place * inter;
+    set_tokens(o, here, wave, lane, [&](int, unsigned row) { return row * inter; });
+    stream<S>(o, begin, end, inter, wave, lane, (here + 15) / 16, moe_lds);
+    const float(*red)[S::kPitch] = reinterpret_cast<const float(*)[S::kPitch]>(moe_lds);
+    for (unsigned n = threadIdx.x; n < here * (kCols / 2); n += kThreads) {
+      const unsigned i = n / (kCols / 2), j = n % (kCols / 2) * 2;
+      if (j < cols) *reinterpret_cast<v2f *>(a.r.out + ((size_t)split * a.r.places + place + i) * hidden + col0 + j) = v2f{red[i][j], red[i][j + 1]};
     }
     __syncthreads();
   }
-  if (!arrives_last(a.r.counters + 1 + blockIdx.x, active * a.r.out_splits, &arrived)) return;
-  for (unsigned n = threadIdx.x; n < p.tokens * kOutCols; n += kWaves * 64) {
-    const unsigned t = n / kOutCols, j = n % kOutCols;
-    if (j >= cols) continue;
-    float v = 0.0f;
-    for (unsigned c = 0; c < p.top_k; ++c) {
-      const float *from = a.r.out + (size_t)a.r.place[t * p.top_k + c] * hidden + col0 + j;
-      for (unsigned s = 0; s < a.r.out_splits; ++s) v += found(from + (size_t)s * a.r.places * hidden);
+}
+
+// y: two columns of a token to a thread. (Left to the workgroup that is the last of its columns, this took 2 us more at 1 token, 5 at 7 and 35 at 64 tokens of 128 experts,
+// whose output products are 4 MiB.)
+__global__ void __launch_bounds__(256) moe_sum_kernel(MoeArgs a) {
+  const unsigned j = (blockIdx.x * 256u + threadIdx.x) * 2u;
+  if (j >= a.p.hidden) return;
+  const skl_moe_problem &p = a.p;
+  const unsigned t = blockIdx.y, terms = (unsigned)p.top_k * a.r.out_splits;
+  v2f v = {0.0f, 0.0f};
+  for (unsigned q = 0; q < terms; q += 8) {  // by choice, then by part of K; requested together
+    v2f part[8];
+#pragma unroll
+    for (unsigned i = 0; i < 8; ++i) {
+      const unsigned at = q + i < terms ? q + i : terms - 1, c = at / a.r.out_splits, s = at % a.r.out_splits;
+      part[i] = *reinterpret_cast<const v2f *>(a.r.out + ((size_t)s * a.r.places + a.r.place[t * p.top_k + c]) * p.hidden + j);
     }
-    if (p.residual) v = __fadd_rn(__fmul_rn(p.beta, p.residual[t * p.ld_residual + col0 + j]), v);
-    p.y[t * p.ldy + col0 + j] = v;
+#pragma unroll
+    for (unsigned i = 0; i < 8; ++i)
+      if (q + i < terms) v.x += part[i].x, v.y += part[i].y;
   }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) p.y[t * p.ldy + j + i] = p.residual ? __fadd_rn(__fmul_rn(p.beta, p.residual[t * p.ld_residual + j + i]), v[i]) : v[i];
 }
 
 inline size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 
-// Parts of K that give the output products of `slots` experts about four workgroups per compute unit; a part keeps a chunk for each wave.
-unsigned out_splits_for(const skl_moe_problem *p, unsigned slots) {
-  const size_t tiles = (p->hidden + kOutCols - 1) / kOutCols * slots, most = (p->inter + 128 * kWaves - 1) / (128 * kWaves);
-  const size_t want = (1024 + tiles - 1) / tiles;
+// Groups of 16 rows of weights per pair of waves: two, for fewer requests of tokens, where that leaves a workgroup per compute unit.
+int groups_for(size_t columns, size_t per_group, size_t slots) { return (columns + 2 * per_group - 1) / (2 * per_group) * slots >= 256 ? 2 : 1; }
+int in_groups(const skl_moe_problem *p, size_t slots) { return groups_for(p->inter, 32, slots); }
+int out_groups(const skl_moe_problem *p, size_t slots) { return groups_for(p->hidden, 64, slots); }
+
+// 32 tokens of an expert at a time where many experts have more than 16; below 8 each on average, 1 in 250 has, and its weights are read twice.
+int token_groups(const skl_moe_problem *p) { return p->tokens <= 16 || p->tokens * p->top_k <= 8 * p->experts ? 1 : 2; }
+
+// Parts of K that give the output products of `slots` experts as many workgroups as run at a time, of two chunks at least: 4 tokens, 2 of 8 x 14336, 65 us without, 53 with.
+unsigned out_splits_for(const skl_moe_problem *p, size_t slots) {
+  const size_t cols = 64 * (size_t)out_groups(p, slots), tiles = (p->hidden + cols - 1) / cols * slots, most = (p->inter + 2 * kChunk - 1) / (2 * kChunk);
+  const size_t want = ((token_groups(p) == 1 ? 512 : 256) + tiles - 1) / tiles;
   return (unsigned)(want < 1 ? 1 : want < most ? want : most);
 }
 
@@ -445,7 +664,7 @@ size_t lay_out(const skl_moe_problem *p, char *base, Routing *r) {
   };
   r->places = (unsigned)places;
   r->router_splits = (unsigned)((p->hidden + 511) / 512);
-  r->out_splits = out_splits_for(p, (unsigned)slots);
+  r->out_splits = out_splits_for(p, slots);
   r->parts = reinterpret_cast<float *>(take((size_t)r->router_splits * p->tokens * p->experts * 4));
   r->active = reinterpret_cast<unsigned *>(take(4));
   r->slots = reinterpret_cast<Slot *>(take(slots * sizeof(Slot)));
@@ -457,24 +676,38 @@ size_t lay_out(const skl_moe_problem *p, char *base, Routing *r) {
   return at;
 }
 
-size_t counters_of(const skl_moe_problem *p) { return 1 + (p->hidden + kOutCols - 1) / kOutCols; }
-
+template <class S>
+int launch_as(void (*kernel)(MoeArgs), const MoeArgs &a, dim3 grid, std::atomic<bool> &done, const char *what) {
+  if (!done.load(std::memory_order_acquire)) {  // racing threads set the same value
+    const int rc = skl_check_hip(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, S::kLds), what);
+    if (rc != 0) return rc;
+    done.store(true, std::memory_order_release);
+  }
+  kernel<<<grid, kThreads, S::kLds, skl_current_stream()>>>(a);
+  return skl_check_launch(what);
+}
+template <int CG, int RG>
+int launch_in(const MoeArgs &a, unsigned slots) {
+  static std::atomic<bool> done{false};
+  return launch_as<Shape<CG, RG, 1>>(moe_in_kernel<CG, RG>, a, dim3(skl_div_up(a.p.inter, 32 * CG), slots), done, "moe_in");
+}
+template <int CG, int RG>
+int launch_out(const MoeArgs &a, unsigned slots) {
+  static std::atomic<bool> done{false};
+  return launch_as<Shape<CG, RG, 3>>(moe_out_kernel<CG, RG>, a, dim3(skl_div_up(a.p.hidden, 64 * CG), slots, a.r.out_splits), done, "moe_out");
+}
 template <int RG>
-int launch_products(const MoeArgs &a, unsigned slots, hipStream_t st) {
-  // 32 inner columns per workgroup where that leaves one for every compute unit twice, else 16
-  const unsigned wide = (unsigned)(a.p.inter / 32);
-  if (wide * slots >= 512) moe_in_kernel<4, RG><<<dim3(wide, slots), kWaves * 64, 0, st>>>(a);
-  else moe_in_kernel<2, RG><<<dim3(2 * wide, slots), kWaves * 64, 0, st>>>(a);
-  const int rc = skl_check_launch("moe_in");
+int launch_products(const MoeArgs &a, unsigned slots) {
+  const int in = in_groups(&a.p, slots), out = out_groups(&a.p, slots);
+  const int rc = in == 2 ? launch_in<2, RG>(a, slots) : launch_in<1, RG>(a, slots);
   if (rc != 0) return rc;
-  moe_out_kernel<RG><<<dim3(skl_div_up(a.p.hidden, kOutCols), slots, a.r.out_splits), kWaves * 64, 0, st>>>(a);
-  return skl_check_launch("moe_out");
+  return out == 2 ? launch_out<2, RG>(a, slots) : launch_out<1, RG>(a, slots);
 }
 
-int launch_on(const skl_moe_problem *p, char *block, unsigned *counters) {
+int launch_on(const skl_moe_problem *p, char *block, unsigned *counter) {
   MoeArgs a = {*p, {}};
   lay_out(p, block, &a.r);
-  a.r.counters = counters;
+  a.r.counter = counter;
   const unsigned slots = (unsigned)(p->experts < a.r.places ? p->experts : a.r.places);
   hipStream_t st = skl_current_stream();
   const dim3 grid(skl_div_up(p->experts, 16), skl_div_up(p->tokens, 16), a.r.router_splits);
@@ -484,24 +717,27 @@ int launch_on(const skl_moe_problem *p, char *block, unsigned *counters) {
   else moe_router_kernel<16><<<grid, kRouterThreads, 0, st>>>(a);
   const int rc = skl_check_launch("moe_router");
   if (rc != 0) return rc;
-  return p->tokens <= 16 ? launch_products<1>(a, slots, st) : launch_products<2>(a, slots, st);
+  const int done = token_groups(p) == 1 ? launch_products<1>(a, slots) : launch_products<2>(a, slots);
+  if (done != 0) return done;
+  moe_sum_kernel<<<dim3(skl_div_up(p->hidden, 512), (unsigned)p->tokens), 256, 0, st>>>(a);
+  return skl_check_launch("moe_sum");
 }
 
 }  // namespace
 
 extern "C" int skl_hip_launch_moe(const skl_moe_problem *p) {
   Routing r;
-  const size_t bytes = lay_out(p, nullptr, &r), counters = counters_of(p) * sizeof(unsigned);
+  const size_t bytes = lay_out(p, nullptr, &r), zero = sizeof(unsigned);
   const int pending = skl_hip_pending_error();
   int rc;
   skl_hip_sequence_begin();  // the launches hand data on through the stream's scratch memory
   char *block = static_cast<char *>(skl_hip_operand_scratch(bytes));
-  unsigned *zeroed = block ? static_cast<unsigned *>(skl_hip_zeroed_sums(counters)) : nullptr;
+  unsigned *zeroed = block ? static_cast<unsigned *>(skl_hip_zeroed_sums(zero)) : nullptr;
   char *own = nullptr;
   if (!block || !zeroed) {
     // a stream without scratch memory, or no room for it: a block for this call alone, released once the stream has drained
-    own = static_cast<char *>(skl_hip_malloc(bytes + counters));
-    if (own && skl_hip_memset(own + bytes, 0, counters) != 0) {
+    own = static_cast<char *>(skl_hip_malloc(bytes + zero));
+    if (own && skl_hip_memset(own + bytes, 0, zero) != 0) {
       skl_hip_free(own);
       own = nullptr;
     }
