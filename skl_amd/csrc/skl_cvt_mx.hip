@@ -7,9 +7,11 @@
 // values (v_cvt_scalef32_pk_fp4_f32 / _bf16: to nearest even, saturating).
 //
 // All of it is bound by memory. Rows that are contiguous (or any others, value by value): four lanes hold a block, eight values of
-// 16 (bf16) or 32 bytes each, and meet in two exchanges between neighbours; a lane's codes are a dword. Columns (contiguous across the rows of the
-// result): a lane holds two neighbouring rows of a block of 32 k, whose loads - 32, each a whole line or two per wave - are all under way
-// together; the codes go through LDS, where 256 k of a row become a whole line.
+// 16 (bf16) or 32 bytes each, and meet in two exchanges between neighbours; a lane's codes are a dword. 8192 x 8192 fp32: 66 us,
+// 4.6 TB/s; 2048 x 8192 bf16 12.9. Columns (contiguous across the rows of the result): a lane holds two neighbouring rows of a block
+// of 32 k, whose loads - 32, each a whole line or two per wave - are all under way together; the codes go through LDS, where 256 k of
+// a row become a whole line. 4096 x 11008 bf16: 33 us, 3.5 TB/s, 2048 x 2048 6.3 (with two blocks to a wave, one after the other,
+// 9.0); the order of the workgroups and four rows to a lane changed nothing. The way back, 4096 x 11008 to bf16: 18 us, 6.3 TB/s.
 #include <hip/hip_runtime.h>
 
 #include "skl_device.hpp"
@@ -145,8 +147,8 @@ __global__ void __launch_bounds__(256) cvt_to_mx_rows_kernel(const typename Eigh
   }
 }
 
-// Columns: rs == 1. A workgroup takes 128 rows of the result and 256 k of each, a wave two of the eight blocks.
-constexpr int kAcrossRows = 128, kAcrossK = 256, kAcrossPitch = 144;  // bytes of a row in LDS: 16 more than it holds, against bank conflicts
+// Columns: rs == 1. A workgroup takes 128 rows of the result and 256 k of each, a wave one of the eight blocks.
+constexpr int kAcrossThreads = 512, kAcrossRows = 128, kAcrossK = 256, kAcrossPitch = 144;  // bytes of a row in LDS: 16 more than it holds, against bank conflicts
 
 template <class T>
 struct PairOfRows;
@@ -202,46 +204,42 @@ struct PairOfRows<float> {
 };
 
 template <class T>
-__global__ void __launch_bounds__(256) cvt_to_mx_columns_kernel(const T *__restrict__ src, size_t cs, size_t m, size_t k, uint8_t *__restrict__ dst,
+__global__ void __launch_bounds__(kAcrossThreads) cvt_to_mx_columns_kernel(const T *__restrict__ src, size_t cs, size_t m, size_t k, uint8_t *__restrict__ dst,
                                                                 size_t row_bytes, uint8_t *__restrict__ scales, size_t lds) {
   __shared__ __attribute__((aligned(16))) uint8_t lines[kAcrossRows * kAcrossPitch];
-  __shared__ uint8_t bytes[kAcrossRows][8];
+  __shared__ __attribute__((aligned(8))) uint8_t bytes[kAcrossRows][8];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const size_t row0 = (size_t)blockIdx.y * kAcrossRows, k0 = (size_t)blockIdx.x * kAcrossK;
   const size_t row = row0 + 2 * (size_t)lane;
   const bool one = row < m, two = row + 1 < m;
+  const size_t kb = k0 + 32 * (size_t)wave;
+  PairOfRows<T> v;
+  const T *p = src + row;
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int block = 2 * wave + j;
-    const size_t kb = k0 + 32 * (size_t)block;
-    PairOfRows<T> v;
-    const T *p = src + row;
-#pragma unroll
-    for (int i = 0; i < 32; ++i) {
-      if (one && kb + i < k) v.load(i, p + (kb + i) * cs, two);
-      else v.clear(i);
-    }
-    unsigned m0, m1;
-    v.largest(m0, m1);
-    const unsigned s0 = scale_byte(m0), s1 = scale_byte(m1);
-    const float f0 = __uint_as_float(s0 << 23), f1 = __uint_as_float(s1 << 23);
-    u4 c0, c1;
-#pragma unroll
-    for (int at = 0; at < 4; ++at) {
-      c0[at] = s0 == 255u ? 0u : v.template codes<0>(at, f0);
-      c1[at] = s1 == 255u ? 0u : v.template codes<1>(at, f1);
-    }
-    *reinterpret_cast<u4 *>(lines + (2 * lane) * kAcrossPitch + 16 * block) = c0;
-    *reinterpret_cast<u4 *>(lines + (2 * lane + 1) * kAcrossPitch + 16 * block) = c1;
-    bytes[2 * lane][block] = (uint8_t)s0;
-    bytes[2 * lane + 1][block] = (uint8_t)s1;
+  for (int i = 0; i < 32; ++i) {
+    if (one && kb + i < k) v.load(i, p + (kb + i) * cs, two);
+    else v.clear(i);
   }
+  unsigned m0, m1;
+  v.largest(m0, m1);
+  const unsigned s0 = scale_byte(m0), s1 = scale_byte(m1);
+  const float f0 = __uint_as_float(s0 << 23), f1 = __uint_as_float(s1 << 23);
+  u4 c0, c1;
+#pragma unroll
+  for (int at = 0; at < 4; ++at) {
+    c0[at] = s0 == 255u ? 0u : v.template codes<0>(at, f0);
+    c1[at] = s1 == 255u ? 0u : v.template codes<1>(at, f1);
+  }
+  *reinterpret_cast<u4 *>(lines + (2 * lane) * kAcrossPitch + 16 * wave) = c0;
+  *reinterpret_cast<u4 *>(lines + (2 * lane + 1) * kAcrossPitch + 16 * wave) = c1;
+  bytes[2 * lane][wave] = (uint8_t)s0;
+  bytes[2 * lane + 1][wave] = (uint8_t)s1;
   __syncthreads();
   const size_t rows = m - row0 < (size_t)kAcrossRows ? m - row0 : (size_t)kAcrossRows;
   const size_t left = k - k0;  // values from here on
 #pragma unroll
-  for (int pass = 0; pass < 4; ++pass) {
-    const unsigned r = 32u * pass + (threadIdx.x >> 3), piece = threadIdx.x & 7u;
+  for (int pass = 0; pass < 2; ++pass) {
+    const unsigned r = 64u * pass + (threadIdx.x >> 3), piece = threadIdx.x & 7u;
     if (r >= rows || 32 * (size_t)piece >= left) continue;
     uint8_t *to = dst + (row0 + r) * row_bytes + k0 / 2 + 16 * piece;
     const uint8_t *from = lines + r * kAcrossPitch + 16 * piece;
@@ -252,7 +250,12 @@ __global__ void __launch_bounds__(256) cvt_to_mx_columns_kernel(const T *__restr
       for (size_t i = 0; 32 * (size_t)piece + 2 * i < left; ++i) to[i] = from[i];
     }
   }
-  for (unsigned at = threadIdx.x; at < kAcrossRows * 8u; at += 256u) {
+  if (left >= (size_t)kAcrossK) {
+    typedef u2 u2a1 __attribute__((aligned(1)));
+    if (threadIdx.x < rows) *reinterpret_cast<u2a1 *>(scales + (row0 + threadIdx.x) * lds + k0 / 32) = *reinterpret_cast<const u2 *>(bytes[threadIdx.x]);
+    return;
+  }
+  for (unsigned at = threadIdx.x; at < kAcrossRows * 8u; at += kAcrossThreads) {
     const unsigned r = at >> 3, block = at & 7u;
     if (r < rows && 32 * (size_t)block < left) scales[(row0 + r) * lds + k0 / 32 + block] = bytes[r][block];
   }
@@ -377,7 +380,7 @@ int launch_columns(size_t m, size_t k, const T *src, size_t cs, uint8_t *codes, 
   }
   for (size_t i = 0; i < m; i += most) {
     const size_t here = m - i < most ? m - i : most;
-    cvt_to_mx_columns_kernel<T><<<dim3((unsigned)gx, skl_div_up(here, kAcrossRows)), 256, 0, skl_current_stream()>>>(
+    cvt_to_mx_columns_kernel<T><<<dim3((unsigned)gx, skl_div_up(here, kAcrossRows)), kAcrossThreads, 0, skl_current_stream()>>>(
         src + i, cs, here, k, codes + i * (ld / 2), ld / 2, scales + i * lds, lds);
     const int rc = skl_check_launch("cvt_to_mx_columns");
     if (rc != 0) return rc;

@@ -125,9 +125,9 @@ constexpr int kRowPitch = 32 * TN * 4 + 16;  // 16 bytes more, so that 16 lanes 
 template <int TN>
 constexpr int kRowSpace = 32 * kRowPitch<TN>;
 
-enum { kThrough, kPast, kRead, kAny };  // stored through the caches or past them; read first; any strides, columns that do not exist
+enum { kThrough, kPast, kRead, kAny };  // stored through the caches or past them; read first; any strides. EDGE: columns that do not exist
 
-template <int HOW, int TM, int TN>
+template <int HOW, bool EDGE, int TM, int TN>
 __device__ __forceinline__ void write_rows(const MxArgs &p, const v16f (&sum)[TN][TM], unsigned row0, unsigned col0, unsigned rows, unsigned cols, int lane, char *space) {
   const int l = lane & 31, half = lane >> 5;
   constexpr int kLanes = 8 * TN, kRowsAt = 64 / kLanes, kPasses = 32 / kRowsAt;  // lanes that hold a row, rows of a pass, passes per row of blocks
@@ -162,7 +162,13 @@ __device__ __forceinline__ void write_rows(const MxArgs &p, const v16f (&sum)[TN
 #pragma unroll
           for (int n = 0; n < kBatch; ++n) {
             const unsigned r = 32u * i + (unsigned)(n0 + n) * kRowsAt;
-            old[n] = *reinterpret_cast<const v4f_any *>(r + at_row < rows ? first + (size_t)r * p.rsc : first);
+            const float *const there = r + at_row < rows ? first + (size_t)r * p.rsc : first;
+            if (EDGE && at_col + 4 > cols) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) old[n][e] = at_col + e < cols ? there[e] : 0.0f;
+            } else {
+              old[n] = *reinterpret_cast<const v4f_any *>(there);
+            }
           }
         }
 #pragma unroll
@@ -176,6 +182,12 @@ __device__ __forceinline__ void write_rows(const MxArgs &p, const v16f (&sum)[TN
                                 : skl_combine(v[e], old[n][e], p.alpha, p.beta);
           if (r + at_row >= rows) continue;
           float *const to = first + (size_t)r * p.rsc;
+          if (EDGE && at_col + 4 > cols) {
+#pragma unroll
+            for (int e = 0; e < 3; ++e)
+              if (at_col + e < cols) to[e] = v[e];
+            continue;
+          }
           if constexpr (HOW == kPast) asm volatile("global_store_dwordx4 %0, %1, off nt" ::"v"(to), "v"(v) : "memory");  // (the compiler makes one of two branches that differ in this alone)
           else *reinterpret_cast<v4f_any *>(to) = v;
         }
@@ -201,10 +213,14 @@ __device__ __forceinline__ void write_c(const MxArgs &p, const v16f (&sum)[TN][T
     read_c = __any(needs);
   }
   row0 += wave_row, col0 += wave_col, rows -= wave_row, cols -= wave_col;
-  if (p.csc != 1 || cols < 32u * TN) write_rows<kAny, TM, TN>(p, sum, row0, col0, rows, cols, lane, space);
-  else if (read_c) write_rows<kRead, TM, TN>(p, sum, row0, col0, rows, cols, lane, space);
-  else if (p.past_caches) write_rows<kPast, TM, TN>(p, sum, row0, col0, rows, cols, lane, space);
-  else write_rows<kThrough, TM, TN>(p, sum, row0, col0, rows, cols, lane, space);
+  // (Columns that do not exist, value by value through kAny, made 2816 x 5000 x 7168 14 us slower than 2816 x 5120 x 7168.)
+  const bool edge = cols < 32u * TN;
+  if (p.csc != 1) write_rows<kAny, true, TM, TN>(p, sum, row0, col0, rows, cols, lane, space);
+  else if (read_c && edge) write_rows<kRead, true, TM, TN>(p, sum, row0, col0, rows, cols, lane, space);
+  else if (read_c) write_rows<kRead, false, TM, TN>(p, sum, row0, col0, rows, cols, lane, space);
+  else if (edge) write_rows<kThrough, true, TM, TN>(p, sum, row0, col0, rows, cols, lane, space);
+  else if (p.past_caches) write_rows<kPast, false, TM, TN>(p, sum, row0, col0, rows, cols, lane, space);
+  else write_rows<kThrough, false, TM, TN>(p, sum, row0, col0, rows, cols, lane, space);
 }
 
 // Any layout: 64 x 64 tiles of four waves, one block of 32 x 32 each, operands through registers.
@@ -936,6 +952,7 @@ struct PadJob {
   size_t from_row;   // bytes
   size_t rows;       // 0: nothing to copy
   unsigned words;    // of 16 bytes in a row of the copy
+  unsigned lanes_log;  // threads to a row
   unsigned bytes;    // of a row that exist; the rest are `fill`
   unsigned last_mask;  // of its last byte's bits
   unsigned fill;
@@ -943,36 +960,51 @@ struct PadJob {
 struct PadJobs {
   PadJob job[4];
 };
+// 16 bytes of a row from `at` on. A row's end is loaded from further down and moved into place: a load in a branch of its own would be waited for there.
+__device__ __forceinline__ unsigned word_from(const PadJob &p, unsigned at) { return p.bytes < 16 ? 0u : at + 16 <= p.bytes ? at : p.bytes - 16; }
+__device__ __forceinline__ v4i load_word(const PadJob &p, const uint8_t *row, unsigned from) {
+  if (p.bytes >= 16) return *reinterpret_cast<const v4i_any *>(row + from);
+  v4i v = {0, 0, 0, 0};
+  for (unsigned b = 0; b < p.bytes; ++b) v[b >> 2] |= (int)((unsigned)row[b] << (8 * (b & 3u)));
+  return v;
+}
+__device__ __forceinline__ v4i padded_word(const PadJob &p, v4i v, unsigned at, unsigned from) {
+  if (at + 16 < p.bytes) return v;
+  typedef unsigned __int128 u128;
+  const unsigned over = at - from, have = at < p.bytes ? p.bytes - at : 0u;
+  u128 bits = over < 16 ? __builtin_bit_cast(u128, v) >> (8 * over) : (u128)0;
+  u128 fill = (u128)(p.fill * 0x0101010101010101ull);
+  fill |= fill << 64;
+  const u128 kept = have >= 16 ? ~(u128)0 : ((u128)1 << (8 * have)) - 1;
+  bits = (bits & kept) | (fill & ~kept);
+  if (have != 0) bits &= ~((u128)(p.last_mask ^ 255u) << (8 * (have - 1)));
+  return __builtin_bit_cast(v4i, bits);
+}
+constexpr int kPadRows = 4;  // a thread's loads under way
 __global__ void __launch_bounds__(256) mx_pad_kernel(PadJobs jobs) {
   const PadJob &p = jobs.job[blockIdx.y];
-  const size_t all = p.rows * p.words;
-  for (size_t n = (size_t)blockIdx.x * 256 + threadIdx.x; n < all; n += (size_t)gridDim.x * 256) {
-    const size_t row = n / p.words;
-    const unsigned at = 16 * (unsigned)(n - row * p.words);
-    const uint8_t *from = p.from + row * p.from_row + at;
-    v4i v;
-    if (at + 16 < p.bytes) {
-      v = *reinterpret_cast<const v4i_any *>(from);
-    } else {
+  const unsigned each = 256u >> p.lanes_log, lane = threadIdx.x & ((1u << p.lanes_log) - 1u);  // rows at a time
+  const size_t step = (size_t)gridDim.x * each;
+  for (size_t first = (size_t)blockIdx.x * each + (threadIdx.x >> p.lanes_log); first < p.rows; first += kPadRows * step)
+    for (unsigned word = lane; word < p.words; word += 1u << p.lanes_log) {
+      const unsigned from = word_from(p, 16 * word);
+      v4i v[kPadRows];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        unsigned u = 0;
-        for (unsigned b = 0; b < 4; ++b) {
-          const unsigned k = at + 4 * i + b;
-          const unsigned byte = k + 1 < p.bytes ? from[4 * i + b] : k + 1 == p.bytes ? from[4 * i + b] & p.last_mask : p.fill;
-          u |= byte << (8 * b);
-        }
-        v[i] = (int)u;
+      for (int i = 0; i < kPadRows; ++i) {
+        const size_t row = first + i * step;
+        v[i] = load_word(p, p.from + (row < p.rows ? row : first) * p.from_row, from);
       }
+#pragma unroll
+      for (int i = 0; i < kPadRows; ++i)
+        if (const size_t row = first + i * step; row < p.rows) reinterpret_cast<v4i *>(p.to)[row * p.words + word] = padded_word(p, v[i], 16 * word, from);
     }
-    *reinterpret_cast<v4i *>(p.to + 16 * n) = v;
-  }
 }
 
 // Rows that loads to LDS read: on 4-byte boundaries, a tile's offsets 31-bit numbers.
-bool lines_ok(const uint8_t *first, size_t pitch) { return ((uintptr_t)first & 3) == 0 && (pitch & 3) == 0 && pitch <= ((size_t)1 << 22); }
+bool rows_ok(const uint8_t *first, size_t pitch) { return ((uintptr_t)first & 3) == 0 && (pitch & 3) == 0 && pitch <= ((size_t)1 << 22); }
+bool on_lines(const uint8_t *first, size_t pitch) { return rows_ok(first, pitch) && ((uintptr_t)first & (kLine - 1)) == 0 && (pitch & (kLine - 1)) == 0; }
 // ... and scales, 16 bytes at a time.
-bool scales_ok(const uint8_t *first, size_t pitch, size_t k) { return lines_ok(first, pitch) && ((k + 31) / 32) % 16 == 0; }
+bool scales_ok(const uint8_t *first, size_t pitch, size_t k) { return rows_ok(first, pitch) && ((k + 31) / 32) % 16 == 0; }
 
 size_t up(size_t v, size_t to) { return (v + to - 1) / to * to; }
 
@@ -1105,17 +1137,21 @@ extern "C" int skl_hip_launch_gemm_mx(const skl_mx_gemm *g) {
   p.past_caches = g->m * g->n >= ((size_t)48 << 20);
   if (p.k == 0 || p.k > ((size_t)1 << 26)) return launch_any(p);
   const Kind kind = kind_of(p);
-  // Operands in rows that the kernel does not read are copied first.
+  // Operands in rows that the kernel does not read are copied first; for large tiles also those whose rows do not begin on lines, as every request of theirs takes a line
+  // more (us with and without the copy: 3000 x 5000 x 7000 76 / 85, 2048 x 4096 x 4112 36 / 41, 2048 x 2048 x 3000 24 / 26, 8192 x 8192 x 3000 175 / 205).
   const unsigned exist = (unsigned)((p.k + 1) / 2), blocks = (unsigned)((p.k + 31) / 32), mask = p.k % 2 ? 15u : 255u;
   PadJobs jobs = {};
   const uint8_t **first[4] = {&p.a, &p.b, &p.sa, &p.sb};
   size_t *pitch[4] = {&p.a_row, &p.b_col, &p.sa_row, &p.sb_col}, bytes = 0, most = 0;
   for (int i = 0; i < 4; ++i) {
-    if (i < 2 ? lines_ok(*first[i], *pitch[i]) : kind > kWide2 || scales_ok(*first[i], *pitch[i], p.k)) continue;
-    const unsigned row = i < 2 ? blocks * 16 : (unsigned)up(blocks, 16);
-    jobs.job[i] = {*first[i], nullptr, *pitch[i], i % 2 ? p.n : p.m, row / 16, i < 2 ? exist : blocks, i < 2 ? mask : 255u, i < 2 ? 0u : 127u};
+    if (i < 2 ? (kind <= kWide2 ? on_lines(*first[i], *pitch[i]) : rows_ok(*first[i], *pitch[i])) : kind > kWide2 || scales_ok(*first[i], *pitch[i], p.k)) continue;
+    const unsigned row = i < 2 ? (unsigned)up(blocks * 16, kLine) : (unsigned)up(blocks, 16);
+    unsigned lanes_log = 0;
+    while (lanes_log < 8 && (16u << lanes_log) < row) ++lanes_log;
+    jobs.job[i] = {*first[i], nullptr, *pitch[i], i % 2 ? p.n : p.m, row / 16, lanes_log, i < 2 ? exist : blocks, i < 2 ? mask : 255u, i < 2 ? 0u : 127u};
     bytes += up(jobs.job[i].rows * row, 256);
-    most = jobs.job[i].rows * jobs.job[i].words > most ? jobs.job[i].rows * jobs.job[i].words : most;
+    const size_t grid = (jobs.job[i].rows << lanes_log) / (256 * kPadRows) + 1;
+    most = grid > most ? grid : most;
   }
   if (bytes == 0) return launch_kind(p, kind);
   const int pending = skl_hip_pending_error();
@@ -1130,8 +1166,7 @@ extern "C" int skl_hip_launch_gemm_mx(const skl_mx_gemm *g) {
         block += up(j.rows * j.words * 16, 256);
       }
     if (jobs.job[0].rows != 0 && jobs.job[1].rows != 0) p.k = (size_t)blocks * 32;  // both filled up with zeros
-    const size_t grid = (most + 255) / 256;
-    mx_pad_kernel<<<dim3((unsigned)(grid < 4096 ? grid : 4096), 4), 256, 0, skl_current_stream()>>>(jobs);
+    mx_pad_kernel<<<dim3((unsigned)(most < 4096 ? most : 4096), 4), 256, 0, skl_current_stream()>>>(jobs);
     rc = skl_check_launch("mx_pad");
     if (rc == 0) rc = launch_kind(p, kind);
   } else {
