@@ -409,7 +409,8 @@ void skl_cvt_f32rc_mxf4e2m1_gfx950(size_t m, size_t k, const float *src, size_t 
                                    uint8_t *scales, size_t lds);
 void skl_cvt_bf16rc_mxf4e2m1_gfx950(size_t m, size_t k, const skl_bf16_t *src, size_t rs, size_t cs, uint8_t *dst, size_t ldd,
                                     uint8_t *scales, size_t lds);
-/* The way back, exact for every scale byte: f32 and bf16 hold each of these values (the smallest is 2^-128, subnormal in both).
+/* The way back, exact: f32 and bf16 hold each of these values (the smallest is 2^-128, subnormal in both) but those of 2^128 and more, from
+ * scale bytes 253 and 254, which become infinities.
  * Element (i, p) of the result at dst[i * rs + p * cs]. */
 void skl_cvt_mxf4e2m1_f32rc_gfx950(size_t m, size_t k, const uint8_t *src, size_t ldsrc, const uint8_t *scales, size_t lds,
                                    float *dst, size_t rs, size_t cs);
@@ -441,13 +442,14 @@ void skl_gemm_mxf4e2m1r_mxf4e2m1c_f32rc_gfx950(size_t m, size_t n, size_t k, flo
  *   w_j = exp(l_j - max l) / sum exp(l - max l), the sum over the chosen ones (normalise != 0) or over all experts
  *   h_j = act(x gate_j^T) * (x up_j^T)                                    `inter` values, gate and up of expert j: inter x hidden
  *   y   = beta * residual + sum_j w_j * (h_j down_j^T)                    `hidden` values, down: hidden x inter
- * X, the logits' and all further products and sums are exact products summed in fp32; h, times its w, is held as the sum of two bf16
- * values (16 bits of significand, the error of a sum of a few hundred fp32 products), nothing else is rounded to fewer bits. Every sum's order depends
+ * X, the logits' and all further products and sums are exact products summed in fp32; h, times its w, is held as the sum of three bf16
+ * values, which is all of its 24 bits, and nothing is rounded to fewer. Weights are widened to bf16, exactly, for every scale byte from 0 on; one of 2^128 or
+ * more (scale bytes 253 and 254) makes an infinity or a NaN of what it enters, a block with the byte 255 a NaN. Every sum's order depends
  * on the sizes and on who was chosen alone: the same call gives the same bits.
  * residual may be y (each with its own row distance), or NULL with beta == 0, where it is not read. Made for a few tokens: the weights are read once for up to 64
  * tokens, and again for each further 64.
- * hidden and inter are multiples of 32; experts <= 1024, top_k <= experts, top_k <= 64; every row of weights and of X begins on a
- * 16-byte boundary (pointers and distances); anything else is SKL_HIP_ERR_BAD_ARGUMENT, and nothing is done. */
+ * hidden and inter are multiples of 32 and at most 2^24; experts <= 1024, top_k <= experts, top_k <= 64; every row of weights, of the router and of X begins on a
+ * 16-byte boundary (pointers and distances); ld_in and ld_down are at most 2^24, ldx at most 2^23; anything else is SKL_HIP_ERR_BAD_ARGUMENT, and nothing is done. */
 typedef struct skl_gfx950_moe {
   size_t hidden, inter, experts, top_k;
   const skl_bf16_t *router; /* experts x hidden, rows ld_router apart */

@@ -755,7 +755,10 @@ extern "C" int skl_hip_launch_moe(const skl_moe_problem *p) {
   if (own) {
     skl_hip_synchronize();
     skl_hip_free(own);
-    if (rc == 0 && pending != SKL_HIP_ERR_WORKSPACE) skl_hip_withdraw_error(SKL_HIP_ERR_WORKSPACE);
+    if (rc == 0) {  // nothing is missing
+      if (pending != SKL_HIP_ERR_WORKSPACE) skl_hip_withdraw_error(SKL_HIP_ERR_WORKSPACE);
+      if (pending != SKL_HIP_ERR_STREAM_SLOTS) skl_hip_withdraw_error(SKL_HIP_ERR_STREAM_SLOTS);
+    }
   }
   return rc;
 }
