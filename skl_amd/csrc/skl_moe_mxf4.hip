@@ -234,11 +234,11 @@ __global__ void __launch_bounds__(kRouterThreads) moe_router_kernel(MoeArgs a) {
 // The two products. A workgroup of eight waves has 64 CG rows of one expert's weights - columns of the result - and up to 16 RG of its tokens at a time. K comes in
 // chunks of 256, a line of a row of weights and four (TERMS times) of a token, from memory to LDS without registers, whole lines at a time, a few chunks ahead. Four
 // pairs of waves have 16 CG rows of weights each; of a pair, each has its half of every chunk, so that a token is read from LDS four times and not eight.
-// 64 tokens, 2 of 8 experts of 14336 x 4096: 114 us for h (500 MB of weights, 4.4 TB/s) and 93 for the output products (250 MB and three terms of h, of which each
+// 64 tokens, 2 of 8 experts of 14336 x 4096: 113 us for h (500 MB of weights, 4.4 TB/s) and 94 for the output products (250 MB and three terms of h, of which each
 // workgroup has to have all: 2.7 TB/s). Read straight into registers as the operands lie - 16 lines for 1024 bytes, and as many for every token's - the compute
-// units' address paths bound them: 193 and 205 us. 7 tokens, 3 of 20 experts of 1440 x 2080: 20 and 12 us, 1 token, 4 of 32 of 1024 x 2048: 9 and 6, most of it the
-// way to a launch's first bytes.
-// A chunk half is four steps of 32 k (8 from each lane group's block): the products of one run while the operands of the next come from LDS.
+// units' address paths bound them: 193 and 205 us. 7 tokens, 3 of 20 experts of 1440 x 2080: 16.6 and 11.4 us; 1 token, 4 of 32 of 1024 x 2048: 7.8 and 5.6, most of
+// it the way to a launch's first bytes. There, with one group of 16 tokens, a wave reads a chunk's operands together (step by step, below, 17.7 and 8.4 us for h);
+// weights past the caches took 20 us at 7 tokens, whose rows of 1040 bytes share lines.
 // ---------------------------------------------------------------------------------------------------------------------
 typedef __attribute__((address_space(3))) char lds_char;
 typedef unsigned unsigned_any __attribute__((aligned(1)));
@@ -266,34 +266,25 @@ struct Shape {
 // One step: acc[r][c] += x[r][t] b[c] over G groups of tokens, T terms and CG groups of columns, while the tokens' values of the next step come from `px` on into n - and,
 // if that is the first of a chunk, its weights from `pw` into w. The wait is the block's own: the compiler would make every read of LDS wait for all requests under way.
 #define SKL_MOE_MUL(a, x, b) "v_mfma_f32_16x16x32_bf16 %[" a "], %[" x "], %[" b "], %[" a "]\n"
-#define SKL_MOE_M1(c, t) SKL_MOE_MUL("a0" #c, "x0" #t, "b" #c)
-#define SKL_MOE_M2(c, t) SKL_MOE_M1(c, t) SKL_MOE_MUL("a1" #c, "x1" #t, "b" #c)
+#define SKL_MOE_M2(c, t) SKL_MOE_MUL("a0" #c, "x0" #t, "b" #c) SKL_MOE_MUL("a1" #c, "x1" #t, "b" #c)
 #define SKL_MOE_C1(G, t) SKL_MOE_M##G(0, t)
 #define SKL_MOE_C2(G, t) SKL_MOE_C1(G, t) SKL_MOE_M##G(1, t)
 #define SKL_MOE_T1(C, G) SKL_MOE_C##C(G, 0)
 #define SKL_MOE_T3(C, G) SKL_MOE_C##C(G, 0) SKL_MOE_C##C(G, 1) SKL_MOE_C##C(G, 2)
 #define SKL_MOE_RX(r, t) "ds_read_b128 %[n" #r #t "], %[px] offset:%c[o" #r #t "]\n"
-#define SKL_MOE_RX11 SKL_MOE_RX(0, 0)
-#define SKL_MOE_RX21 SKL_MOE_RX11 SKL_MOE_RX(1, 0)
-#define SKL_MOE_RX13 SKL_MOE_RX11 SKL_MOE_RX(0, 1) SKL_MOE_RX(0, 2)
-#define SKL_MOE_RX23 SKL_MOE_RX13 SKL_MOE_RX(1, 0) SKL_MOE_RX(1, 1) SKL_MOE_RX(1, 2)
+#define SKL_MOE_RX21 SKL_MOE_RX(0, 0) SKL_MOE_RX(1, 0)
+#define SKL_MOE_RX23 SKL_MOE_RX21 SKL_MOE_RX(0, 1) SKL_MOE_RX(1, 1) SKL_MOE_RX(0, 2) SKL_MOE_RX(1, 2)
 #define SKL_MOE_RW1 "ds_read_b128 %[w0], %[pw]\n"
 #define SKL_MOE_RW2 SKL_MOE_RW1 "ds_read_b128 %[w1], %[pw] offset:2048\n"
 #define SKL_MOE_A(r, c) [a##r##c] "+v"(acc[r][c])
-#define SKL_MOE_A11 SKL_MOE_A(0, 0)
-#define SKL_MOE_A21 SKL_MOE_A11, SKL_MOE_A(0, 1)
-#define SKL_MOE_A12 SKL_MOE_A11, SKL_MOE_A(1, 0)
-#define SKL_MOE_A22 SKL_MOE_A21, SKL_MOE_A(1, 0), SKL_MOE_A(1, 1)
+#define SKL_MOE_A12 SKL_MOE_A(0, 0), SKL_MOE_A(1, 0)
+#define SKL_MOE_A22 SKL_MOE_A12, SKL_MOE_A(0, 1), SKL_MOE_A(1, 1)
 #define SKL_MOE_N(r, t) [n##r##t] "=&v"(n[r][t])
-#define SKL_MOE_N11 SKL_MOE_N(0, 0)
-#define SKL_MOE_N21 SKL_MOE_N11, SKL_MOE_N(1, 0)
-#define SKL_MOE_N13 SKL_MOE_N11, SKL_MOE_N(0, 1), SKL_MOE_N(0, 2)
-#define SKL_MOE_N23 SKL_MOE_N13, SKL_MOE_N(1, 0), SKL_MOE_N(1, 1), SKL_MOE_N(1, 2)
+#define SKL_MOE_N21 SKL_MOE_N(0, 0), SKL_MOE_N(1, 0)
+#define SKL_MOE_N23 SKL_MOE_N21, SKL_MOE_N(0, 1), SKL_MOE_N(1, 1), SKL_MOE_N(0, 2), SKL_MOE_N(1, 2)
 #define SKL_MOE_X(r, t) [x##r##t] "v"(x[r][t])
-#define SKL_MOE_X11 SKL_MOE_X(0, 0)
-#define SKL_MOE_X21 SKL_MOE_X11, SKL_MOE_X(1, 0)
-#define SKL_MOE_X13 SKL_MOE_X11, SKL_MOE_X(0, 1), SKL_MOE_X(0, 2)
-#define SKL_MOE_X23 SKL_MOE_X13, SKL_MOE_X(1, 0), SKL_MOE_X(1, 1), SKL_MOE_X(1, 2)
+#define SKL_MOE_X21 SKL_MOE_X(0, 0), SKL_MOE_X(1, 0)
+#define SKL_MOE_X23 SKL_MOE_X21, SKL_MOE_X(0, 1), SKL_MOE_X(1, 1), SKL_MOE_X(0, 2), SKL_MOE_X(1, 2)
 #define SKL_MOE_W(c) [w##c] "=&v"(w[c])
 #define SKL_MOE_W1 SKL_MOE_W(0)
 #define SKL_MOE_W2 SKL_MOE_W1, SKL_MOE_W(1)
@@ -314,7 +305,7 @@ struct Shape {
   if constexpr (CG == C && GROUPS == G && TERMS == T)                                                                                                                  \
     asm volatile(SKL_MOE_RW##C SKL_MOE_RX##G##T "s_waitcnt lgkmcnt(0)" : SKL_MOE_N##G##T, SKL_MOE_W##C : SKL_MOE_OFFSETS, [px] "v"(px), [pw] "v"(pw) : "memory");
 #define SKL_MOE_EACH(F) \
-  F(1, 1, 1) F(2, 1, 1) F(1, 2, 1) F(2, 2, 1) F(1, 1, 3) F(2, 1, 3) F(1, 2, 3) F(2, 2, 3)
+  F(1, 2, 1) F(2, 2, 1) F(1, 2, 3) F(2, 2, 3)
 template <int CG, int RG, int TERMS, int GROUPS, bool LAST>
 __device__ __forceinline__ void step(v4f (&acc)[RG][CG], const v4i (&x)[GROUPS][TERMS], const v8bf (&b)[CG], v4i (&n)[GROUPS][TERMS], v4i (&w)[CG], unsigned px, unsigned pw) {
   constexpr int TERM = 16 * RG * 512;
@@ -324,6 +315,23 @@ template <int CG, int RG, int TERMS, int GROUPS>
 __device__ __forceinline__ void read_first(v4i (&n)[GROUPS][TERMS], v4i (&w)[CG], unsigned px, unsigned pw) {
   constexpr int TERM = 16 * RG * 512;
   SKL_MOE_EACH(SKL_MOE_READ)
+}
+
+// All that a wave takes of a chunk of one group of tokens: TERMS terms TERM bytes apart, four pieces each, whose places are those at `px`.
+#define SKL_MOE_P(t) \
+  "ds_read_b128 %[n" #t "0], %[p0] offset:%c[o" #t "]\nds_read_b128 %[n" #t "1], %[p1] offset:%c[o" #t "]\nds_read_b128 %[n" #t "2], %[p2] offset:%c[o" #t "]\nds_read_b128 %[n" #t "3], %[p3] offset:%c[o" #t "]\n"
+#define SKL_MOE_Q(t) [n##t##0] "=&v"(x[t][0]), [n##t##1] "=&v"(x[t][1]), [n##t##2] "=&v"(x[t][2]), [n##t##3] "=&v"(x[t][3])
+#define SKL_MOE_P1 SKL_MOE_P(0)
+#define SKL_MOE_P3 SKL_MOE_P(0) SKL_MOE_P(1) SKL_MOE_P(2)
+#define SKL_MOE_Q1 SKL_MOE_Q(0)
+#define SKL_MOE_Q3 SKL_MOE_Q(0), SKL_MOE_Q(1), SKL_MOE_Q(2)
+#define SKL_MOE_CHUNK(C, T)                                                                                                                                     \
+  if constexpr (CG == C && TERMS == T)                                                                                                                          \
+    asm volatile(SKL_MOE_RW##C SKL_MOE_P##T "s_waitcnt lgkmcnt(0)" : SKL_MOE_W##C, SKL_MOE_Q##T                                                                 \
+                 : [p0] "v"(px[0]), [p1] "v"(px[1]), [p2] "v"(px[2]), [p3] "v"(px[3]), [pw] "v"(pw), [o0] "n"(0), [o1] "n"(TERM), [o2] "n"(2 * TERM) : "memory");
+template <int CG, int TERMS, int TERM>
+__device__ __forceinline__ void read_chunk(v4i (&x)[TERMS][4], v4i (&w)[CG], const unsigned (&px)[4], unsigned pw) {
+  SKL_MOE_CHUNK(1, 1) SKL_MOE_CHUNK(2, 1) SKL_MOE_CHUNK(1, 3) SKL_MOE_CHUNK(2, 3)
 }
 
 // What a wave's lanes hold of weights and tokens while they stream.
@@ -357,7 +365,7 @@ __device__ __forceinline__ void multiply(const Operands<S> &o, v4f (&acc)[S::RG]
     const __amdgpu_buffer_rsrc_t w = __builtin_amdgcn_make_buffer_rsrc((void *)(o.codes + byte), 0, (int)kRange, 0x00027000);
 #pragma unroll
     for (int i = 0; i < CG; ++i)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(w, (__attribute__((address_space(3))) void *)(to + (wave * CG + i) * 8 * kLine), 16, (int)(in ? o.off[i] : kOutside), 0, 0, 2);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(w, (__attribute__((address_space(3))) void *)(to + (wave * CG + i) * 8 * kLine), 16, (int)(in ? o.off[i] : kOutside), 0, 0, 0);
   };
   const auto request_tokens = [&](unsigned chunk) __attribute__((always_inline)) {
     lds_char *const to = stages + S::kTokensAt + (chunk - begin) % S::kTokenStages * S::kTokenBytes;
@@ -391,7 +399,7 @@ __device__ __forceinline__ void multiply(const Operands<S> &o, v4f (&acc)[S::RG]
 #pragma unroll
     for (int c = 0; c < CG; ++c) s[c] = over > 31 ? 0u : v[c] >> over;
   };
-  unsigned raw[CG], ahead[CG], four[CG];  // scales of four chunks, of the next four
+  unsigned raw[CG], ahead[CG], four[CG];  // scales as they were loaded, of four chunks, of the next four
 #pragma unroll
   for (int c = 0; c < CG; ++c) from[c] = o.scales[c];
   if (per_row >= 4) {
@@ -405,59 +413,102 @@ __device__ __forceinline__ void multiply(const Operands<S> &o, v4f (&acc)[S::RG]
     }
   }
   load_scales(ahead, begin + 4);
+  const auto factors = [&](float (&f)[CG], unsigned chunk) __attribute__((always_inline)) {
+#pragma unroll
+    for (int c = 0; c < CG; ++c) {
+      const unsigned s = (unsigned)__builtin_amdgcn_ds_bpermute((int)(4 * l + 64 * ((chunk - begin) & 3u)), (int)four[c]);  // the lane group's that has this chunk
+      f[c] = __uint_as_float(__builtin_amdgcn_ubfe(s, 8u * (unsigned)g, 8u) << 23);
+    }
+  };
+  v4i w[CG];
+  const auto widen = [&](v8bf (&b)[CG], const float (&f)[CG], int j) __attribute__((always_inline)) {
+#pragma unroll
+    for (int c = 0; c < CG; ++c) b[c] = widen_f4((unsigned)w[c][j], f[c]);
+  };
+  const unsigned at_w = base + (pair * CG * 16 + l) * kLine + (unsigned)((4 * half + g) ^ (l & 7)) * 16u;
+  const unsigned at_x = base + S::kTokensAt + l * 512 + 256 * half + ((4u * g) ^ turn_of(l)) * 16u;
+  unsigned at = 0, stage = 0;  // where the chunk's weights and tokens are in their rings
+  const auto advance = [&]() __attribute__((always_inline)) {
+    at = at == (S::kWeightStages - 1) * S::kWeightBytes ? 0 : at + S::kWeightBytes;
+    stage = stage == (S::kTokenStages - 1) * S::kTokenBytes ? 0 : stage + S::kTokenBytes;
+  };
 #pragma unroll
   for (int c = 0; c < S::kWeightStages - S::kTokenStages; ++c) request_weights(begin + (unsigned)c);
 #pragma unroll
-  for (int c = 0; c < S::kTokenStages; ++c) request(c - S::kTokenStages);
-  __builtin_amdgcn_sched_barrier(0);
-  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(S::kUnderWay + S::kLoads) : "memory");
-  __builtin_amdgcn_s_barrier();
-  const unsigned at_w = base + (pair * CG * 16 + l) * kLine + (unsigned)((4 * half + g) ^ (l & 7)) * 16u;
-  const unsigned at_x = base + S::kTokensAt + l * 512 + 256 * half + ((4u * g) ^ turn_of(l)) * 16u;
-  place_scales(four, raw, begin);
-  v4i w[CG], x0[GROUPS][TERMS], x1[GROUPS][TERMS];
-  read_first<CG, RG, TERMS, GROUPS>(x0, w, at_x, at_w);
-  unsigned at = 0, stage = 0;  // where the chunk's weights and tokens are in their rings
+  for (int c = 0; c < S::kTokenStages - 1; ++c) request(c - S::kTokenStages);
+  if constexpr (GROUPS == 1) {
+    // Little to multiply: a chunk's operands are read together and waited for once. Its stages' predecessors are free behind the barrier.
 #pragma unroll 1
-  for (unsigned chunk = begin; chunk < stop; ++chunk) {
-    const unsigned of = (chunk - begin) & 3u;
-    float f[CG];
+    for (unsigned chunk = begin; chunk < stop; ++chunk) {
+      __builtin_amdgcn_sched_barrier(0);
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(S::kUnderWay) : "memory");
+      __builtin_amdgcn_s_barrier();
+      if (((chunk - begin) & 3u) == 0) {
+        if (chunk == begin) {
+          place_scales(four, raw, chunk);
+        } else {
+          place_scales(four, ahead, chunk);
+          load_scales(ahead, chunk + 4);
+        }
+      }
+      request((int)(chunk - begin) - 1);
+      __builtin_amdgcn_sched_barrier(0);
+      v4i x[TERMS][4];
+      const unsigned px[4] = {at_x + stage, (at_x ^ 16u) + stage, (at_x ^ 32u) + stage, (at_x ^ 48u) + stage};
+      read_chunk<CG, TERMS, 16 * RG * 512>(x, w, px, at_w + at);
+      float f[CG];
+      factors(f, chunk);
 #pragma unroll
-    for (int c = 0; c < CG; ++c) {
-      const unsigned s = (unsigned)__builtin_amdgcn_ds_bpermute((int)(4 * l + 64 * of), (int)four[c]);  // the lane group's that has this chunk
-      f[c] = __uint_as_float(__builtin_amdgcn_ubfe(s, 8u * (unsigned)g, 8u) << 23);
+      for (int j = 0; j < 4; ++j) {
+        v8bf b[CG];
+        widen(b, f, j);
+#pragma unroll
+        for (int t = 0; t < TERMS; ++t)
+#pragma unroll
+          for (int c = 0; c < CG; ++c) acc[0][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, x[t][j]), b[c], acc[0][c], 0, 0, 0);
+      }
+      advance();
     }
-    const auto widen = [&](v8bf (&b)[CG], int j) __attribute__((always_inline)) {
-#pragma unroll
-      for (int c = 0; c < CG; ++c) b[c] = widen_f4((unsigned)w[c][j], f[c]);
-    };
-    v8bf b[CG];
-    v4i none[CG];
-    widen(b, 0);
-    step<CG, RG, TERMS, GROUPS, false>(acc, x0, b, x1, none, (at_x ^ 16u) + stage, 0);
-    widen(b, 1);
-    step<CG, RG, TERMS, GROUPS, false>(acc, x1, b, x0, none, (at_x ^ 32u) + stage, 0);
-    widen(b, 2);
-    step<CG, RG, TERMS, GROUPS, false>(acc, x0, b, x1, none, (at_x ^ 48u) + stage, 0);
-    widen(b, 3);
-    // Every wave has read all of this chunk; the next one is there once the requests of all waves for it are. Then this one's stage is free.
+  } else {
+    // Four steps of 32 k (8 from each lane group's block): the products of one run while the operands of the next come from LDS.
+    request(-1);
     __builtin_amdgcn_sched_barrier(0);
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(S::kUnderWay) : "memory");
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(S::kUnderWay + S::kLoads) : "memory");
     __builtin_amdgcn_s_barrier();
-    if (of == 3) {
-      place_scales(four, ahead, chunk + 1);
-      load_scales(ahead, chunk + 5);
+    place_scales(four, raw, begin);
+    v4i x0[GROUPS][TERMS], x1[GROUPS][TERMS];
+    read_first<CG, RG, TERMS, GROUPS>(x0, w, at_x, at_w);
+#pragma unroll 1
+    for (unsigned chunk = begin; chunk < stop; ++chunk) {
+      float f[CG];
+      factors(f, chunk);
+      v8bf b[CG];
+      v4i none[CG];
+      widen(b, f, 0);
+      step<CG, RG, TERMS, GROUPS, false>(acc, x0, b, x1, none, (at_x ^ 16u) + stage, 0);
+      widen(b, f, 1);
+      step<CG, RG, TERMS, GROUPS, false>(acc, x1, b, x0, none, (at_x ^ 32u) + stage, 0);
+      widen(b, f, 2);
+      step<CG, RG, TERMS, GROUPS, false>(acc, x0, b, x1, none, (at_x ^ 48u) + stage, 0);
+      widen(b, f, 3);
+      // Every wave has read all of this chunk; the next one is there once the requests of all waves for it are. Then this one's stages are free.
+      __builtin_amdgcn_sched_barrier(0);
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(S::kUnderWay) : "memory");
+      __builtin_amdgcn_s_barrier();
+      if (((chunk - begin) & 3u) == 3) {
+        place_scales(four, ahead, chunk + 1);
+        load_scales(ahead, chunk + 5);
+      }
+      request((int)(chunk - begin));
+      __builtin_amdgcn_sched_barrier(0);
+      advance();
+      step<CG, RG, TERMS, GROUPS, true>(acc, x1, b, x0, w, at_x + stage, at_w + at);
     }
-    request((int)(chunk - begin));
-    __builtin_amdgcn_sched_barrier(0);
-    at = at == (S::kWeightStages - 1) * S::kWeightBytes ? 0 : at + S::kWeightBytes;
-    stage = stage == (S::kTokenStages - 1) * S::kTokenBytes ? 0 : stage + S::kTokenBytes;
-    step<CG, RG, TERMS, GROUPS, true>(acc, x1, b, x0, w, at_x + stage, at_w + at);
+#pragma unroll
+    for (int r = 0; r < GROUPS; ++r)
+#pragma unroll
+      for (int c = 0; c < CG; ++c) asm volatile("s_nop 15" : "+v"(acc[r][c]));  // the last products' results, before anything but a product reads them
   }
-#pragma unroll
-  for (int r = 0; r < GROUPS; ++r)
-#pragma unroll
-    for (int c = 0; c < CG; ++c) asm volatile("s_nop 15" : "+v"(acc[r][c]));  // the last products' results, before anything but a product reads them
 }
 
 // red[row of tokens][row of weights] = their products over k in [first, end), first a multiple of 256, `total` values in all.
