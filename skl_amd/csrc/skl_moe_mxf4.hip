@@ -8,8 +8,8 @@
 // The tokens of an expert are gathered: only rows of tokens that chose it are multiplied, 16 at a time. h travels as the sum of three bf16
 // values, which is all of its 24 bits: two (7.6e-6 off at most) left y 1.0e-6 off, three 3e-7, and the stream covers the third's products.
 //
-// Four launches, each with a workgroup per piece of work so that the stream finds every compute unit: the router, whose last workgroup (a counter that is zero
-// between calls) makes the choice behind everyone's sums; the two products; the weighted sum over a token's experts. Every sum has a fixed order.
+// Five launches: the router's sums, the choice, the two products, the weighted sum over a token's experts; but for the choice each with a workgroup per piece of work so
+// that the stream finds every compute unit. Every sum has a fixed order.
 #include <hip/hip_runtime.h>
 
 #include <atomic>
@@ -41,7 +41,6 @@ struct Routing {
   unsigned *place;       // [token][j], of its j-th choice
   uint16_t *h[3];        // [place][inter]: the terms
   float *out;            // [split][place][hidden], the output products
-  unsigned *counter;     // zero between launches
   unsigned router_splits, out_splits, places;
 };
 
@@ -57,22 +56,6 @@ __device__ __forceinline__ v8bf widen_f4(unsigned w, float scale) {  // eight E2
 }
 __device__ __forceinline__ unsigned short bf16_of(float v) { return __builtin_bit_cast(unsigned short, (__bf16)v); }  // to nearest even
 __device__ __forceinline__ float of_bf16(unsigned short v) { return __uint_as_float((unsigned)v << 16); }
-
-// What one workgroup leaves for another of the same launch goes past its die's cache and is read past it, value by value; a fence
-// instead writes all of that cache back, for every workgroup (tens of microseconds).
-__device__ __forceinline__ void leave(float *to, float v) { __hip_atomic_store(to, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
-__device__ __forceinline__ float found(const float *from) { return __hip_atomic_load(from, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
-
-// Whether this workgroup is the last of `all` to come here; what the others have left is then there to be found.
-__device__ __forceinline__ bool arrives_last(unsigned *counter, unsigned all, unsigned *shared) {
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's stores have reached memory
-  __syncthreads();
-  if (threadIdx.x == 0) *shared = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  __syncthreads();
-  const bool last = *shared == all - 1;
-  if (last && threadIdx.x == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  return last;
-}
 
 // A logit as a number that orders like it: NaN lowest, the two zeros alike; 0 is none.
 __device__ __forceinline__ unsigned order_of(float v) {
@@ -125,11 +108,11 @@ __device__ __forceinline__ void choose(const MoeArgs &a, Choice &c, unsigned t, 
       for (; split + 4 <= a.r.router_splits; split += 4) {  // requested together
         float v[4];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) v[q] = found(part + (split + q) * step);
+        for (int q = 0; q < 4; ++q) v[q] = part[(split + q) * step];
         value[i] += (v[0] + v[1]) + (v[2] + v[3]);
       }
 #pragma unroll 1
-      for (; split < a.r.router_splits; ++split) value[i] += found(part + split * step);
+      for (; split < a.r.router_splits; ++split) value[i] += part[split * step];
       key[i] = order_of(value[i]);
     }
   }
@@ -170,14 +153,9 @@ __device__ __forceinline__ void choose(const MoeArgs &a, Choice &c, unsigned t, 
   if ((unsigned)lane < top) c.share[t * top + lane] = mine / sum;
 }
 
-// The router: a workgroup takes 16 experts, 16 tokens and 512 of hidden, a wave 32 of these; the last one chooses.
-template <int NE>
+// The router's sums: a workgroup takes 16 experts, 16 tokens and 512 of hidden, a wave 32 of these. 3.5 us for 1 token of 32 x 2048, 4.7 for 64 of 8 x 4096: a launch and a latency.
 __global__ void __launch_bounds__(kRouterThreads) moe_router_kernel(MoeArgs a) {
-  __shared__ union {
-    float red[kRouterThreads / 64][16][17];
-    Choice c;
-  } s;
-  __shared__ unsigned arrived;
+  __shared__ float red[kRouterThreads / 64][16][17];
   const skl_moe_problem &p = a.p;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, l = lane & 15, g = lane >> 4;
   const size_t e0 = (size_t)blockIdx.x * 16, t0 = (size_t)blockIdx.y * 16, k = (size_t)blockIdx.z * 512 + 32 * (size_t)wave;
@@ -187,46 +165,53 @@ __global__ void __launch_bounds__(kRouterThreads) moe_router_kernel(MoeArgs a) {
     acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*reinterpret_cast<const v8bf *>(p.x + tr * p.ldx + k + 8 * g),
                                                   *reinterpret_cast<const v8bf *>(p.router + er * p.ld_router + k + 8 * g), acc, 0, 0, 0);
 #pragma unroll
-  for (int r = 0; r < 4; ++r) s.red[wave][4 * g + r][l] = acc[r];
+  for (int r = 0; r < 4; ++r) red[wave][4 * g + r][l] = acc[r];
   __syncthreads();
-  if (threadIdx.x < 256) {
-    const unsigned i = threadIdx.x >> 4, j = threadIdx.x & 15;
-    float v = 0.0f;
+  if (threadIdx.x >= 256) return;
+  const unsigned i = threadIdx.x >> 4, j = threadIdx.x & 15;
+  float v = 0.0f;
 #pragma unroll
-    for (int w = 0; w < kRouterThreads / 64; ++w) v += s.red[w][i][j];
-    if (t0 + i < p.tokens && e0 + j < p.experts) leave(a.r.parts + ((size_t)blockIdx.z * p.tokens + t0 + i) * p.experts + e0 + j, v);
-  }
-  if (!arrives_last(a.r.counter, gridDim.x * gridDim.y * gridDim.z, &arrived)) return;
-  const unsigned top = (unsigned)p.top_k, tokens = (unsigned)p.tokens, e = threadIdx.x;
-  s.c.mask[e][0] = s.c.mask[e][1] = 0;  // one thread per expert
+  for (int w = 0; w < kRouterThreads / 64; ++w) v += red[w][i][j];
+  if (t0 + i < p.tokens && e0 + j < p.experts) a.r.parts[((size_t)blockIdx.z * p.tokens + t0 + i) * p.experts + e0 + j] = v;
+}
+
+// The choice: one workgroup of a wave per token and a thread per expert, as far as there are that many. 3.4 us for 1 token, 8.8 for 64, bound by what follows one another: the sums read back,
+// top_k rounds of a maximum, a scan. (Behind a counter in the router's last workgroup the layer took as long, to 2 %.)
+template <int NE>
+__global__ void __launch_bounds__(kRouterThreads) moe_choice_kernel(MoeArgs a) {
+  __shared__ Choice c;
+  const skl_moe_problem &p = a.p;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const unsigned threads = blockDim.x, top = (unsigned)p.top_k, tokens = (unsigned)p.tokens, e = threadIdx.x;
+  c.mask[e][0] = c.mask[e][1] = 0;  // one thread per expert
   __syncthreads();
-  for (unsigned t = wave; t < tokens; t += kRouterThreads / 64) choose<NE>(a, s.c, t, lane);
+  for (unsigned t = wave; t < tokens; t += threads / 64) choose<NE>(a, c, t, lane);
   __syncthreads();
   // Where each expert's tokens begin, and its slot: one scan over the experts, the count in the lower half, the slot in the upper.
-  const unsigned count = __popc(s.c.mask[e][0]) + __popc(s.c.mask[e][1]), own = count | (count ? 0x10000u : 0u);
+  const unsigned count = __popc(c.mask[e][0]) + __popc(c.mask[e][1]), own = count | (count ? 0x10000u : 0u);
   unsigned scan = own;
 #pragma unroll
   for (int step = 1; step < 64; step <<= 1) {
     const unsigned other = __shfl_up(scan, step, 64);
     if (lane >= step) scan += other;
   }
-  if (lane == 63) s.c.totals[wave] = scan;
+  if (lane == 63) c.totals[wave] = scan;
   __syncthreads();
-  for (int w = 0; w < wave; ++w) scan += s.c.totals[w];
-  s.c.start[e] = (scan - own) & 0xFFFFu;
-  s.c.slot[e] = (unsigned short)((scan - own) >> 16);
-  if (count) a.r.slots[s.c.slot[e]] = Slot{e, s.c.start[e], count, 0};
-  if (e == kMaxExperts - 1) *a.r.active = scan >> 16;
+  for (int w = 0; w < wave; ++w) scan += c.totals[w];
+  c.start[e] = (scan - own) & 0xFFFFu;
+  c.slot[e] = (unsigned short)((scan - own) >> 16);
+  if (count) a.r.slots[c.slot[e]] = Slot{e, c.start[e], count, 0};
+  if (e == threads - 1) *a.r.active = scan >> 16;
   __syncthreads();
-  for (unsigned at = threadIdx.x; at < tokens * top; at += kRouterThreads) {
-    const unsigned t = at / top, c = s.c.chosen[at], below = (1u << (t & 31u)) - 1u;
-    const unsigned before = t < 32 ? __popc(s.c.mask[c][0] & below) : __popc(s.c.mask[c][0]) + __popc(s.c.mask[c][1] & below);
-    const unsigned place = s.c.start[c] + before;
-    a.r.tokens[s.c.slot[c] * kMaxTokens + before] = (uint8_t)t;
-    a.r.weight[place] = s.c.share[at];
+  for (unsigned at = threadIdx.x; at < tokens * top; at += threads) {
+    const unsigned t = at / top, chosen = c.chosen[at], below = (1u << (t & 31u)) - 1u;
+    const unsigned before = t < 32 ? __popc(c.mask[chosen][0] & below) : __popc(c.mask[chosen][0]) + __popc(c.mask[chosen][1] & below);
+    const unsigned place = c.start[chosen] + before;
+    a.r.tokens[c.slot[chosen] * kMaxTokens + before] = (uint8_t)t;
+    a.r.weight[place] = c.share[at];
     a.r.place[at] = place;
-    if (p.ids) p.ids[at] = (int32_t)c;
-    if (p.weights) p.weights[at] = s.c.share[at];
+    if (p.ids) p.ids[at] = (int32_t)chosen;
+    if (p.weights) p.weights[at] = c.share[at];
   }
 }
 
@@ -664,8 +649,8 @@ __global__ void __launch_bounds__(kThreads) moe_out_kernel(MoeArgs a) {
   }
 }
 
-// y: two columns of a token to a thread. (Left to the workgroup that is the last of its columns, this took 2 us more at 1 token, 5 at 7 and 35 at 64 tokens of 128 experts,
-// whose output products are 4 MiB.)
+// y: two columns of a token to a thread. 3.3 to 5 us, a launch and a latency. (Left to the workgroup that is the last of its columns, the sum took 2 us more at 1 token,
+// 5 at 7 and 35 at 64 tokens of 128 experts, whose output products are 4 MiB.)
 __global__ void __launch_bounds__(256) moe_sum_kernel(MoeArgs a) {
   const unsigned j = (blockIdx.x * 256u + threadIdx.x) * 2u;
   if (j >= a.p.hidden) return;
@@ -755,21 +740,25 @@ int launch_products(const MoeArgs &a, unsigned slots) {
   return out == 2 ? launch_out<2, RG>(a, slots) : launch_out<1, RG>(a, slots);
 }
 
-int launch_on(const skl_moe_problem *p, char *block, unsigned *counter) {
+int launch_on(const skl_moe_problem *p, char *block) {
   MoeArgs a = {*p, {}};
   lay_out(p, block, &a.r);
-  a.r.counter = counter;
   const unsigned slots = (unsigned)(p->experts < a.r.places ? p->experts : a.r.places);
   hipStream_t st = skl_current_stream();
   const dim3 grid(skl_div_up(p->experts, 16), skl_div_up(p->tokens, 16), a.r.router_splits);
-  if (p->experts <= 64) moe_router_kernel<1><<<grid, kRouterThreads, 0, st>>>(a);
-  else if (p->experts <= 128) moe_router_kernel<2><<<grid, kRouterThreads, 0, st>>>(a);
-  else if (p->experts <= 256) moe_router_kernel<4><<<grid, kRouterThreads, 0, st>>>(a);
-  else moe_router_kernel<16><<<grid, kRouterThreads, 0, st>>>(a);
-  const int rc = skl_check_launch("moe_router");
+  moe_router_kernel<<<grid, kRouterThreads, 0, st>>>(a);
+  int rc = skl_check_launch("moe_router");
   if (rc != 0) return rc;
-  const int done = token_groups(p) == 1 ? launch_products<1>(a, slots) : launch_products<2>(a, slots);
-  if (done != 0) return done;
+  const size_t want = p->experts > 64 * p->tokens ? p->experts : 64 * p->tokens;
+  const unsigned threads = want < kRouterThreads ? (unsigned)(want + 63) / 64 * 64 : kRouterThreads;
+  if (p->experts <= 64) moe_choice_kernel<1><<<1, threads, 0, st>>>(a);
+  else if (p->experts <= 128) moe_choice_kernel<2><<<1, threads, 0, st>>>(a);
+  else if (p->experts <= 256) moe_choice_kernel<4><<<1, threads, 0, st>>>(a);
+  else moe_choice_kernel<16><<<1, threads, 0, st>>>(a);
+  rc = skl_check_launch("moe_choice");
+  if (rc != 0) return rc;
+  rc = token_groups(p) == 1 ? launch_products<1>(a, slots) : launch_products<2>(a, slots);
+  if (rc != 0) return rc;
   moe_sum_kernel<<<dim3(skl_div_up(p->hidden, 512), (unsigned)p->tokens), 256, 0, st>>>(a);
   return skl_check_launch("moe_sum");
 }
@@ -778,25 +767,15 @@ int launch_on(const skl_moe_problem *p, char *block, unsigned *counter) {
 
 extern "C" int skl_hip_launch_moe(const skl_moe_problem *p) {
   Routing r;
-  const size_t bytes = lay_out(p, nullptr, &r), zero = sizeof(unsigned);
+  const size_t bytes = lay_out(p, nullptr, &r);
   const int pending = skl_hip_pending_error();
   int rc;
   skl_hip_sequence_begin();  // the launches hand data on through the stream's scratch memory
-  char *block = static_cast<char *>(skl_hip_operand_scratch(bytes));
-  unsigned *zeroed = block ? static_cast<unsigned *>(skl_hip_zeroed_sums(zero)) : nullptr;
-  char *own = nullptr;
-  if (!block || !zeroed) {
-    // a stream without scratch memory, or no room for it: a block for this call alone, released once the stream has drained
-    own = static_cast<char *>(skl_hip_malloc(bytes + zero));
-    if (own && skl_hip_memset(own + bytes, 0, zero) != 0) {
-      skl_hip_free(own);
-      own = nullptr;
-    }
-    block = own;
-    zeroed = reinterpret_cast<unsigned *>(own + bytes);
-  }
+  char *block = static_cast<char *>(skl_hip_operand_scratch(bytes)), *own = nullptr;
+  // a stream without scratch memory, or no room for it: a block for this call alone, released once the stream has drained
+  if (!block) block = own = static_cast<char *>(skl_hip_malloc(bytes));
   if (block) {
-    rc = launch_on(p, block, zeroed);
+    rc = launch_on(p, block);
   } else {
     rc = SKL_HIP_ERR_WORKSPACE;
     skl_hip_withdraw_error(SKL_HIP_ERR_STREAM_SLOTS);
