@@ -1114,8 +1114,10 @@ int launch_rows(const MxArgs &p) {
 enum Kind { kWide4, kWide2, kRows, kSmall };
 Kind kind_of(const MxArgs &p) {
   if (p.m <= 64 && p.k >= 256 && rows_scale_bytes(row_groups(p), skl_kcstream::column_groups(p.n), p.k) <= (size_t)kRowsScaleSpace) return kRows;
-  if (tiles_of(p, 256, 256) >= 200 && p.k >= 2560) return kWide4;
-  if (tiles_of(p, 128, 128) >= 256 && p.k >= 1024) return kWide2;
+  if (p.k <= ((size_t)1 << 23)) {  // a large tile's offsets from its first row are 31-bit numbers, 255 rows of half a byte per value
+    if (tiles_of(p, 256, 256) >= 200 && p.k >= 2560) return kWide4;
+    if (tiles_of(p, 128, 128) >= 256 && p.k >= 1024) return kWide2;
+  }
   return kSmall;
 }
 
@@ -1142,7 +1144,7 @@ extern "C" int skl_hip_launch_gemm_mx(const skl_mx_gemm *g) {
   if (p.k == 0 || p.k > ((size_t)1 << 26)) return launch_any(p);
   const Kind kind = kind_of(p);
   // Operands in rows that the kernel does not read are copied first; for large tiles also those whose rows do not begin on lines, as every request of theirs takes a line
-  // more (us with and without the copy: 3000 x 5000 x 7000 76 / 85, 2048 x 4096 x 4112 36 / 41, 2048 x 2048 x 3000 24 / 26, 8192 x 8192 x 3000 175 / 205).
+  // more (us with and without the copy: 3000 x 5000 x 7000 81 / 88, 2048 x 4096 x 4112 38 / 41, 2048 x 2048 x 3000 26 / 26, 8192 x 8192 x 3000 176 / 210).
   const unsigned exist = (unsigned)((p.k + 1) / 2), blocks = (unsigned)((p.k + 31) / 32), mask = p.k % 2 ? 15u : 255u;
   PadJobs jobs = {};
   const uint8_t **first[4] = {&p.a, &p.b, &p.sa, &p.sb};
