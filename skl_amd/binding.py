@@ -90,14 +90,24 @@ class MoeLayer:
     def as_struct(self):
         return self._struct
 
+    @property
+    def _as_parameter_(self):
+        return ctypes.addressof(self._struct)
+
 
 def _wrap(raw, sig):
     ptr_positions = [i for i, ch in enumerate(sig) if ch == "p"]
     epilogue_positions = [i for i, ch in enumerate(sig) if ch in "EM"]
 
+    count = len(sig)
+
     def call(*args):
-        if len(args) != len(sig):
-            raise TypeError(f"{raw.__name__}: expected {len(sig)} arguments, got {len(args)}")
+        if len(args) != count:
+            raise TypeError(f"{raw.__name__}: expected {count} arguments, got {len(args)}")
+        try:
+            return raw(*args)  # integers, None and what gives ctypes its address (_as_parameter_): 0.4 us less than by way of a list
+        except ctypes.ArgumentError:  # raised before the call
+            pass
         args = list(args)
         for i in ptr_positions:
             args[i] = _as_pointer(args[i])
@@ -168,6 +178,10 @@ class DeviceBuffer:
         if rc != 0:
             check_error()
         return out
+
+    @property
+    def _as_parameter_(self):
+        return self.ptr
 
     def offset(self, nbytes):
         """Address `nbytes` into the buffer (for misalignment tests)."""
