@@ -49,6 +49,41 @@ constexpr int kChunkK = 256, kLine = 128;
 // The slot of a row's 16-byte piece in the row's line in LDS: lanes that read the same piece of 32 rows meet in no bank.
 __device__ __forceinline__ unsigned slot_of(unsigned row, unsigned piece) { return piece ^ ((row >> 1) & 7u); }
 
+// The ends of rows. What lies behind a row is loaded by nobody: 16 bytes (eight scales) at an end are loaded from further down and moved into place, in one load - byte by byte, each
+// waited for, the last chunk took longer than all others of a short K. Shorter rows do go byte by byte.
+typedef unsigned __int128 u128;
+struct EndOf {  // of the 16 bytes at `at`, in a row of `bytes`: where they are loaded from
+  size_t from;
+  __device__ __forceinline__ EndOf(size_t bytes, size_t at) : from(at + 16 <= bytes || bytes < 16 ? at : bytes - 16) {}
+};
+__device__ __forceinline__ v4i load_end(const uint8_t *row, size_t bytes, EndOf e) {
+  if (bytes >= 16) return *reinterpret_cast<const v4i_any *>(row + e.from);
+  v4i v = {0, 0, 0, 0};
+  for (unsigned b = 0; e.from + b < bytes; ++b) v[b >> 2] |= (int)((unsigned)row[e.from + b] << (8 * (b & 3u)));
+  return v;
+}
+// The values from 2 `at` on of a row of k, zeros behind its end; v: loaded from e.
+__device__ __forceinline__ v4i settle_end(v4i v, size_t k, size_t at, EndOf e) {
+  const size_t over = at - e.from;
+  u128 bits = over < 16 ? __builtin_bit_cast(u128, v) >> (8 * (unsigned)over) : (u128)0;
+  const size_t have = 2 * at < k ? k - 2 * at : 0;  // values
+  if (have < 32) bits &= ((u128)1 << (4 * (unsigned)have)) - 1;
+  return __builtin_bit_cast(v4i, bits);
+}
+// Eight scale bytes from `at` on of a row of `bytes`; ones behind its end.
+__device__ __forceinline__ v2u load_scale_end(const uint8_t *row, size_t bytes, size_t at) {
+  if (bytes >= 8) return *reinterpret_cast<const v2u_any *>(row + (at + 8 <= bytes ? at : bytes - 8));
+  v2u v = {0, 0};
+  for (unsigned b = 0; at + b < bytes; ++b) v[b >> 2] |= (unsigned)row[at + b] << (8 * (b & 3u));
+  return v;
+}
+__device__ __forceinline__ v2u settle_scale_end(v2u v, size_t bytes, size_t at) {
+  if (at + 8 <= bytes) return v;
+  const unsigned over = bytes >= 8 ? (unsigned)(at + 8 - bytes) : 0u, have = at < bytes ? (unsigned)(bytes - at) : 0u;
+  const unsigned long long kept = (1ull << (8 * have)) - 1, bits = over < 8 ? __builtin_bit_cast(unsigned long long, v) >> (8 * over) : 0ull;
+  return __builtin_bit_cast(v2u, (bits & kept) | (0x7F7F7F7F7F7F7F7Full & ~kept));
+}
+
 // One of a workgroup's operands on its way from memory to LDS: ROWS rows of a chunk, 16 bytes at a time.
 template <int ROWS, int THREADS>
 struct Stage {
@@ -61,41 +96,26 @@ struct Stage {
   // lies behind K in its last block is not part of the matrix and counts as zero.
   __device__ __forceinline__ void load(const uint8_t *first, size_t pitch, const uint8_t *scales, size_t scale_pitch, unsigned rows, size_t k, size_t k0) {
     const bool whole = k0 + kChunkK <= k;  // the same for every thread
+    const size_t bytes = (k + 1) / 2, blocks = (k + 31) / 32;
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
       const unsigned at = (unsigned)i * THREADS + threadIdx.x, r = at >> 3, q = at & 7u;
-      const uint8_t *p = first + (size_t)(r < rows ? r : rows - 1) * pitch + k0 / 2 + 16 * q;
-      if (whole) {
-        piece[i] = *reinterpret_cast<const v4i_any *>(p);
-      } else {
-        const size_t kp = k0 + 32 * (size_t)q;
-        piece[i] = v4i{0, 0, 0, 0};
-        if (kp + 32 <= k) {
-          piece[i] = *reinterpret_cast<const v4i_any *>(p);
-        } else if (kp < k) {
-          const unsigned left = (unsigned)(k - kp);  // values, 1 to 31
-          for (unsigned byte = 0; 2 * byte < left; ++byte) {
-            const unsigned v = 2 * byte + 1 < left ? p[byte] : p[byte] & 15u;
-            piece[i][byte >> 2] |= (int)(v << (8 * (byte & 3u)));
-          }
-        }
-      }
+      const uint8_t *row = first + (size_t)(r < rows ? r : rows - 1) * pitch;
+      piece[i] = whole ? *reinterpret_cast<const v4i_any *>(row + k0 / 2 + 16 * q) : load_end(row, bytes, EndOf(bytes, k0 / 2 + 16 * q));
     }
 #pragma unroll
     for (int i = 0; i < kScales; ++i) {
       const unsigned r = (unsigned)i * THREADS + threadIdx.x;
-      const uint8_t *p = scales + (size_t)(r < rows ? r : rows - 1) * scale_pitch + k0 / 32;
-      if (whole) {
-        scale[i] = *reinterpret_cast<const v2u_any *>(p);
-      } else {
-        scale[i] = v2u{0x7F7F7F7Fu, 0x7F7F7F7Fu};
-        for (unsigned byte = 0; byte < 8; ++byte)
-          if (k0 + 32 * (size_t)byte < k) {
-            const unsigned shift = 8 * (byte & 3u);
-            scale[i][byte >> 2] = (scale[i][byte >> 2] & ~(255u << shift)) | ((unsigned)p[byte] << shift);
-          }
-      }
+      scale[i] = load_scale_end(scales + (size_t)(r < rows ? r : rows - 1) * scale_pitch, blocks, k0 / 32);
     }
+    if (whole) return;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const size_t at = k0 / 2 + 16 * (((unsigned)i * THREADS + threadIdx.x) & 7u);
+      piece[i] = settle_end(piece[i], k, at, EndOf(bytes, at));
+    }
+#pragma unroll
+    for (int i = 0; i < kScales; ++i) scale[i] = settle_scale_end(scale[i], blocks, k0 / 32);
   }
   __device__ __forceinline__ void store(char *lines, char *scale_bytes) const {
 #pragma unroll
@@ -223,7 +243,7 @@ __device__ __forceinline__ void write_c(const MxArgs &p, const v16f (&sum)[TN][T
   else write_rows<kThrough, false, TM, TN>(p, sum, row0, col0, rows, cols, lane, space);
 }
 
-// Any layout: 64 x 64 tiles of four waves, one block of 32 x 32 each, operands through registers.
+// Any layout: 64 x 64 tiles of four waves, one block of 32 x 32 each, operands through registers. 700 x 700 x 700 6.1 us, 1500 x 1500 x 1500 14.0.
 __global__ void __launch_bounds__(256) gemm_mx_kernel(MxArgs p) {
   constexpr int WM = 2, WN = 2, TM = 1, TN = 1;
   constexpr int kThreads = WM * WN * 64, kRows = WM * TM * 32, kCols = WN * TN * 32;
@@ -408,37 +428,29 @@ __global__ void __launch_bounds__(256) gemm_mx_stream_kernel(MxArgs p) {
     const unsigned r = (unsigned)i * kThreads + threadIdx.x, c = r - kRows;
     scale_at[i] = r < (unsigned)kRows ? p.sa + (size_t)(row0 + (r < rows ? r : rows - 1)) * p.sa_row : p.sb + (size_t)(col0 + (c < cols ? c : cols - 1)) * p.sb_col;
   }
+  const size_t per_row = blocks + (part != 0);
   auto load_scales = [&](size_t chunk) {
 #pragma unroll
     for (int i = 0; i < kScales; ++i) {
-      const uint8_t *from = scale_at[i] + chunk * 8;
-      if ((chunk + 1) * 8 <= blocks + (part != 0)) {
-        scale[i] = *reinterpret_cast<const v2u_any *>(from);
-      } else {
-        scale[i] = v2u{0x7F7F7F7Fu, 0x7F7F7F7Fu};
-        for (unsigned byte = 0; byte < 8; ++byte)
-          if (chunk * 8 + byte < blocks + (part != 0)) {
-            const unsigned shift = 8 * (byte & 3u);
-            scale[i][byte >> 2] = (scale[i][byte >> 2] & ~(255u << shift)) | ((unsigned)from[byte] << shift);
-          }
-      }
+      scale[i] = load_scale_end(scale_at[i], per_row, chunk * 8);
     }
   };
   auto keep_scales = [&](size_t chunk) {
 #pragma unroll
     for (int i = 0; i < kScales; ++i) {
+      scale[i] = settle_scale_end(scale[i], per_row, chunk * 8);
       const unsigned r = (unsigned)i * kThreads + threadIdx.x;
       if ((kRows + kCols) % kThreads == 0 || r < (unsigned)(kRows + kCols))
         asm volatile("ds_write_b64 %0, %1" ::"v"(ring + 2 * kStageBytes + (unsigned)(chunk & 1) * kScaleBytes + r * 8), "v"(scale[i]) : "memory");
     }
   };
-  // A last block that is not whole: read and masked value by value, written over the zeros that stand for it.
+  // A last block that is not whole: read and masked, written over the zeros that stand for it.
   auto keep_part = [&](size_t chunk) {
     for (unsigned r = threadIdx.x; r < (unsigned)(kRows + kCols); r += kThreads) {
       const unsigned c = r - kRows;
-      const uint8_t *from = (r < (unsigned)kRows ? p.a + (size_t)(row0 + (r < rows ? r : rows - 1)) * p.a_row : p.b + (size_t)(col0 + (c < cols ? c : cols - 1)) * p.b_col) + 16 * (size_t)blocks;
-      v4i v = {0, 0, 0, 0};
-      for (unsigned byte = 0; 2 * byte < part; ++byte) v[byte >> 2] |= (int)((2 * byte + 1 < part ? from[byte] : from[byte] & 15u) << (8 * (byte & 3u)));
+      const uint8_t *const row = r < (unsigned)kRows ? p.a + (size_t)(row0 + (r < rows ? r : rows - 1)) * p.a_row : p.b + (size_t)(col0 + (c < cols ? c : cols - 1)) * p.b_col;
+      const size_t bytes = (p.k + 1) / 2, at = 16 * (size_t)blocks;
+      const v4i v = settle_end(load_end(row, bytes, EndOf(bytes, at)), p.k, at, EndOf(bytes, at));
       asm volatile("ds_write_b128 %0, %1" ::"v"(ring + (unsigned)(chunk & 1) * kStageBytes + r * kLine + slot_of(r, blocks & 7u) * 16), "v"(v) : "memory");
     }
   };
@@ -743,14 +755,14 @@ __global__ void __launch_bounds__(256, TM == 2 ? 2 : 1) gemm_mx_wide_kernel(MxAr
       advance(rs[i], kGroupBytes);
     }
   };
-  // A last block that is not whole: read and masked value by value, written over the zeros that stand for it.
+  // A last block that is not whole: read and masked, written over the zeros that stand for it.
   const auto keep_part = [&](unsigned chunk) {
     __builtin_amdgcn_s_barrier();  // the zeros that other waves' requests wrote are there
     for (unsigned r = threadIdx.x; r < (unsigned)(kRows + kCols); r += 256) {
       const unsigned c = r - kRows;
-      const uint8_t *from = (r < (unsigned)kRows ? a0 + (size_t)(r < rows ? r : rows - 1) * p.a_row : b0 + (size_t)(c < cols ? c : cols - 1) * p.b_col) + 16 * (size_t)blocks;
-      v4i v = {0, 0, 0, 0};
-      for (unsigned byte = 0; 2 * byte < part; ++byte) v[byte >> 2] |= (int)((2 * byte + 1 < part ? from[byte] : from[byte] & 15u) << (8 * (byte & 3u)));
+      const uint8_t *const row = r < (unsigned)kRows ? a0 + (size_t)(r < rows ? r : rows - 1) * p.a_row : b0 + (size_t)(c < cols ? c : cols - 1) * p.b_col;
+      const size_t bytes = (p.k + 1) / 2, at = 16 * (size_t)blocks;
+      const v4i v = settle_end(load_end(row, bytes, EndOf(bytes, at)), p.k, at, EndOf(bytes, at));
       asm volatile("ds_write_b128 %0, %1" ::"v"(ring + (chunk & 1u) * kStageBytes + r * kLine + slot_of(r, blocks & 7u) * 16), "v"(v) : "memory");
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -1160,6 +1172,9 @@ extern "C" int skl_hip_launch_gemm_mx(const skl_mx_gemm *g) {
     most = grid > most ? grid : most;
   }
   if (bytes == 0) return launch_kind(p, kind);
+  // With a short K the kernel that reads anything is done before a copy would be (us, copied and not: 700 x 700 x 700 9.5 / 6.1, 100 x 300 x 2001 11.5 / 9.6, 1500 x 1500 x 1500
+  // 14.9 / 14.0, 50 x 3000 x 301 9.5 / 4.9, 1 x 4096 x 1001 8.5 / 5.7; 1500 x 1500 x 2998 22.0 / 25.9, 100 x 300 x 5001 14.2 / 19.2).
+  if (kind >= kRows && p.k <= 2048) return launch_any(p);
   const int pending = skl_hip_pending_error();
   skl_hip_sequence_begin();
   uint8_t *block = static_cast<uint8_t *>(skl_hip_converted_scratch(bytes));  // (apart from the block that a product's shares of K take)
