@@ -63,6 +63,7 @@ __device__ __forceinline__ unsigned order_of(float v) {
   const unsigned b = __float_as_uint(v + 0.0f);
   return (b & 0x80000000u) ? ~b : b | 0x80000000u;
 }
+__device__ __forceinline__ float logit_of(unsigned key) { return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key); }  // the way back; of 1, a NaN
 template <int CTRL, int ROWS>
 __device__ __forceinline__ unsigned max_with(unsigned v) {  // of lanes that nothing comes to: v
   const unsigned o = (unsigned)__builtin_amdgcn_update_dpp((int)v, (int)v, CTRL, ROWS, 0xF, false);
@@ -89,68 +90,70 @@ struct Choice {
   unsigned totals[kRouterThreads / 64];
 };
 
-// The choice of one token by one wave: NE logits per lane, expert 64 i + lane.
-template <int NE>
-__device__ __forceinline__ void choose(const MoeArgs &a, Choice &c, unsigned t, int lane) {
+template <int G>
+__device__ __forceinline__ unsigned max_of(unsigned v) {  // over the G lanes of a token
+  if constexpr (G == 64) return wave_max(v);
+  v = max_with<0x128, 0xF>(v);  // eight, four, two and one lanes round a row of 16
+  v = max_with<0x124, 0xF>(v);
+  v = max_with<0x122, 0xF>(v);
+  return max_with<0x121, 0xF>(v);
+}
+
+// The choice of 64 / G tokens by one wave: NE logits per lane, expert G i + l. A round finds the largest that is left and the lowest expert that has it; the j-th lane keeps
+// those of round j, so that exponentials, quotients and stores come once for all rounds. Tokens from `tokens` on: the last one again, not kept.
+template <int G, int NE>
+__device__ __forceinline__ void choose(const MoeArgs &a, Choice &c, unsigned t, unsigned l) {
+  constexpr unsigned kAhead = 8;  // parts of a sum requested together
   const skl_moe_problem &p = a.p;
-  const unsigned experts = (unsigned)p.experts, top = (unsigned)p.top_k;
+  const unsigned experts = (unsigned)p.experts, top = (unsigned)p.top_k, splits = a.r.router_splits, tokens = (unsigned)p.tokens;
   float value[NE];
   unsigned key[NE];
 #pragma unroll
-  for (int i = 0; i < NE; ++i) {
-    const unsigned e = 64u * i + lane;
-    value[i] = 0.0f, key[i] = 0;
-    if (e < experts) {
-      const float *part = a.r.parts + (size_t)t * experts + e;
-      const size_t step = (size_t)p.tokens * experts;
-      unsigned split = 0;
+  for (int i = 0; i < NE; ++i) value[i] = 0.0f;
 #pragma unroll 1
-      for (; split + 4 <= a.r.router_splits; split += 4) {  // requested together
-        float v[4];
+  for (unsigned split = 0; split < splits; split += kAhead) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) v[q] = part[(split + q) * step];
-        value[i] += (v[0] + v[1]) + (v[2] + v[3]);
-      }
-#pragma unroll 1
-      for (; split < a.r.router_splits; ++split) value[i] += part[split * step];
-      key[i] = order_of(value[i]);
+    for (int i = 0; i < NE; ++i) {
+      const unsigned e = G * i + l;
+      float v[kAhead];
+#pragma unroll
+      for (unsigned q = 0; q < kAhead; ++q)
+        v[q] = a.r.parts[((size_t)(split + q < splits ? split + q : splits - 1) * tokens + (t < tokens ? t : tokens - 1)) * experts + (e < experts ? e : experts - 1)];
+#pragma unroll
+      for (unsigned q = 0; q < kAhead; ++q)
+        if (split + q < splits) value[i] += v[q];
     }
   }
-  float largest = 0.0f, sum = 0.0f, mine = 0.0f;
+#pragma unroll
+  for (int i = 0; i < NE; ++i) key[i] = G * i + l < experts ? order_of(value[i]) : 0;
+  unsigned my_key = 0, my_expert = 0;
   for (unsigned j = 0; j < top; ++j) {
-    unsigned best = key[0];
+    unsigned best = key[0], at = 0;
 #pragma unroll
-    for (int i = 1; i < NE; ++i) best = key[i] > best ? key[i] : best;
-    best = wave_max(best);
-    unsigned e = 0xFFFFFFFFu;
-    float v = 0.0f;
+    for (int i = 1; i < NE; ++i)
+      if (key[i] > best) best = key[i], at = i;
+    const unsigned largest = max_of<G>(best);
+    const unsigned e = G == 64 && NE == 1 ? (unsigned)__builtin_ctzll(__ballot(best == largest)) : ~max_of<G>(best == largest ? ~(G * at + l) : 0u);
 #pragma unroll
-    for (int i = 0; i < NE; ++i) {  // the lowest expert that has it
-      const unsigned long long who = __ballot(key[i] == best);
-      if (e == 0xFFFFFFFFu && who) {
-        const int at = __builtin_ctzll(who);
-        e = 64u * i + (unsigned)at;
-        v = __uint_as_float((unsigned)__builtin_amdgcn_readlane((int)__float_as_uint(value[i]), at));
-        if (lane == at) key[i] = 0;
-      }
-    }
-    if (j == 0) largest = v;
-    const float x = expf(v - largest);
-    if (p.normalise) sum += x;
-    if ((unsigned)lane == j) mine = x;
-    if (lane == 0) {
-      c.chosen[t * top + j] = (unsigned short)e;
-      atomicOr(&c.mask[e][t >> 5], 1u << (t & 31u));
-    }
+    for (int i = 0; i < NE; ++i) key[i] = G * i + l == e ? 0u : key[i];
+    if (l == j) my_key = largest, my_expert = e;
   }
+  const float mine = logit_of(my_key), largest = __shfl(mine, 0, G);
+  const float x = l < top ? expf(mine - largest) : 0.0f;
+  float sum = x;
   if (!p.normalise) {
+    sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < NE; ++i)
-      if (64u * i + lane < experts) sum += expf(value[i] - largest);
-#pragma unroll
-    for (int step = 32; step > 0; step >>= 1) sum += __shfl_xor(sum, step, 64);
+      if (G * i + l < experts) sum += expf(value[i] - largest);
   }
-  if ((unsigned)lane < top) c.share[t * top + lane] = mine / sum;
+#pragma unroll
+  for (int step = G / 2; step > 0; step >>= 1) sum += __shfl_xor(sum, step, 64);
+  if (l < top && t < tokens) {
+    c.share[t * top + l] = x / sum;
+    c.chosen[t * top + l] = (unsigned short)my_expert;
+    atomicOr(&c.mask[my_expert][t >> 5], 1u << (t & 31u));
+  }
 }
 
 // The router's sums: a workgroup takes 16 experts, 16 tokens and 512 of hidden, a wave 32 of these. 3.5 us for 1 token of 32 x 2048, 4.7 for 64 of 8 x 4096: a launch and a latency.
@@ -175,9 +178,10 @@ __global__ void __launch_bounds__(kRouterThreads) moe_router_kernel(MoeArgs a) {
   if (t0 + i < p.tokens && e0 + j < p.experts) a.r.parts[((size_t)blockIdx.z * p.tokens + t0 + i) * p.experts + e0 + j] = v;
 }
 
-// The choice: one workgroup of a wave per token and a thread per expert, as far as there are that many. 3.4 us for 1 token, 8.8 for 64, bound by what follows one another: the sums read back,
-// top_k rounds of a maximum, a scan. (Behind a counter in the router's last workgroup the layer took as long, to 2 %.)
-template <int NE>
+// The choice: one workgroup, of a wave per token or, for many tokens and not too many experts, per four, and a thread per expert, as far as there are that many. 3.5 us for 1
+// token, for 64 tokens 5.8 (4 of 20 experts) and 11 (8 of 128; 10 and 22 with a wave per token), 54 of 512, bound by what follows one another: the sums read back, top_k rounds of
+// two maxima, a scan. (Behind a counter in the router's last workgroup the layer took as long, to 2 %.)
+template <int G, int NE>
 __global__ void __launch_bounds__(kRouterThreads) moe_choice_kernel(MoeArgs a) {
   __shared__ Choice c;
   const skl_moe_problem &p = a.p;
@@ -185,7 +189,8 @@ __global__ void __launch_bounds__(kRouterThreads) moe_choice_kernel(MoeArgs a) {
   const unsigned threads = blockDim.x, top = (unsigned)p.top_k, tokens = (unsigned)p.tokens, e = threadIdx.x;
   c.mask[e][0] = c.mask[e][1] = 0;  // one thread per expert
   __syncthreads();
-  for (unsigned t = wave; t < tokens; t += threads / 64) choose<NE>(a, c, t, lane);
+  constexpr unsigned kEach = 64 / G;
+  for (unsigned first = wave * kEach; first < tokens; first += threads / 64 * kEach) choose<G, NE>(a, c, first + lane / G, lane % G);
   __syncthreads();
   // Where each expert's tokens begin, and its slot: one scan over the experts, the count in the lower half, the slot in the upper.
   const unsigned count = __popc(c.mask[e][0]) + __popc(c.mask[e][1]), own = count | (count ? 0x10000u : 0u);
@@ -749,12 +754,14 @@ int launch_on(const skl_moe_problem *p, char *block) {
   moe_router_kernel<<<grid, kRouterThreads, 0, st>>>(a);
   int rc = skl_check_launch("moe_router");
   if (rc != 0) return rc;
-  const size_t want = p->experts > 64 * p->tokens ? p->experts : 64 * p->tokens;
+  const bool four = p->tokens > 16 && p->top_k <= 16 && p->experts <= 128;  // tokens to a wave
+  const size_t lanes = (four ? 16 : 64) * p->tokens, want = p->experts > lanes ? p->experts : lanes;
   const unsigned threads = want < kRouterThreads ? (unsigned)(want + 63) / 64 * 64 : kRouterThreads;
-  if (p->experts <= 64) moe_choice_kernel<1><<<1, threads, 0, st>>>(a);
-  else if (p->experts <= 128) moe_choice_kernel<2><<<1, threads, 0, st>>>(a);
-  else if (p->experts <= 256) moe_choice_kernel<4><<<1, threads, 0, st>>>(a);
-  else moe_choice_kernel<16><<<1, threads, 0, st>>>(a);
+  if (four && p->experts <= 64) moe_choice_kernel<16, 4><<<1, threads, 0, st>>>(a);
+  else if (four) moe_choice_kernel<16, 8><<<1, threads, 0, st>>>(a);
+  else if (p->experts <= 64) moe_choice_kernel<64, 1><<<1, threads, 0, st>>>(a);
+  else if (p->experts <= 256) moe_choice_kernel<64, 4><<<1, threads, 0, st>>>(a);
+  else moe_choice_kernel<64, 16><<<1, threads, 0, st>>>(a);
   rc = skl_check_launch("moe_choice");
   if (rc != 0) return rc;
   rc = token_groups(p) == 1 ? launch_products<1>(a, slots) : launch_products<2>(a, slots);
