@@ -224,8 +224,8 @@ __global__ void __launch_bounds__(kRouterThreads) moe_choice_kernel(MoeArgs a) {
 // The two products. A workgroup of eight waves has 64 CG rows of one expert's weights - columns of the result - and up to 16 RG of its tokens at a time. K comes in
 // chunks of 256, a line of a row of weights and four (TERMS times) of a token, from memory to LDS without registers, whole lines at a time, a few chunks ahead. Four
 // pairs of waves have 16 CG rows of weights each; of a pair, each has its half of every chunk, so that a token is read from LDS four times and not eight.
-// 64 tokens, 2 of 8 experts of 14336 x 4096: 113 us for h (500 MB of weights, 4.4 TB/s) and 94 for the output products (250 MB and three terms of h, of which each
-// workgroup has to have all: 2.7 TB/s). Read straight into registers as the operands lie - 16 lines for 1024 bytes, and as many for every token's - the compute
+// 64 tokens, 2 of 8 experts of 14336 x 4096: 113 us for h (500 MB of weights, 4.4 TB/s) and 94 to 110 for the output products (250 MB and three terms of h, of which
+// each workgroup has to have all; the more, the more experts have over 16 tokens). Read straight into registers as the operands lie - 16 lines for 1024 bytes, and as many for every token's - the compute
 // units' address paths bound them: 193 and 205 us. 7 tokens, 3 of 20 experts of 1440 x 2080: 16.6 and 11.4 us; 1 token, 4 of 32 of 1024 x 2048: 7.8 and 5.6, most of
 // it the way to a launch's first bytes. There, with one group of 16 tokens, a wave reads a chunk's operands together (step by step, below, 17.7 and 8.4 us for h);
 // weights past the caches took 20 us at 7 tokens, whose rows of 1040 bytes share lines.
