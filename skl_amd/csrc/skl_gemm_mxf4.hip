@@ -15,6 +15,7 @@
 #include "skl_device.hpp"
 #include "skl_kcstream.hpp"
 #include "skl_mx.h"
+#include "skl_mx_rows.hpp"
 #include "../../include/skl-hip.h"
 
 namespace {
@@ -150,9 +151,9 @@ enum { kThrough, kPast, kRead, kAny };  // stored through the caches or past the
 template <int HOW, bool EDGE, int TM, int TN>
 __device__ __forceinline__ void write_rows(const MxArgs &p, const v16f (&sum)[TN][TM], unsigned row0, unsigned col0, unsigned rows, unsigned cols, int lane, char *space) {
   const int l = lane & 31, half = lane >> 5;
-  constexpr int kLanes = 8 * TN, kRowsAt = 64 / kLanes, kPasses = 32 / kRowsAt;  // lanes that hold a row, rows of a pass, passes per row of blocks
-  const unsigned at_row = (unsigned)lane / kLanes, at_col = (unsigned)lane % kLanes * 4u;
-  float *const first = p.c + (size_t)(row0 + at_row) * p.rsc + (size_t)(col0 + at_col) * p.csc;
+  constexpr int kRowsAt = MxRows<TN>::kRowsAt, kPasses = MxRows<TN>::kPasses;
+  const MxRows<TN> mine(p.c + (size_t)row0 * p.rsc + (size_t)col0 * p.csc, p.rsc, p.csc, (unsigned)lane);
+  const unsigned at_row = mine.at_row, at_col = mine.at_col;
   const bool init = skl_beta_is_zero<float>(p.beta);
 #pragma unroll
   for (int i = 0; i < TM; ++i) {
@@ -170,7 +171,7 @@ __device__ __forceinline__ void write_rows(const MxArgs &p, const v16f (&sum)[TN
         const v4f v = *reinterpret_cast<const v4f *>(from + n * kRowsAt * kRowPitch<TN>);
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          if (r + at_row < rows && at_col + e < cols) skl_update(v[e], first + (size_t)r * p.rsc + (size_t)e * p.csc, p.alpha, p.beta);
+          if (mine.exists(r, rows) && at_col + e < cols) skl_update(v[e], mine.row(r) + (size_t)e * p.csc, p.alpha, p.beta);
       }
     } else {
       constexpr int kBatch = kPasses < 8 ? kPasses : 8;  // old values under way together
@@ -182,7 +183,7 @@ __device__ __forceinline__ void write_rows(const MxArgs &p, const v16f (&sum)[TN
 #pragma unroll
           for (int n = 0; n < kBatch; ++n) {
             const unsigned r = 32u * i + (unsigned)(n0 + n) * kRowsAt;
-            const float *const there = r + at_row < rows ? first + (size_t)r * p.rsc : first;
+            const float *const there = mine.readable(r, rows);
             if (EDGE && at_col + 4 > cols) {
 #pragma unroll
               for (int e = 0; e < 4; ++e) old[n][e] = at_col + e < cols ? there[e] : 0.0f;
@@ -200,8 +201,8 @@ __device__ __forceinline__ void write_rows(const MxArgs &p, const v16f (&sum)[TN
             v[e] = HOW != kRead ? skl_initialise_plain(v[e], p.alpha, p.beta)
                    : init       ? skl_initialise_with(v[e], old[n][e], p.alpha, p.beta)
                                 : skl_combine(v[e], old[n][e], p.alpha, p.beta);
-          if (r + at_row >= rows) continue;
-          float *const to = first + (size_t)r * p.rsc;
+          if (!mine.exists(r, rows)) continue;
+          float *const to = mine.row(r);
           if (EDGE && at_col + 4 > cols) {
 #pragma unroll
             for (int e = 0; e < 3; ++e)
