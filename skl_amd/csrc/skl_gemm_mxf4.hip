@@ -209,7 +209,8 @@ __device__ __forceinline__ void write_rows(const MxArgs &p, const v16f (&sum)[TN
               if (at_col + e < cols) to[e] = v[e];
             continue;
           }
-          if constexpr (HOW == kPast) asm volatile("global_store_dwordx4 %0, %1, off nt" ::"v"(to), "v"(v) : "memory");  // (the compiler makes one of two branches that differ in this alone)
+          // (Assembly: the compiler makes one of two branches that differ in this alone. The store reads its data for two states more, which the compiler does not look after here.)
+          if constexpr (HOW == kPast) asm volatile("global_store_dwordx4 %0, %1, off nt\ns_nop 1" ::"v"(to), "v"(v) : "memory");
           else *reinterpret_cast<v4f_any *>(to) = v;
         }
       }
