@@ -443,7 +443,7 @@ void skl_gemm_mxf4e2m1r_mxf4e2m1c_f32rc_gfx950(size_t m, size_t n, size_t k, flo
  *   h_j = act(x gate_j^T) * (x up_j^T)                                    `inter` values, gate and up of expert j: inter x hidden
  *   y   = beta * residual + sum_j w_j * (h_j down_j^T)                    `hidden` values, down: hidden x inter
  * X, the logits' and all further products and sums are exact products summed in fp32; h, times its w, is held as the sum of three bf16
- * values, which is all of its 24 bits, and nothing is rounded to fewer. Weights are widened to bf16, exactly, for every scale byte from 0 on; one of 2^128 or
+ * values, which is all of its 24 bits (less those below 2^-133), up to the largest number and for infinities, and nothing is rounded to fewer. Weights are widened to bf16, exactly, for every scale byte from 0 on; one of 2^128 or
  * more (scale bytes 253 and 254) makes an infinity or a NaN of what it enters, a block with the byte 255 a NaN. Every sum's order depends
  * on the sizes and on who was chosen alone: the same call gives the same bits.
  * residual may be y (each with its own row distance), or NULL with beta == 0, where it is not read. Made for a few tokens: 64 at a

@@ -6,7 +6,7 @@
 // values, exact, summed in fp32. A lane's 16 bytes are one block of 32 k of one row of weights; which k of a chunk of 128 meet in which
 // of its four instructions is free as long as both operands' lanes take the same.
 // The tokens of an expert are gathered: only rows of tokens that chose it are multiplied, 16 at a time. h travels as the sum of three bf16
-// values, which is all of its 24 bits: two (7.6e-6 off at most) left y 1.0e-6 off, three 3e-7, and the stream covers the third's products.
+// values, eight of its 24 bits each (none below 2^-133, where bf16 ends): two left y 1.0e-6 off, three 3e-7, and the stream covers the third's products.
 //
 // Five launches: the router's sums, the choice, the two products, the weighted sum over a token's experts; but for the choice each with a workgroup per piece of work so
 // that the stream finds every compute unit. Every sum has a fixed order.
@@ -56,6 +56,8 @@ __device__ __forceinline__ v8bf widen_f4(unsigned w, float scale) {  // eight E2
 }
 __device__ __forceinline__ unsigned short bf16_of(float v) { return __builtin_bit_cast(unsigned short, (__bf16)v); }  // to nearest even
 __device__ __forceinline__ float of_bf16(unsigned short v) { return __uint_as_float((unsigned)v << 16); }
+__device__ __forceinline__ unsigned short upper_half(float v) { return (unsigned short)(__float_as_uint(v) >> 16); }  // as a bf16 value: v cut off
+__device__ __forceinline__ bool is_number(float v) { return (__float_as_uint(v) & 0x7F800000u) != 0x7F800000u; }
 
 // A logit as a number that orders like it: NaN lowest, the two zeros alike; 0 is none.
 __device__ __forceinline__ unsigned order_of(float v) {
@@ -608,9 +610,11 @@ __global__ void __launch_bounds__(kThreads) moe_in_kernel(MoeArgs a) {
       if (j >= cols) continue;
       const unsigned place = own.first + done + i;
       const float h = skl_activate(red[i][j], p.activation) * red[i][kCols + j] * a.r.weight[place];
-      const unsigned short t0 = bf16_of(h);
-      const float rest = h - of_bf16(t0);
-      const unsigned short t1 = bf16_of(rest);
+      // Its bits from the top, eight to a term: none is larger than what is left, so that neither a term nor a sum of the first two is an infinity where h is none. (The nearest
+      // bf16 value is, from 2^128 - 2^119 on.) An infinity or a NaN - the arithmetic's have their upper half's bits set - has no other terms.
+      const unsigned short t0 = upper_half(h);
+      const float rest = is_number(h) ? h - of_bf16(t0) : 0.0f;
+      const unsigned short t1 = upper_half(rest);
       const size_t to = (size_t)place * p.inter + col0 + j;
       a.r.h[0][to] = t0;
       a.r.h[1][to] = t1;
