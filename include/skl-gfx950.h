@@ -446,8 +446,8 @@ void skl_gemm_mxf4e2m1r_mxf4e2m1c_f32rc_gfx950(size_t m, size_t n, size_t k, flo
  * values, which is all of its 24 bits (less those below 2^-133), up to the largest number and for infinities, and nothing is rounded to fewer. Weights are widened to bf16, exactly, for every scale byte from 0 on; one of 2^128 or
  * more (scale bytes 253 and 254) makes an infinity or a NaN of what it enters, a block with the byte 255 a NaN. Every sum's order depends
  * on the sizes and on who was chosen alone: the same call gives the same bits.
- * residual may be y (each with its own row distance), or NULL with beta == 0, where it is not read. Made for a few tokens: 64 at a
- * time, and an expert's weights once for every 16 of its tokens - 32 where there are more than eight to an expert on average.
+ * residual may be y with the same row distance (of more than one token; any other is refused), or NULL with beta == 0, where it is not read; otherwise it and y do not overlap, and
+ * rows of both are hidden values apart at least. Made for a few tokens: 64 at a time, and an expert's weights once for every 16 of its tokens - 32 where there are more than eight to an expert on average.
  * hidden and inter are multiples of 32 and at most 2^24; experts <= 1024, top_k <= experts, top_k <= 64; every row of weights, of the router and of X begins on a
  * 16-byte boundary (pointers and distances); ld_in and ld_down are at most 2^24, ldx at most 2^23; anything else is SKL_HIP_ERR_BAD_ARGUMENT, and nothing is done. */
 typedef struct skl_gfx950_moe {

@@ -172,6 +172,12 @@ static int moe_ok(const skl_gfx950_moe_t *l, size_t tokens, const void *x, size_
   return 1;
 }
 
+/* More than one token: rows do not run into each other, and a residual that is y has its rows where y's are: it is read while other rows of y are written. */
+static int rows_of_y_ok(size_t hidden, float beta, const float *residual, size_t ld_residual, const float *y, size_t ldy) {
+  if (ldy < hidden) return 0;
+  return beta == 0.0f || (ld_residual >= hidden && (residual != y || ld_residual == ldy));
+}
+
 static int moe_on_device(const skl_gfx950_moe_t *l, size_t tokens, const void *x, size_t ldx, float beta, const float *residual,
                          size_t ld_residual, float *y, size_t ldy) {
   size_t t;
@@ -205,7 +211,7 @@ void skl_moe_bf16_mxf4e2m1_f32_gfx950(const skl_gfx950_moe_t *layer, size_t toke
   const skl_gfx950_moe_t *l = layer;
   int where;
   if (tokens == 0) return;
-  if (!l || !moe_ok(l, tokens, x, ldx, beta, residual, y) || (tokens > 1 && (ldy < l->hidden || (beta != 0.0f && ld_residual < l->hidden)))) {
+  if (!l || !moe_ok(l, tokens, x, ldx, beta, residual, y) || (tokens > 1 && !rows_of_y_ok(l->hidden, beta, residual, ld_residual, y, ldy))) {
     bad_argument(__func__);
     return;
   }
