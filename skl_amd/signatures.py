@@ -61,6 +61,10 @@ class MoeStruct(ctypes.Structure):
         ("activation", ctypes.c_int), ("normalise", ctypes.c_int), ("ids", ctypes.c_void_p), ("weights", ctypes.c_void_p)]
 
 
+#: What the pointer at such a position points to.
+STRUCTS = {"E": EpilogueStruct, "M": MoeStruct}
+
+
 def _rc(s):      # m n k alpha a rsa csa b rsb csb beta c rsc csc
     return "zzz" + s + "pzz" + "pzz" + s + "pzz"
 
