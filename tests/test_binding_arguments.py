@@ -68,3 +68,35 @@ def test_descriptors_are_of_their_own_kind():
 def test_the_number_of_arguments():
     with pytest.raises(TypeError, match="expected 9 arguments, got 8"):
         skl_amd.load().skl_moe_bf16_mxf4e2m1_f32_gfx950(None, 0, None, 4, 0.0, None, 0, None)
+
+
+def test_every_argument_is_looked_at_once():
+    """Also where some are addresses, others buffers, halves or descriptors: none is converted, found wanting and converted again."""
+    lib, looked = skl_amd.load(), []
+
+    class Counted(Buffer):
+        @property
+        def ptr(self):
+            looked.append("buffer")
+            return 4096
+
+        @ptr.setter
+        def ptr(self, value):
+            pass
+
+    class Half:
+        def __float__(self):
+            looked.append("half")
+            return 1.5
+
+    class CountedEpilogue(Epilogue):
+        def as_struct(self):
+            looked.append("epilogue")
+            return super().as_struct()
+
+    a = Counted()
+    lib.skl_gemm_f16_f16_f16_gfx950(0, 4, 4, Half(), 4096, 4, a, 4, Half(), np.zeros(4, np.float16), 4)
+    assert sorted(looked) == ["buffer", "half", "half"]
+    looked.clear()
+    lib.skl_gemm_fused_i8rc_i8rc_i32rc_gfx950(0, 4, 4, 1, a, 4, 1, 4096, 4, 1, 0, np.zeros(4, np.int32), 4, 1, CountedEpilogue())
+    assert sorted(looked) == ["buffer", "epilogue"]
