@@ -336,19 +336,18 @@ __global__ void __launch_bounds__(256) cvt_from_mx_kernel(const uint8_t *__restr
   }
 }
 
-// Rows in slabs whose blocks a 32-bit number counts. f(first row, rows, blocks of the slab)
+// Rows in slabs whose blocks a 32-bit number counts, rows longer than that in pieces; four threads to a block, of which a launch has less than 2^32.
+// f(first row, first value, values of a row here, blocks here)
+constexpr size_t kMostBlocks = (size_t)1 << 29;
 template <class F>
 int in_slabs(size_t m, size_t k, F f) {
-  const size_t blocks = (k + 31) / 32, most = (size_t)1 << 30;
-  if (blocks > most) {
-    skl_hip_record_error(-2, "MXFP4 conversion: row too long");
-    return -2;
-  }
-  const size_t rows = most / blocks;
-  for (size_t i = 0; i < m; i += rows) {
-    const size_t here = m - i < rows ? m - i : rows;
-    const int rc = f(i, here, (unsigned)(here * blocks));
-    if (rc != 0) return rc;
+  for (size_t p = 0; p < k; p += kMostBlocks * 32) {
+    const size_t values = k - p < kMostBlocks * 32 ? k - p : kMostBlocks * 32, blocks = (values + 31) / 32, rows = kMostBlocks / blocks;
+    for (size_t i = 0; i < m; i += rows) {
+      const size_t here = m - i < rows ? m - i : rows;
+      const int rc = f(i, p, values, (unsigned)(here * blocks));
+      if (rc != 0) return rc;
+    }
   }
   return 0;
 }
@@ -358,10 +357,10 @@ constexpr unsigned kFewBlocks = 64u * 4u * 512u;
 
 template <class Eight>
 int launch_rows(size_t m, size_t k, const typename Eight::T *src, size_t rs, size_t cs, uint8_t *codes, size_t ld, uint8_t *scales, size_t lds) {
-  const unsigned blocks = (unsigned)((k + 31) / 32);
-  return in_slabs(m, k, [&](size_t i, size_t, unsigned all) {
-    const typename Eight::T *s = src + i * rs;
-    uint8_t *c = codes + i * (ld / 2), *sc = scales + i * lds;
+  return in_slabs(m, k, [&](size_t i, size_t p, size_t k, unsigned all) {
+    const unsigned blocks = (unsigned)((k + 31) / 32);
+    const typename Eight::T *s = src + i * rs + p * cs;
+    uint8_t *c = codes + i * (ld / 2) + p / 2, *sc = scales + i * lds + p / 32;
     hipStream_t st = skl_current_stream();
     if (cs != 1) cvt_to_mx_rows_kernel<Eight, 1, false><<<skl_div_up(all, 64), 256, 0, st>>>(s, rs, cs, blocks, all, k, c, ld / 2, sc, lds);
     else if (all <= kFewBlocks) cvt_to_mx_rows_kernel<Eight, 1, true><<<skl_div_up(all, 64), 256, 0, st>>>(s, rs, cs, blocks, all, k, c, ld / 2, sc, lds);
@@ -372,19 +371,15 @@ int launch_rows(size_t m, size_t k, const typename Eight::T *src, size_t rs, siz
 
 template <class T>
 int launch_columns(size_t m, size_t k, const T *src, size_t cs, uint8_t *codes, size_t ld, uint8_t *scales, size_t lds) {
-  const size_t most = (size_t)65535 * kAcrossRows;  // rows of a grid
-  const size_t gx = (k + kAcrossK - 1) / kAcrossK;
-  if (gx > 0x7FFFFFFFu) {
-    skl_hip_record_error(-2, "MXFP4 conversion: row too long");
-    return -2;
-  }
-  for (size_t i = 0; i < m; i += most) {
-    const size_t here = m - i < most ? m - i : most;
-    cvt_to_mx_columns_kernel<T><<<dim3((unsigned)gx, skl_div_up(here, kAcrossRows)), kAcrossThreads, 0, skl_current_stream()>>>(
-        src + i, cs, here, k, codes + i * (ld / 2), ld / 2, scales + i * lds, lds);
-    const int rc = skl_check_launch("cvt_to_mx_columns");
-    if (rc != 0) return rc;
-  }
+  constexpr size_t kMostRows = (size_t)65535 * kAcrossRows, kMostK = (size_t)1 << 30;  // of a grid: two threads to a value of k, less than 2^32
+  for (size_t p = 0; p < k; p += kMostK)
+    for (size_t i = 0; i < m; i += kMostRows) {
+      const size_t values = k - p < kMostK ? k - p : kMostK, here = m - i < kMostRows ? m - i : kMostRows;
+      cvt_to_mx_columns_kernel<T><<<dim3(skl_div_up(values, kAcrossK), skl_div_up(here, kAcrossRows)), kAcrossThreads, 0, skl_current_stream()>>>(
+          src + i + p * cs, cs, here, values, codes + i * (ld / 2) + p / 2, ld / 2, scales + i * lds + p / 32, lds);
+      const int rc = skl_check_launch("cvt_to_mx_columns");
+      if (rc != 0) return rc;
+    }
   return 0;
 }
 
@@ -402,17 +397,17 @@ extern "C" int skl_hip_launch_cvt_to_mx(int dt, size_t m, size_t k, const void *
 }
 
 extern "C" int skl_hip_launch_cvt_from_mx(int dt, size_t m, size_t k, const skl_mx_operand *src, void *dst, size_t rs, size_t cs) {
-  const unsigned blocks = (unsigned)((k + 31) / 32);
-  return in_slabs(m, k, [&](size_t i, size_t, unsigned all) {
-    const uint8_t *c = src->codes + i * (src->ld / 2), *sc = src->scales + i * src->lds;
+  return in_slabs(m, k, [&](size_t i, size_t p, size_t k, unsigned all) {
+    const unsigned blocks = (unsigned)((k + 31) / 32);
+    const uint8_t *c = src->codes + i * (src->ld / 2) + p / 2, *sc = src->scales + i * src->lds + p / 32;
     hipStream_t st = skl_current_stream();
     const unsigned grid = skl_div_up(all, 128);
     if (dt == SKL_DT_F32) {
-      float *d = static_cast<float *>(dst) + i * rs;
+      float *d = static_cast<float *>(dst) + i * rs + p * cs;
       if (cs == 1) cvt_from_mx_kernel<float, true><<<grid, 256, 0, st>>>(c, src->ld / 2, sc, src->lds, blocks, all, k, d, rs, cs);
       else cvt_from_mx_kernel<float, false><<<grid, 256, 0, st>>>(c, src->ld / 2, sc, src->lds, blocks, all, k, d, rs, cs);
     } else {
-      uint16_t *d = static_cast<uint16_t *>(dst) + i * rs;
+      uint16_t *d = static_cast<uint16_t *>(dst) + i * rs + p * cs;
       if (cs == 1) cvt_from_mx_kernel<uint16_t, true><<<grid, 256, 0, st>>>(c, src->ld / 2, sc, src->lds, blocks, all, k, d, rs, cs);
       else cvt_from_mx_kernel<uint16_t, false><<<grid, 256, 0, st>>>(c, src->ld / 2, sc, src->lds, blocks, all, k, d, rs, cs);
     }
