@@ -1035,9 +1035,9 @@ int configure(const void *kernel, int bytes, std::atomic<bool> &done) {  // raci
 
 size_t tiles_of(const MxArgs &p, size_t rows, size_t cols) { return (p.m + rows - 1) / rows * ((p.n + cols - 1) / cols); }
 
-// The grid for tiles of `rows` x `cols`, or 0 with the error recorded.
+// The grid for tiles of `rows` x `cols`, or 0 with the error recorded: 256 threads to a tile, of which a launch has less than 2^32.
 unsigned grid_for(MxArgs &p, unsigned rows, unsigned cols) {
-  if (tiles_of(p, rows, cols) > 0x7FFFFFFFu) {
+  if (tiles_of(p, rows, cols) >= 1u << 24) {
     skl_hip_record_error(SKL_HIP_ERR_BAD_ARGUMENT, "gemm_mx: grid too large");
     return 0;
   }
@@ -1144,13 +1144,7 @@ int launch_kind(const MxArgs &p, Kind kind) {
   }
 }
 
-}  // namespace
-
-extern "C" int skl_hip_launch_gemm_mx(const skl_mx_gemm *g) {
-  if (g->m > 0x7FFFFFFFu || g->n > 0x7FFFFFFFu) {
-    skl_hip_record_error(SKL_HIP_ERR_BAD_ARGUMENT, "gemm_mx: more than 2^31 rows or columns");
-    return SKL_HIP_ERR_BAD_ARGUMENT;
-  }
+int launch_slab(const skl_mx_gemm *g) {
   MxArgs p = {g->a.codes, g->b.codes, g->a.ld / 2, g->b.ld / 2, g->a.scales, g->b.scales, g->a.lds, g->b.lds, g->c, g->rsc, g->csc,
               (unsigned)g->m, (unsigned)g->n, g->k, g->alpha, g->beta, 0, 0, 0, nullptr, nullptr};
   // C through the caches or past them (us): 8192 x 8192 x 8192 314 / 292, x 256 106 / 103; 4096 x 8192 x 4096 109.6 / 112.7, x 256 40.6 / 49.8.
@@ -1199,4 +1193,24 @@ extern "C" int skl_hip_launch_gemm_mx(const skl_mx_gemm *g) {
   }
   skl_hip_sequence_end();
   return rc;
+}
+
+}  // namespace
+
+// In slabs of 2^28 rows and columns, so that the tiles fit a launch also where they are mostly empty (one column, or one row).
+extern "C" int skl_hip_launch_gemm_mx(const skl_mx_gemm *g) {
+  constexpr size_t kMost = (size_t)1 << 28;
+  for (size_t i = 0; i < g->m; i += kMost)
+    for (size_t j = 0; j < g->n; j += kMost) {
+      skl_mx_gemm slab = *g;
+      slab.m = g->m - i < kMost ? g->m - i : kMost, slab.n = g->n - j < kMost ? g->n - j : kMost;
+      if (g->k != 0) {
+        slab.a.codes += i * (g->a.ld / 2), slab.a.scales += i * g->a.lds;
+        slab.b.codes += j * (g->b.ld / 2), slab.b.scales += j * g->b.lds;
+      }
+      slab.c += i * g->rsc + j * g->csc;
+      const int rc = launch_slab(&slab);
+      if (rc != 0) return rc;
+    }
+  return 0;
 }
