@@ -52,3 +52,38 @@ def test_an_infinite_h_makes_infinities(gpu, tokens):
     got = run(gpu, x, codes, scales, hidden, inter)
     want = np.where(codes["down"][:, 5] & MINUS, np.inf, -np.inf)
     assert np.array_equal(got, np.tile(want, (tokens, 1)).astype(np.float32))
+
+
+def cut(h, terms):
+    """What `terms` bf16 values, rounded to the nearest one after the other, hold of whole numbers h."""
+    kept, rest = np.zeros(h.shape), h.astype(np.float64)
+    for _ in range(terms):
+        m, e = np.frexp(rest)
+        term = np.ldexp(np.rint(m * 256), e - 8)
+        kept, rest = kept + term, rest - term
+    return kept
+
+
+@pytest.mark.parametrize("exponent", (0, 60, -120, -133))  # of h's last bit: 2^-133 is the smallest that bf16 has
+@pytest.mark.parametrize("tokens,hidden,inter", ((1, 32, 32), (5, 64, 96), (33, 96, 288), (50, 32, 1056)))
+def test_all_bits_of_h_arrive(gpu, tokens, hidden, inter, exponent):
+    """h = (x gate) (x up) of small whole numbers, up to 24 bits; a row of `down` gives back one of its columns, times 1 or -1, to the bit. (Two terms would
+    not do: checked on the host.)"""
+    rng = np.random.default_rng(inter + tokens)
+    codes, scales = parts(hidden, inter)
+    whole = np.array([0, 2, 4, 5, 6], np.uint8)  # 0, 1, 2, 3, 4
+    for name in ("gate", "up"):
+        codes[name][:] = rng.choice(whole, size=codes[name].shape) | rng.choice(np.array([0, MINUS], np.uint8), size=codes[name].shape)
+    value = {2: 1, 4: 2, 5: 3, 6: 4, 0: 0}
+    w = {n: np.vectorize(lambda c: value[c & 7] * (-1 if c & 8 else 1))(codes[n]).astype(np.int64) for n in ("gate", "up")}
+    most = int(550 / np.sqrt(hidden))  # so that a sum stays below 2^12, four and a half deviations out
+    x = rng.integers(-most, most + 1, size=(tokens, hidden))
+    h = (x @ w["gate"].T) * (x @ w["up"].T)
+    assert np.abs(h).max() < 2 ** 24 and (cut(h, 2) != h).any() and np.array_equal(cut(h, 3), h)
+    column = rng.integers(0, inter, size=hidden)
+    column[:4] = np.argsort(-np.abs(cut(h, 2) - h).max(axis=0))[:4]  # what the last term matters to is among them
+    sign = rng.choice([1, -1], size=hidden)
+    codes["down"][np.arange(hidden), column] = np.where(sign > 0, ONE, ONE | MINUS)
+    scales["gate"][:], scales["up"][:] = 127 + exponent // 2, 127 + exponent - exponent // 2
+    got = run(gpu, x.astype(np.float32), codes, scales, hidden, inter)
+    assert np.array_equal(got.astype(np.float64), np.ldexp((h[:, column] * sign).astype(np.float64), exponent))
