@@ -403,7 +403,9 @@ void skl_cvt_f4e2m1_f8e4m3_gfx950(uint8_t *dst, const uint8_t *src, size_t n);
  * columns of a row-major matrix - the transposed operand that a layer's gradients multiply. With a the largest magnitude of
  * a block, its scale is 2^s, s = max(floor(log2 a) - 2, -126), and a value x becomes the E2M1 value nearest to x / 2^s,
  * ties to the even code, 6 in magnitude at most, the sign of a zero kept. A block of zeros has s = -126; one that holds a NaN or an infinity
- * gets the scale byte 255 and codes 0. Every scale byte written otherwise lies in [1, 252]. With an odd k the half byte behind a
+ * gets the scale byte 255 and codes 0. Every scale byte written otherwise lies in [1, 252]. (The formats' own floor is s = -127, the byte 0, which everything here
+ * that reads scales takes; what is written ends at 2^-126, fp32's smallest normal number, so that a scale is a normal number wherever it is held as one. It
+ * concerns blocks whose largest magnitude is below 2^-124 alone: their values are multiples of 2^-127, not 2^-128.) With an odd k the half byte behind a
  * row's last value is written as 0; nothing else outside the m x k values and their scales is written. */
 void skl_cvt_f32rc_mxf4e2m1_gfx950(size_t m, size_t k, const float *src, size_t rs, size_t cs, uint8_t *dst, size_t ldd,
                                    uint8_t *scales, size_t lds);
@@ -419,8 +421,10 @@ void skl_cvt_mxf4e2m1_bf16rc_gfx950(size_t m, size_t k, const uint8_t *src, size
 
 /* C = alpha * A * B + beta * C of two MXFP4 operands: A's rows and B's columns are K-contiguous (B is stored column by column,
  * as a linear layer's [out][in] weight is), n columns of B as rows of an MXFP4 matrix. alpha, beta, C and the empty cases as in
- * skl_gemm_f32rc_f32rc_f32rc_gfx950. Products are exact, sums are in fp32 on the matrix cores, in an order that depends on the sizes
- * and layouts alone; the result is that of ref/gemm/gemm_f32rc_f32rc_f32rc.h:44 on the decoded operands, inside its error bound.
+ * skl_gemm_f32rc_f32rc_f32rc_gfx950. Products are exact, sums are in fp32 on the matrix cores, results
+ * below 2^-126 included. The order of a sum depends on the sizes, on the layouts and the boundaries that operands and their rows begin on, and on whether the
+ * stream holds scratch memory: without it - more than 32 streams, or no room - K is not shared and operands are not copied onto lines, which is another order. The same call in
+ * the same place gives the same bits; the result is that of ref/gemm/gemm_f32rc_f32rc_f32rc.h:44 on the decoded operands, inside its error bound.
  * A block whose scale byte is 255 makes NaN of what it enters; every other byte is a scale, 0 (2^-127) included.
  * A layer in training multiplies three times, each operand quantised along the axis that the product sums over:
  *   y (m x n)  = A B            A: x by rows,        B: W by rows

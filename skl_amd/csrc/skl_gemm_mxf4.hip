@@ -1125,6 +1125,8 @@ int launch_rows(const MxArgs &p) {
 //   128 x 128 tiles where there is one per compute unit and K is not short (2048 x 4096 x 4096 25.8, 64 x 64 tiles 42, x 256 14 / 10; 2048 x 2048 x 8192 31 / 42;
 //   1024 x 1024 x 4096, 64 of them, 16.9 / 11.2);
 //   else 64 x 64 tiles.
+// The figures are for whole rounds of tiles, one 256 x 256 or two 128 x 128 tiles to a compute unit, or for less than one round; between 257 and some 400 large tiles, whose second round
+// is mostly empty, neither side was measured.
 enum Kind { kWide4, kWide2, kRows, kSmall };
 Kind kind_of(const MxArgs &p) {
   if (p.m <= 64 && p.k >= 256 && rows_scale_bytes(row_groups(p), skl_kcstream::column_groups(p.n), p.k) <= (size_t)kRowsScaleSpace) return kRows;

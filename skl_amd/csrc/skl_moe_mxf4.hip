@@ -182,7 +182,7 @@ __global__ void __launch_bounds__(kRouterThreads) moe_router_kernel(MoeArgs a) {
 
 // The choice: one workgroup, of a wave per token or, for many tokens and not too many experts, per four, and a thread per expert, as far as there are that many. 3.5 us for 1
 // token, for 64 tokens 5.8 (4 of 20 experts) and 11 (8 of 128; 10 and 22 with a wave per token), 54 of 512, bound by what follows one another: the sums read back, top_k rounds of
-// two maxima, a scan. (Behind a counter in the router's last workgroup the layer took as long, to 2 %.)
+// two maxima, a scan; beyond 256 experts, with 16 logits and their keys to a lane, 15 of the 128 registers that 1024 threads leave are in scratch memory besides. (Behind a counter in the router's last workgroup the layer took as long, to 2 %.)
 template <int G, int NE>
 __global__ void __launch_bounds__(kRouterThreads) moe_choice_kernel(MoeArgs a) {
   __shared__ Choice c;
