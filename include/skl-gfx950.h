@@ -474,6 +474,90 @@ typedef struct skl_gfx950_moe {
 void skl_moe_bf16_mxf4e2m1_f32_gfx950(const skl_gfx950_moe_t *layer, size_t tokens, const skl_bf16_t *x, size_t ldx, float beta,
                                       const float *residual, size_t ld_residual, float *y, size_t ldy);
 
+/* ======================================================================== */
+/* Products grouped by expert                                                */
+/* ======================================================================== */
+
+/* Rows that belong to the same expert lie side by side: group e's are rows offsets[e] to offsets[e + 1] - 1, a group may be empty, and only the GPU
+ * needs to know how long each is. The reference has no such products; each of them is, on its group's rows, the one of
+ * ref/gemm/gemm_f32rc_f32rc_f32rc.h:44 on the widened operands.
+ *
+ * The order: pick i of `count` chose group ids[i] (token t's j-th choice of top_k is pick t * top_k + j). Picks are put in the order of their groups,
+ * those of one group in their own order; a pick whose id is outside [0, groups) belongs to none.
+ *   offsets[e], e = 0 .. groups   where group e begins; offsets[groups] is how many picks belong to a group
+ *   order[p]                      the pick at place p
+ *   rows[p]                       order[p] / per_row: its token, with per_row = top_k
+ *   place[i]                      the place of pick i, -1 where it belongs to no group
+ * order, rows and place have `count` values and may be NULL; of order and rows, what lies from place offsets[groups] on is left as it was. groups is 1
+ * to 4096, count at most 2^30, per_row at least 1; none of the arrays overlap. Every result is the same on every run. */
+void skl_group_rows_gfx950(size_t count, const int32_t *ids, size_t per_row, size_t groups, int32_t *offsets, int32_t *order, int32_t *rows,
+                           int32_t *place);
+
+/* C[i][j] = alpha * sum_p A[r(i)][p] * B_e[p][j] + beta * C[i][j] for the rows i of every group e; r(i) = rows[i], or i where rows is NULL.
+ * A is row-major, `a_rows` rows (rows == NULL: m) rsa apart; B_e(p, j) at b[e * gsb + p * rsb + j * csb], any strides; C is row-major, m rows rsc apart. With
+ * weights W_e [out][in] a layer's output takes rsb = 1, csb = in; the gradient of its input, dX = dY W_e, takes rsb = in, csb = 1 (k = out, n = in).
+ * Rows of C in no group are left as they were. A row whose index is outside [0, a_rows) counts as zeros; the same index may come any number of times.
+ * offsets have to ascend; they are cut off at 0 and m, nothing outside C's m rows is written whatever they are, and which of its rows are written is open where
+ * they do not ascend. offsets may be NULL with groups == 1: all m rows are the group. groups is 1 to 4096; m, n, k and a_rows are at most 2^30.
+ * Products are exact, sums in fp32 on the matrix cores, the result rounded once where C has 16 bits. The order of a sum depends on k and the layouts and, through the
+ * tiles chosen, on groups, m and n, not on the offsets' values: the same call gives the same bits. k == 0: C = beta * C on the groups' rows. beta == 0 leaves C unread
+ * (an old C counts as +0) unless skl_hip_set_beta_zero_mode asks for the reference's evaluation. C overlaps neither A nor B. */
+void skl_gemm_grouped_bf16_bf16rc_f32_gfx950(size_t groups, const int32_t *offsets, size_t m, size_t n, size_t k, float alpha, const skl_bf16_t *a,
+                                             size_t rsa, const int32_t *rows, size_t a_rows, const skl_bf16_t *b, size_t rsb, size_t csb, size_t gsb,
+                                             float beta, float *c, size_t rsc);
+void skl_gemm_grouped_bf16_bf16rc_bf16_gfx950(size_t groups, const int32_t *offsets, size_t m, size_t n, size_t k, float alpha, const skl_bf16_t *a,
+                                              size_t rsa, const int32_t *rows, size_t a_rows, const skl_bf16_t *b, size_t rsb, size_t csb, size_t gsb,
+                                              float beta, skl_bf16_t *c, size_t rsc);
+void skl_gemm_grouped_f16_f16rc_f32_gfx950(size_t groups, const int32_t *offsets, size_t m, size_t n, size_t k, float alpha, const skl_f16_t *a,
+                                           size_t rsa, const int32_t *rows, size_t a_rows, const skl_f16_t *b, size_t rsb, size_t csb, size_t gsb,
+                                           float beta, float *c, size_t rsc);
+void skl_gemm_grouped_f16_f16rc_f16_gfx950(size_t groups, const int32_t *offsets, size_t m, size_t n, size_t k, float alpha, const skl_f16_t *a,
+                                           size_t rsa, const int32_t *rows, size_t a_rows, const skl_f16_t *b, size_t rsb, size_t csb, size_t gsb,
+                                           float beta, skl_f16_t *c, size_t rsc);
+
+/* C_e[i][j] = alpha * sum_r A[ra(r)][i] * B[rb(r)][j] + beta * C_e[i][j], the sum over the rows r of group e: the gradient of such a layer's weights,
+ * dW_e = dY^T X with A = dY, B = X. A has m columns and B n, both row-major; ra(r) = rows_a[r], or r where rows_a is NULL, likewise rb; of `total` rows in all
+ * (offsets are cut off at 0 and total; rows_a == NULL: A has them all). C_e(i, j) at c[e * gsc + i * rsc + j]. An empty group makes C_e = beta * C_e. Everything else as above:
+ * a row whose index is outside [0, a_rows) or [0, b_rows) counts as zeros, offsets may be NULL with groups == 1, total is at most 2^30. A sum is taken in the order of its
+ * rows' places in tiles whose size depends on m, n, groups and total alone. */
+void skl_gemm_groupedk_bf16c_bf16_f32_gfx950(size_t groups, const int32_t *offsets, size_t m, size_t n, size_t total, float alpha, const skl_bf16_t *a,
+                                             size_t rsa, const int32_t *rows_a, size_t a_rows, const skl_bf16_t *b, size_t rsb, const int32_t *rows_b,
+                                             size_t b_rows, float beta, float *c, size_t rsc, size_t gsc);
+void skl_gemm_groupedk_bf16c_bf16_bf16_gfx950(size_t groups, const int32_t *offsets, size_t m, size_t n, size_t total, float alpha, const skl_bf16_t *a,
+                                              size_t rsa, const int32_t *rows_a, size_t a_rows, const skl_bf16_t *b, size_t rsb, const int32_t *rows_b,
+                                              size_t b_rows, float beta, skl_bf16_t *c, size_t rsc, size_t gsc);
+void skl_gemm_groupedk_f16c_f16_f32_gfx950(size_t groups, const int32_t *offsets, size_t m, size_t n, size_t total, float alpha, const skl_f16_t *a,
+                                           size_t rsa, const int32_t *rows_a, size_t a_rows, const skl_f16_t *b, size_t rsb, const int32_t *rows_b,
+                                           size_t b_rows, float beta, float *c, size_t rsc, size_t gsc);
+void skl_gemm_groupedk_f16c_f16_f16_gfx950(size_t groups, const int32_t *offsets, size_t m, size_t n, size_t total, float alpha, const skl_f16_t *a,
+                                           size_t rsa, const int32_t *rows_a, size_t a_rows, const skl_f16_t *b, size_t rsb, const int32_t *rows_b,
+                                           size_t b_rows, float beta, skl_f16_t *c, size_t rsc, size_t gsc);
+
+/* Integer 4-bit weights with scales for groups of `group_k` values, [n][k] as a linear layer's weight is stored: weight (p, j) of matrix e is
+ *   (q - z) * s,   q   4-bit number e * expert + j * ld + p of `codes`, 0 to 15, two to a byte, the first in the low half,
+ *                  s   scales[e * expert_scales + j * ld_scales + p / group_k], of A's type,
+ *                  z   zeros at the same place, 0 to 255; zeros == NULL: 8.
+ * group_k is a multiple of 32, or k or more; k need not be a multiple of it. ld and expert are even (where there is more than one row, or matrix). */
+typedef struct skl_gfx950_u4 {
+  size_t group_k;
+  const uint8_t *codes;
+  size_t ld, expert; /* in values */
+  const void *scales;
+  const uint8_t *zeros;
+  size_t ld_scales, expert_scales;
+} skl_gfx950_u4_t;
+/* C = alpha * A * B_e + beta * C with such a B, the rest as in skl_gemm_grouped_bf16_bf16rc_f32_gfx950; groups == 1 and offsets == NULL is an ordinary layer. q - z is
+ * an integer that bf16 and f16 hold, its products with A are exact, they are summed in fp32 within 32 to 128 values of one group, and those sums are scaled and added up in fp32.
+ * Made for few rows: a group's codes are read once for up to 16 of its rows; more rows take more passes over them. */
+void skl_gemm_grouped_bf16_u4c_f32_gfx950(size_t groups, const int32_t *offsets, size_t m, size_t n, size_t k, float alpha, const skl_bf16_t *a, size_t rsa,
+                                          const int32_t *rows, size_t a_rows, const skl_gfx950_u4_t *b, float beta, float *c, size_t rsc);
+void skl_gemm_grouped_bf16_u4c_bf16_gfx950(size_t groups, const int32_t *offsets, size_t m, size_t n, size_t k, float alpha, const skl_bf16_t *a, size_t rsa,
+                                           const int32_t *rows, size_t a_rows, const skl_gfx950_u4_t *b, float beta, skl_bf16_t *c, size_t rsc);
+void skl_gemm_grouped_f16_u4c_f32_gfx950(size_t groups, const int32_t *offsets, size_t m, size_t n, size_t k, float alpha, const skl_f16_t *a, size_t rsa,
+                                         const int32_t *rows, size_t a_rows, const skl_gfx950_u4_t *b, float beta, float *c, size_t rsc);
+void skl_gemm_grouped_f16_u4c_f16_gfx950(size_t groups, const int32_t *offsets, size_t m, size_t n, size_t k, float alpha, const skl_f16_t *a, size_t rsa,
+                                         const int32_t *rows, size_t a_rows, const skl_gfx950_u4_t *b, float beta, skl_f16_t *c, size_t rsc);
+
 #ifdef __cplusplus
 }
 #endif

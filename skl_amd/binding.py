@@ -74,25 +74,38 @@ class Epilogue:
                                          _as_pointer(self.q_scale), int(self.q_format))
 
 
-class MoeLayer:
-    """A mixture-of-experts layer (`skl_gfx950_moe_t`, every member by its name there) for `skl_moe_bf16_mxf4e2m1_f32`. Pointers are
-    DeviceBuffers, numpy arrays, integer addresses or None; what they refer to is kept as long as the layer is. The C descriptor is
-    made once."""
+class _Members:
+    """A C descriptor from its members, every one by its name there. Pointers are DeviceBuffers, numpy arrays, integer addresses or None; what they
+    refer to is kept as long as the descriptor is. The C structure is made once."""
+
+    _STRUCT = None
 
     def __init__(self, **members):
-        fields = dict(signatures.MoeStruct._fields_)
+        fields = dict(self._STRUCT._fields_)
         unknown = set(members) - set(fields)
         if unknown:
-            raise TypeError(f"skl_gfx950_moe_t has no member {sorted(unknown)[0]}")
+            raise TypeError(f"{self._NAME} has no member {sorted(unknown)[0]}")
         self.members = members
-        self._struct = signatures.MoeStruct(**{name: _as_pointer(v) if fields[name] is ctypes.c_void_p else int(v) for name, v in members.items()})
+        self._struct = self._STRUCT(**{name: _as_pointer(v) if fields[name] is ctypes.c_void_p else int(v) for name, v in members.items()})
 
     def as_struct(self):
         return self._struct
 
 
+class MoeLayer(_Members):
+    """A mixture-of-experts layer (`skl_gfx950_moe_t`) for `skl_moe_bf16_mxf4e2m1_f32`."""
+
+    _STRUCT, _NAME = signatures.MoeStruct, "skl_gfx950_moe_t"
+
+
+class U4Weights(_Members):
+    """Integer 4-bit weights with scales for groups along k (`skl_gfx950_u4_t`) for the `skl_gemm_grouped_*_u4c_*` entry points."""
+
+    _STRUCT, _NAME = signatures.U4Struct, "skl_gfx950_u4_t"
+
+
 def _descriptor(x, struct):
-    """The C structure that an Epilogue or a MoeLayer stands for."""
+    """The C structure that an Epilogue, a MoeLayer or U4Weights stand for."""
     made = x.as_struct() if hasattr(x, "as_struct") else None
     if not isinstance(made, struct):
         raise TypeError(f"expected what describes a {struct.__name__}, got {type(x).__name__}")

@@ -1,0 +1,42 @@
+// skl_groups.hpp - what the kernels of the products grouped by expert share: which tile of which group a workgroup takes, elements of
+// 16 bits, and the last step of a result (not installed).
+#pragma once
+
+#include "skl_device.hpp"
+#include "skl_grouped.h"
+
+namespace {
+
+// Inclusive sum over the lanes of a wave up to this one.
+__device__ __forceinline__ unsigned skl_wave_scan(unsigned v) {
+#define SKL_SCAN_STEP(CTRL, ROWS) v += (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false)
+  SKL_SCAN_STEP(0x111, 0xf);  // from 1, 2, 4 and 8 lanes below in the row of 16
+  SKL_SCAN_STEP(0x112, 0xf);
+  SKL_SCAN_STEP(0x114, 0xf);
+  SKL_SCAN_STEP(0x118, 0xf);
+  SKL_SCAN_STEP(0x142, 0xa);  // the row's last lane to the next row
+  SKL_SCAN_STEP(0x143, 0xc);  // the lower half's last lane to the upper half
+#undef SKL_SCAN_STEP
+  return v;
+}
+
+// Rows first .. first + rows - 1 of a list of groups: group e's, cut off at 0 and `most`.
+struct SklRange {
+  unsigned first, rows;
+};
+__device__ __forceinline__ unsigned skl_cut(int at, unsigned most) { return at < 0 ? 0u : (unsigned)at < most ? (unsigned)at : most; }
+__device__ __forceinline__ SklRange skl_group_range(const int32_t *offsets, unsigned e, unsigned most) {
+  if (!offsets) return {0, most};
+  const unsigned b = skl_cut(offsets[e], most), f = skl_cut(offsets[e + 1], most);
+  return {b, f > b ? f - b : 0u};
+}
+
+__device__ __forceinline__ float skl_widen(uint16_t v, bool bf16) { return bf16 ? __uint_as_float((unsigned)v << 16) : (float)__builtin_bit_cast(_Float16, v); }
+
+// The result for one element of C: TC is float, __bf16 or _Float16; a 16-bit C is widened, combined in fp32 and rounded once, to the nearest.
+template <typename TC>
+__device__ __forceinline__ TC skl_grouped_result(float acc, const TC *c, skl_scalar alpha, skl_scalar beta, bool read_c) {
+  return (TC)(read_c ? skl_combine(acc, (float)*c, alpha, beta) : skl_initialise_plain(acc, alpha, beta));
+}
+
+}  // namespace

@@ -3,7 +3,7 @@
 Each character is one C parameter: ``z`` size_t, ``p`` pointer, ``i`` int32_t,
 ``f`` float, ``d`` double, ``b`` uint8_t, ``h`` uint16_t, ``w`` uint32_t,
 ``B`` bool,
-``H`` a ``_Float16`` passed by value, ``E`` a pointer to a ``skl_gfx950_epilogue_t``, ``M`` one to a ``skl_gfx950_moe_t``.
+``H`` a ``_Float16`` passed by value, ``E`` a pointer to a ``skl_gfx950_epilogue_t``, ``M`` one to a ``skl_gfx950_moe_t``, ``U`` one to a ``skl_gfx950_u4_t``.
 Names are given without the implementation suffix (``_gfx950`` for the GPU
 library); the parameter order is the reference's (include/skl-gfx950.h cites
 the prototype each one mirrors).
@@ -39,6 +39,7 @@ CTYPES = {
     "H": HalfByValue,
     "E": ctypes.c_void_p,
     "M": ctypes.c_void_p,
+    "U": ctypes.c_void_p,
 }
 
 
@@ -61,8 +62,14 @@ class MoeStruct(ctypes.Structure):
         ("activation", ctypes.c_int), ("normalise", ctypes.c_int), ("ids", ctypes.c_void_p), ("weights", ctypes.c_void_p)]
 
 
+class U4Struct(ctypes.Structure):
+    """``skl_gfx950_u4_t`` (include/skl-gfx950.h)."""
+    _fields_ = [("group_k", ctypes.c_size_t), ("codes", ctypes.c_void_p), ("ld", ctypes.c_size_t), ("expert", ctypes.c_size_t),
+                ("scales", ctypes.c_void_p), ("zeros", ctypes.c_void_p), ("ld_scales", ctypes.c_size_t), ("expert_scales", ctypes.c_size_t)]
+
+
 #: What the pointer at such a position points to.
-STRUCTS = {"E": EpilogueStruct, "M": MoeStruct}
+STRUCTS = {"E": EpilogueStruct, "M": MoeStruct, "U": U4Struct}
 
 
 def _rc(s):      # m n k alpha a rsa csa b rsb csb beta c rsc csc
@@ -193,6 +200,12 @@ def gfx950_only():
         sigs[f"skl_cvt_mxf4e2m1_{src}rc"] = "zzpzpzpzz"
     sigs["skl_gemm_mxf4e2m1r_mxf4e2m1c_f32rc"] = "zzzfpzpzpzpzfpzz"     # m n k alpha a lda sa lsa b ldb sb lsb beta c rsc csc
     sigs["skl_moe_bf16_mxf4e2m1_f32"] = "Mzpzfpzpz"                     # layer tokens x ldx beta residual ld y ldy
+    sigs["skl_group_rows"] = "zpzzpppp"                                 # count ids per_row groups offsets order rows place
+    for a in ("bf16", "f16"):
+        for c in ("f32", a):
+            sigs[f"skl_gemm_grouped_{a}_{a}rc_{c}"] = "zpzzzfpzpzpzzzfpz"   # groups offsets m n k alpha a rsa rows a_rows b rsb csb gsb beta c rsc
+            sigs[f"skl_gemm_groupedk_{a}c_{a}_{c}"] = "zpzzzfpzpzpzpzfpzz"  # groups offsets m n total alpha a rsa rows_a a_rows b rsb rows_b b_rows beta c rsc gsc
+            sigs[f"skl_gemm_grouped_{a}_u4c_{c}"] = "zpzzzfpzpzUfpz"        # groups offsets m n k alpha a rsa rows a_rows weights beta c rsc
     for name, sig in GEMM_FUSED.items():
         sigs[name] = sig + "E"
     for w, pad in _PAD.items():
