@@ -1,5 +1,12 @@
 // skl_group_rows.hip - the order of picks by their groups (include/skl-gfx950.h: skl_group_rows).
+//
+// A counting sort that keeps the order of equals. Every wave owns a run of picks and has a row of counters in LDS; a pick's place is where its group begins, the
+// picks of that group in earlier workgroups and waves, those of earlier steps of its own wave - all in the counters - and those in lower lanes of its step, which are the
+// lanes that agree with it in every bit of the group's number: a ballot for each bit. No order comes from an atomic: those only count.
+// Up to 8192 picks one workgroup does it in a launch; more are counted by a first launch, whose counts each workgroup of the second adds up for itself.
 #include <hip/hip_runtime.h>
+
+#include <atomic>
 
 #include "skl_groups.hpp"
 #include "../../include/skl-hip.h"
@@ -8,58 +15,111 @@ namespace {
 
 struct GroupRowsArgs {
   const int32_t *ids;
-  unsigned count, per_row, groups;
+  unsigned count, per_row, groups, bits;
+  unsigned each;      // picks of a wave
+  unsigned *counts;   // [groups][workgroups], from the launch before; NULL: there is one workgroup
   int32_t *offsets, *order, *rows, *place;
 };
 
-// One workgroup: counts, their sums, then the picks in turn, 1024 at a time, each behind those of its group before it.
-__global__ void __launch_bounds__(1024) group_rows_kernel(GroupRowsArgs p) {
-  __shared__ unsigned next[SKL_MAX_GROUPS];  // where the next pick of a group goes
-  __shared__ unsigned carried, total[16];
-  __shared__ int batch[1024];
-  const unsigned t = threadIdx.x, lane = t & 63u, wave = t >> 6;
-  for (unsigned g = t; g < p.groups; g += 1024) next[g] = 0;
-  if (t == 0) carried = 0;
+// The picks of this wave.
+__device__ __forceinline__ void run_of(const GroupRowsArgs &p, unsigned wave, unsigned waves, unsigned &first, unsigned &end) {
+  first = (blockIdx.x * waves + wave) * p.each;
+  end = first < p.count ? (p.count - first < p.each ? p.count : first + p.each) : first;
+}
+
+__global__ void __launch_bounds__(1024) group_count_kernel(GroupRowsArgs p) {
+  extern __shared__ unsigned count_lds[];
+  const unsigned waves = blockDim.x / 64, lane = threadIdx.x & 63u;
+  for (unsigned g = threadIdx.x; g < p.groups; g += blockDim.x) count_lds[g] = 0;
   __syncthreads();
-  for (unsigned i = t; i < p.count; i += 1024) {
+  unsigned first, end;
+  run_of(p, threadIdx.x >> 6, waves, first, end);
+  for (unsigned i = first + lane; i < end; i += 64) {
     const unsigned g = (unsigned)p.ids[i];
-    if (g < p.groups) atomicAdd(&next[g], 1u);
+    if (g < p.groups) atomicAdd(&count_lds[g], 1u);
   }
   __syncthreads();
-  for (unsigned g0 = 0; g0 < p.groups; g0 += 1024) {
-    const unsigned g = g0 + t, mine = g < p.groups ? next[g] : 0u, upto = skl_wave_scan(mine);
-    if (lane == 63) total[wave] = upto;
-    __syncthreads();
-    unsigned before = carried;
-    for (unsigned w = 0; w < wave; ++w) before += total[w];
-    if (g < p.groups) {
-      next[g] = before + upto - mine;
-      p.offsets[g] = (int)(before + upto - mine);
+  for (unsigned g = threadIdx.x; g < p.groups; g += blockDim.x) p.counts[(size_t)g * gridDim.x + blockIdx.x] = count_lds[g];
+}
+
+__device__ __forceinline__ unsigned wave_sum(unsigned v) { return (unsigned)__builtin_amdgcn_readlane((int)skl_wave_scan(v), 63); }
+
+__global__ void __launch_bounds__(1024) group_rows_kernel(GroupRowsArgs p) {
+  extern __shared__ unsigned rows_lds[];  // [waves][groups] next places; [groups] where a group begins; [groups] its picks in earlier workgroups
+  __shared__ unsigned sums[16];
+  const unsigned threads = blockDim.x, waves = threads / 64, lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, groups = p.groups;
+  unsigned *const next = rows_lds, *const begin = next + waves * groups, *const before = begin + groups;
+  for (unsigned g = threadIdx.x; g < waves * groups; g += threads) next[g] = 0;
+  unsigned first, end;
+  run_of(p, wave, waves, first, end);
+  unsigned held = first + lane < end ? (unsigned)p.ids[first + lane] : ~0u;  // the first step's, looked at again below
+  __syncthreads();
+  if (p.counts) {  // a wave per group: 64 workgroups' counts at a time
+    for (unsigned g = wave; g < groups; g += waves) {
+      unsigned all = 0, lower = 0;
+      for (unsigned b = lane; b < gridDim.x; b += 64) {
+        const unsigned c = p.counts[(size_t)g * gridDim.x + b];
+        all += c;
+        lower += b < blockIdx.x ? c : 0u;
+      }
+      all = wave_sum(all), lower = wave_sum(lower);
+      if (lane == 0) begin[g] = all, before[g] = lower;
     }
-    __syncthreads();
-    if (t == 1023) carried = before + upto;
-    __syncthreads();
   }
-  if (t == 0) p.offsets[p.groups] = (int)carried;
-  for (unsigned i0 = 0; i0 < p.count; i0 += 1024) {
-    const unsigned i = i0 + t, g = i < p.count ? (unsigned)p.ids[i] : ~0u;
-    batch[t] = (int)g;
-    __syncthreads();
-    unsigned before = 0, after = 0;
-    for (unsigned j = 0; j < 1024; ++j) {
-      before += j < t && batch[j] == (int)g;
-      after += j > t && batch[j] == (int)g;
+  unsigned *const mine = next + wave * groups;
+  for (unsigned i = first + lane; i < end; i += 64) {
+    const unsigned g = i < first + 64 ? held : (unsigned)p.ids[i];
+    if (g < groups) atomicAdd(&mine[g], 1u);
+  }
+  __syncthreads();
+  // Thread t: groups t * per .. + per - 1.
+  const unsigned per = (groups + threads - 1) / threads, g0 = threadIdx.x * per, g1 = g0 + per < groups ? g0 + per : groups;
+  unsigned sum = 0;
+  for (unsigned g = g0; g < g1; ++g) {
+    if (!p.counts) {
+      unsigned all = 0;
+      for (unsigned w = 0; w < waves; ++w) all += next[w * groups + g];
+      begin[g] = all, before[g] = 0;
     }
-    const bool in = g < p.groups;
-    const unsigned at = in ? next[g] + before : 0u;
-    __syncthreads();
-    if (in && after == 0) next[g] = at + 1;
+    sum += begin[g];
+  }
+  const unsigned upto = skl_wave_scan(sum);
+  if (lane == 63) sums[wave] = upto;
+  __syncthreads();
+  unsigned at = upto - sum;
+  for (unsigned w = 0; w < wave; ++w) at += sums[w];
+  for (unsigned g = g0; g < g1; ++g) {
+    const unsigned all = begin[g];
+    if (blockIdx.x == 0) p.offsets[g] = (int)at;
+    unsigned to = at + before[g];
+    for (unsigned w = 0; w < waves; ++w) {
+      const unsigned c = next[w * groups + g];
+      next[w * groups + g] = to;
+      to += c;
+    }
+    at += all;
+  }
+  if (blockIdx.x == 0 && g1 == groups && g0 < groups) p.offsets[groups] = (int)at;
+  __syncthreads();
+  for (unsigned i0 = first; i0 < end; i0 += 64) {
+    const unsigned i = i0 + lane, g = i0 == first ? held : i < end ? (unsigned)p.ids[i] : ~0u;
+    const bool in = g < groups;
+    unsigned long long same = __ballot(in);
+    for (unsigned b = 0; b < p.bits; ++b) {
+      const bool set = (g >> b) & 1u;
+      const unsigned long long of_bit = __ballot(set);
+      same &= set ? of_bit : ~of_bit;
+    }
+    const unsigned lower = __builtin_amdgcn_mbcnt_hi((unsigned)(same >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)same, 0u));
+    unsigned to = 0;
     if (in) {
-      if (p.order) p.order[at] = (int)i;
-      if (p.rows) p.rows[at] = (int)(i / p.per_row);
+      volatile unsigned *const here = &mine[g];  // other lanes write it
+      to = *here + lower;
+      if (p.order) p.order[to] = (int)i;
+      if (p.rows) p.rows[to] = (int)(i / p.per_row);
+      if (lower + 1 == (unsigned)__popcll(same)) *here = to + 1;  // the last of them; a wave's accesses are in order
     }
-    if (p.place && i < p.count) p.place[i] = in ? (int)at : -1;
-    __syncthreads();
+    if (p.place && i < end) p.place[i] = in ? (int)to : -1;
   }
 }
 
@@ -69,8 +129,36 @@ int skl_hip_launch_group_rows(size_t count, const int32_t *ids, size_t per_row, 
                               int32_t *place) {
   GroupRowsArgs p{};
   p.ids = ids, p.count = (unsigned)count, p.groups = (unsigned)groups;
-  p.per_row = per_row > 0xFFFFFFFFu ? 0xFFFFFFFFu : (unsigned)per_row;  // (more than there are picks: one row)
+  p.per_row = per_row > 0xFFFFFFFFu ? 0xFFFFFFFFu : per_row ? (unsigned)per_row : 1u;  // (more than there are picks: one row)
   p.offsets = offsets, p.order = order, p.rows = rows, p.place = place;
-  group_rows_kernel<<<dim3(1), dim3(1024), 0, skl_current_stream()>>>(p);
-  return skl_check_launch("group_rows");
+  while ((size_t(1) << p.bits) < groups) ++p.bits;
+  const unsigned waves = groups <= 2048 ? 16 : 4;  // their counters fit LDS
+  const unsigned lds = (waves + 2) * p.groups * 4;
+  // Workgroups: 2048 picks each and no more than the compute units; what each adds up, groups x workgroups, at most 1 MiB.
+  size_t blocks = count <= 8192 ? 1 : (count + 2047) / 2048;
+  if (blocks > 256) blocks = 256;
+  if (blocks > 262144 / groups) blocks = 262144 / groups;
+  const bool sequence = blocks > 1;
+  if (sequence) {
+    skl_hip_sequence_begin();
+    p.counts = (unsigned *)skl_workspace(blocks * groups * 4, true);
+    if (!p.counts) blocks = 1;  // no scratch memory: the same result from one workgroup
+  }
+  p.each = (skl_div_up(count, blocks * waves) + 63) / 64 * 64;
+  int rc = 0;
+  if (p.counts) {
+    group_count_kernel<<<dim3((unsigned)blocks), dim3(waves * 64), groups * 4, skl_current_stream()>>>(p);
+    rc = skl_check_launch("group_rows: counts");
+  }
+  static std::atomic<int> allowed{0};
+  if (rc == 0 && !allowed.load(std::memory_order_relaxed)) {
+    rc = skl_check_hip(hipFuncSetAttribute(reinterpret_cast<const void *>(&group_rows_kernel), hipFuncAttributeMaxDynamicSharedMemorySize, 18 * 2048 * 4), "group_rows: LDS size");
+    if (rc == 0) allowed.store(1, std::memory_order_relaxed);
+  }
+  if (rc == 0) {
+    group_rows_kernel<<<dim3((unsigned)blocks), dim3(waves * 64), lds, skl_current_stream()>>>(p);
+    rc = skl_check_launch("group_rows");
+  }
+  if (sequence) skl_hip_sequence_end();
+  return rc;
 }
