@@ -94,54 +94,60 @@ __global__ void __launch_bounds__(256) gemm_u4_any_kernel(U4Args p) {
 }
 
 // ---------------------------------------------------------------------------
-// The stream over the codes: rows of codes and of A on 16-byte boundaries, k a multiple of 32, group_k 32, 64, 128 or a multiple of 256 (one group of all k
+// The stream over the codes: rows of codes and of A on 16-byte boundaries, k a multiple of 32, group_k 32, 64 or a multiple of 128 (one group of all k
 // among them).
-// A workgroup takes 16 F columns and all of k, its waves units of 256 k - a line of each column's codes - in turn, and up to 16 R rows per pass; the
-// waves' sums meet in LDS. What bounds it is the codes' way from memory: two units are under way per wave.
+// A workgroup of eight waves takes 16 F columns and all of k, in chunks: a wave UNITS units of 128 k of each, half a line of each column's codes, which go
+// to registers a chunk ahead. ROWS rows of A and the columns' scales go to LDS, where all waves read them; in the end the waves' sums meet there.
 // ---------------------------------------------------------------------------
 
-// Eight values q - z, natural order of k; `z` as prepared by zero_of().
+// Eight values q - z of a column, exact.
 template <typename T>
 struct Zero;
 template <>
 struct Zero<__bf16> {
-  float z;
-  __device__ __forceinline__ explicit Zero(unsigned v) : z((float)v) {}
+  float z;  // -(1024 + zero point)
+  __device__ __forceinline__ explicit Zero(unsigned v) : z(-1024.0f - (float)v) {}
 };
 template <>
 struct Zero<_Float16> {
   v2h z;
   __device__ __forceinline__ explicit Zero(unsigned v) : z(__builtin_bit_cast(v2h, (0x6400u + v) * 0x10001u)) {}  // 1024 + v, twice (v < 1024)
 };
+// The nibbles as they lie are pairs k0 k4, k1 k5, k2 k6, k3 k7; A is put into that order on its way to LDS (arranged()). 0x6400 | q is the f16 number 1024 + q.
+// (An instruction takes one scalar besides, and no literal.)
+__device__ __forceinline__ unsigned pair_of(unsigned codes, int i) {
+  unsigned two;
+  asm("v_and_or_b32 %0, %1, %2, %3" : "=v"(two) : "v"(codes >> (4 * i)), "s"(0x000F000Fu), "v"(0x64006400u));
+  return two;
+}
 __device__ __forceinline__ v4i widened(unsigned codes, Zero<__bf16> z) {
-  const unsigned even = codes & 0x0F0F0F0Fu, odd = (codes >> 4) & 0x0F0F0F0Fu;
-  v8bf w;
+  v4i w;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    w[2 * i] = (__bf16)((float)((even >> (8 * i)) & 255u) - z.z);
-    w[2 * i + 1] = (__bf16)((float)((odd >> (8 * i)) & 255u) - z.z);
+    // The f16 halves as factors of fp32 multiply-adds: 1024 + q - (1024 + z). (By v_cvt_f32_ubyte and a subtraction 23 instructions for eight values, so 19.)
+    const unsigned two = pair_of(codes, i);
+    float low, high;
+    asm("v_fma_mix_f32 %0, %1, 1.0, %2 op_sel_hi:[1,0,0]" : "=v"(low) : "v"(two), "v"(z.z));
+    asm("v_fma_mix_f32 %0, %1, 1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(high) : "v"(two), "v"(z.z));
+    typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
+    w[i] = __builtin_bit_cast(int, v2bf{(__bf16)low, (__bf16)high});
   }
-  return __builtin_bit_cast(v4i, w);
+  return w;
 }
-// f16: k0 k4, k1 k5, k2 k6, k3 k7 as the nibbles lie; the fragment of A is put into that order (arranged()). 1024 + q has q for its last bits.
 __device__ __forceinline__ v4i widened(unsigned codes, Zero<_Float16> z) {
   v4i w;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) w[i] = __builtin_bit_cast(int, __builtin_bit_cast(v2h, ((codes >> (4 * i)) & 0x000F000Fu) | 0x64006400u) - z.z);
+  for (int i = 0; i < 4; ++i) w[i] = __builtin_bit_cast(int, __builtin_bit_cast(v2h, pair_of(codes, i)) - z.z);
   return w;
 }
-template <typename T>
+// k0 .. k7 as k0 k4 k1 k5 k2 k6 k3 k7.
 __device__ __forceinline__ v4i arranged(v4i a) {
-  if constexpr (is_bf16<T>) {
-    return a;
-  } else {
-    v4i r;
-    r[0] = (int)__builtin_amdgcn_perm((unsigned)a[2], (unsigned)a[0], 0x05040100u);
-    r[1] = (int)__builtin_amdgcn_perm((unsigned)a[2], (unsigned)a[0], 0x07060302u);
-    r[2] = (int)__builtin_amdgcn_perm((unsigned)a[3], (unsigned)a[1], 0x05040100u);
-    r[3] = (int)__builtin_amdgcn_perm((unsigned)a[3], (unsigned)a[1], 0x07060302u);
-    return r;
-  }
+  v4i r;
+  r[0] = (int)__builtin_amdgcn_perm((unsigned)a[2], (unsigned)a[0], 0x05040100u);
+  r[1] = (int)__builtin_amdgcn_perm((unsigned)a[2], (unsigned)a[0], 0x07060302u);
+  r[2] = (int)__builtin_amdgcn_perm((unsigned)a[3], (unsigned)a[1], 0x05040100u);
+  r[3] = (int)__builtin_amdgcn_perm((unsigned)a[3], (unsigned)a[1], 0x07060302u);
+  return r;
 }
 
 // Dword i of the four quarters of a wave, transposed: quarter p's dword j becomes quarter j's dword p.
@@ -152,139 +158,170 @@ __device__ __forceinline__ v4i quarters_transposed(v4i v) {
   return v4i{(int)c[0], (int)c[1], (int)d[0], (int)d[1]};
 }
 
-constexpr unsigned kUnit = 256;  // of k
+constexpr unsigned kUnit = 128, kWaves = 8, kThreads = kWaves * 64;  // of k
 
-// Of a column's unit: its codes as two pieces per lane - piece j of quarter p holds k 128 j + 32 p .. + 31 -, its scales and zero points.
-// PER: groups of a unit, 8, 4, 2 or 1.
-template <int PER, bool ZEROS>
-struct UnitOf {
-  v4i piece[2];
-  uint16_t scale[PER];
-  uint8_t zero[ZEROS ? PER : 1];
-  // `tail`: the row's last, partial unit, `left` k of it (a multiple of 32): pieces beyond are zeros, groups beyond the row's last one again.
-  __device__ __forceinline__ void load(const uint8_t *codes, const uint16_t *scales, const uint8_t *zeros, unsigned part, unsigned unit, bool tail, unsigned left, unsigned first_group, unsigned last_group) {
-    const uint8_t *const at = codes + (size_t)unit * (kUnit / 2) + 16 * part;
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const bool there = !tail || 128u * j + 32u * part < left;
-      piece[j] = there ? __builtin_nontemporal_load(reinterpret_cast<const v4i *>(at + 64 * j)) : v4i{0, 0, 0, 0};
-    }
-#pragma unroll
-    for (int g = 0; g < PER; ++g) {
-      const unsigned group = first_group + g < last_group ? first_group + g : last_group;
-      scale[g] = scales[group];
-      if constexpr (ZEROS) zero[g] = zeros[group];
-    }
-  }
+// What a kernel holds. PER: groups of a unit, 4, 2 or 1; F: 16 columns each; ROWS: of A, staged in LDS for a chunk of UNITS units per wave.
+template <int PER, bool ZEROS, int F, int ROWS, int UNITS>
+struct U4Shape {
+  static constexpr unsigned kR = (ROWS + 15) / 16, kCols = 16 * F, kChunk = kUnit * kWaves * UNITS;
+  static constexpr unsigned kPitch = kChunk * 2 + 16;  // bytes of a row of A: 16 rows meet in no bank
+  static constexpr unsigned kPieces = (ROWS * kChunk / 8 + kThreads - 1) / kThreads, kRowPieces = kChunk / 8;
+  static constexpr unsigned kEntries = kChunk / kUnit * PER, kEach = (kCols * kEntries + kThreads - 1) / kThreads;  // scales of a column and chunk, of a thread
+  static constexpr unsigned kBytesA = ROWS * kPitch, kStage = (kBytesA + (kEntries + 1) * kCols * 4 + 15) / 16 * 16;
+  static constexpr unsigned kSums = kWaves * 16 * kR * (kCols + 1) * 4, kLds = 2 * kStage > kSums ? 2 * kStage : kSums;
+  struct Side {  // what goes to LDS, on its way
+    v4i a[kPieces];
+    unsigned scale[kEach], zero[ZEROS ? kEach : 1];
+  };
 };
 
-template <typename T, int PER, bool ZEROS, int F, int R, int WAVES>
-__global__ void __launch_bounds__(WAVES * 64) gemm_u4_stream_kernel(U4Args p, int c_single) {
-  constexpr bool kFine = PER > 2;  // groups smaller than the 128 k whose codes the quarters of a wave hold side by side
-  __shared__ float sums_lds[WAVES][16 * R][16 * F + 1];
+template <typename T, int PER, bool ZEROS, int F, int ROWS, int UNITS, int MIN>
+__global__ void __launch_bounds__(kThreads, MIN) gemm_u4_stream_kernel(U4Args p, int c_single) {
+  using Shape = U4Shape<PER, ZEROS, F, ROWS, UNITS>;
+  constexpr bool kFine = PER > 1;       // groups smaller than the 128 k whose codes the quarters of a wave hold side by side
+  constexpr unsigned kCols = Shape::kCols, kChunk = Shape::kChunk, kEntries = Shape::kEntries, kEach = Shape::kEach, kPitch = Shape::kPitch, kPieces = Shape::kPieces, kRowPieces = Shape::kRowPieces;
+  constexpr int R = Shape::kR;
+  extern __shared__ __attribute__((aligned(16))) char u4_lds_bytes[];
   const unsigned wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u, l = lane & 15u, part = lane >> 4, e = blockIdx.y;
   const SklRange range = skl_group_range(p.offsets, e, p.m);
   if (range.rows == 0) return;
-  const unsigned col0 = blockIdx.x * (16 * F);
-  const unsigned units = (p.k + kUnit - 1) / kUnit, last_group = p.k ? (p.k - 1) / p.group_k : 0;
-  const unsigned units_per_group = PER == 1 ? p.group_k / kUnit : 1;
-  const uint8_t *codes[F], *zeros[F];
-  const uint16_t *scales[F];
+  const unsigned col0 = blockIdx.x * kCols, cols = p.n - col0 < kCols ? p.n - col0 : kCols;
+  const unsigned last_group = p.k ? (p.k - 1) / p.group_k : 0, units_per_group = PER == 1 ? p.group_k / kUnit : 1;
+  const uint8_t *const codes = p.codes + ((size_t)e * p.expert + (size_t)col0 * p.ld) / 2;
+  unsigned code_at[F];
 #pragma unroll
-  for (int f = 0; f < F; ++f) {
-    const unsigned col = col0 + 16 * f + l < p.n ? col0 + 16 * f + l : p.n - 1;
-    codes[f] = p.codes + ((size_t)e * p.expert + (size_t)col * p.ld) / 2;
-    scales[f] = p.scales + (size_t)e * p.expert_scales + (size_t)col * p.ld_scales;
-    zeros[f] = ZEROS ? p.zeros + (size_t)e * p.expert_scales + (size_t)col * p.ld_scales : nullptr;
-  }
+  for (int f = 0; f < F; ++f) code_at[f] = (16 * f + l < cols ? 16 * f + l : cols - 1) * (unsigned)(p.ld / 2);  // (ld below 2^25, see the launch)
+  const size_t scale_base = (size_t)e * p.expert_scales + (size_t)col0 * p.ld_scales;
   const bool read_c = !skl_beta_is_zero<float>(p.beta);
   const unsigned limit = p.rows ? p.a_rows : p.m;  // an A without rows: nothing to multiply
-  for (unsigned row0 = 0; row0 < range.rows; row0 += 16 * R) {
+  const unsigned chunks = limit == 0 ? 0 : (p.k + kChunk - 1) / kChunk;
+
+  struct Codes {
+    v4i v[F];
+  };
+  for (unsigned row0 = 0; row0 < range.rows; row0 += ROWS) {
     // Rows that do not exist are the group's first again, those that an index puts outside A its first: computed, and written nowhere or as zeros.
-    const uint16_t *a[R];
+    const uint16_t *a[kPieces];
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      unsigned row = range.first + (row0 + 16 * r + l < range.rows ? row0 + 16 * r + l : 0u);
+    for (int i = 0; i < (int)kPieces; ++i) {
+      const unsigned r = row0 + (threadIdx.x + i * kThreads) / kRowPieces;
+      unsigned row = range.first + (r < range.rows ? r : 0u);
       if (p.rows) row = (unsigned)p.rows[row];
-      a[r] = p.a + (size_t)(row < limit ? row : 0u) * p.rsa;
+      a[i] = p.a + (size_t)(row < limit ? row : 0u) * p.rsa;
     }
+    // (Without branches, at whose ends what is under way would be waited for: behind k lies what lies at its end again, with zeros for A. And the offsets anew for
+    // every chunk, from a number that the compiler cannot follow: it otherwise keeps all of them.)
+    const auto request_codes = [&](Codes &to, unsigned c, unsigned j) __attribute__((always_inline)) {
+      asm volatile("" : "+s"(c));
+      const unsigned piece = ((c * UNITS + j) * kWaves + wave) * (kUnit / 2) + 16 * part, most = p.k / 2 - 16;
+#pragma unroll
+      for (int f = 0; f < F; ++f) to.v[f] = __builtin_nontemporal_load(reinterpret_cast<const v4i *>(codes + (code_at[f] + (piece < most ? piece : most))));
+    };
+    const auto request_side = [&](typename Shape::Side &to, unsigned c) __attribute__((always_inline)) {
+      asm volatile("" : "+s"(c));
+#pragma unroll
+      for (int i = 0; i < (int)kPieces; ++i) {
+        const unsigned k = c * kChunk + (threadIdx.x + i * kThreads) % kRowPieces * 8;
+        to.a[i] = *reinterpret_cast<const v4i *>(a[i] + (k < p.k ? k : p.k - 8));
+      }
+#pragma unroll
+      for (int i = 0; i < (int)kEach; ++i) {
+        const unsigned at = threadIdx.x + i * kThreads, col = at / kEntries % kCols, entry = at % kEntries + c * kEntries;
+        unsigned group = PER == 1 ? entry / units_per_group : entry;
+        group = (col < cols ? col : cols - 1) * (unsigned)p.ld_scales + (group < last_group ? group : last_group);
+        to.scale[i] = (p.scales + scale_base)[group];
+        if constexpr (ZEROS) to.zero[i] = (p.zeros + scale_base)[group];
+      }
+    };
+    const auto stage = [&](const typename Shape::Side &from, unsigned c) __attribute__((always_inline)) {
+      char *const to = u4_lds_bytes + (c & 1) * Shape::kStage;
+#pragma unroll
+      for (int i = 0; i < (int)kPieces; ++i) {
+        const unsigned at = threadIdx.x + i * kThreads;
+        if (ROWS * kRowPieces % kThreads == 0 || at < ROWS * kRowPieces) *reinterpret_cast<v4i *>(to + at / kRowPieces * kPitch + at % kRowPieces * 16) = c * kChunk + at % kRowPieces * 8 < p.k ? arranged(from.a[i]) : v4i{0, 0, 0, 0};
+      }
+#pragma unroll
+      for (int i = 0; i < (int)kEach; ++i) {  // [column][entry]: a scale with its zero point above
+        const unsigned at = threadIdx.x + i * kThreads;
+        if (kCols * kEntries % kThreads == 0 || at < kCols * kEntries) reinterpret_cast<unsigned *>(to + Shape::kBytesA)[at / kEntries * (kEntries + 1) + at % kEntries] = from.scale[i] | (ZEROS ? from.zero[ZEROS ? i : 0] : 8u) << 16;
+      }
+    };
     v4f sum[R][F];
 #pragma unroll
     for (int r = 0; r < R; ++r)
 #pragma unroll
       for (int f = 0; f < F; ++f) sum[r][f] = v4f{0, 0, 0, 0};
-    UnitOf<PER, ZEROS> unit[2][F];
-    const auto load = [&](int slot, unsigned u) __attribute__((always_inline)) {
-      const bool tail = (u + 1) * kUnit > p.k;
+    const auto multiply = [&](const Codes &b, unsigned c, unsigned j) __attribute__((always_inline)) {
+      const char *const tile = u4_lds_bytes + (c & 1) * Shape::kStage;
+      const unsigned unit = j * kWaves + wave;
+      const unsigned *const entry = reinterpret_cast<const unsigned *>(tile + Shape::kBytesA) + l * (kEntries + 1) + unit * PER;
+      constexpr int kOf = 4 / PER;  // instructions of a group in a unit
+      v4i code[F];
+      v4f acc[R][F];
 #pragma unroll
-      for (int f = 0; f < F; ++f) unit[slot][f].load(codes[f], scales[f], zeros[f], part, u, tail, p.k - u * kUnit, PER == 1 ? u / units_per_group : u * PER, last_group);
-    };
-    const auto multiply = [&](int slot, unsigned u) __attribute__((always_inline)) {
-      const bool tail = (u + 1) * kUnit > p.k;
+      for (int f = 0; f < F; ++f) code[f] = kFine ? quarters_transposed(b.v[f]) : b.v[f];
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        v4i piece[F];
+      for (int i = 0; i < 4; ++i) {
+        v4i x[R];
 #pragma unroll
-        for (int f = 0; f < F; ++f) piece[f] = kFine ? quarters_transposed(unit[slot][f].piece[j]) : unit[slot][f].piece[j];
-        v4f acc[R][F];
+        for (int r = 0; r < R; ++r) x[r] = *reinterpret_cast<const v4i *>(tile + ((16 * r + l) % ROWS) * kPitch + (unit * kUnit + (kFine ? 32u * i + 8 * part : 32 * part + 8u * i)) * 2);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          constexpr int kOf = PER >= 2 ? 8 / PER : 8;  // instructions of a group in a unit
-          const int at = 4 * j + i, group = at / kOf;
-          const bool begins = at % kOf == 0 || i == 0, ends = (at + 1) % kOf == 0 || i == 3;
-          const unsigned k = u * kUnit + 128 * j + (kFine ? 32 * i + 8 * part : 32 * part + 8 * i);
-          v4i x[R];
+        for (int f = 0; f < F; ++f) {
+          const v4i w = widened((unsigned)code[f][i], Zero<T>(entry[16 * f * (kEntries + 1) + i / kOf] >> 16));
 #pragma unroll
-          for (int r = 0; r < R; ++r) {
-            x[r] = !tail || k < p.k ? *reinterpret_cast<const v4i *>(a[r] + k) : v4i{0, 0, 0, 0};
-            x[r] = arranged<T>(x[r]);
-          }
+          for (int r = 0; r < R; ++r) acc[r][f] = product<T>(x[r], w, i % kOf == 0 ? v4f{0, 0, 0, 0} : acc[r][f]);
+        }
+        if ((i + 1) % kOf == 0) {
 #pragma unroll
           for (int f = 0; f < F; ++f) {
-            const v4i w = widened((unsigned)piece[f][i], Zero<T>(ZEROS ? unit[slot][f].zero[ZEROS ? group : 0] : 8u));
+            const float by = skl_widen((uint16_t)entry[16 * f * (kEntries + 1) + i / kOf], is_bf16<T>);
 #pragma unroll
-            for (int r = 0; r < R; ++r) acc[r][f] = product<T>(x[r], w, begins ? v4f{0, 0, 0, 0} : acc[r][f]);
-          }
-          if (ends) {
+            for (int r = 0; r < R; ++r)
 #pragma unroll
-            for (int f = 0; f < F; ++f) {
-              const float scale = skl_widen(unit[slot][f].scale[group], is_bf16<T>);
-#pragma unroll
-              for (int r = 0; r < R; ++r)
-#pragma unroll
-                for (int q = 0; q < 4; ++q) sum[r][f][q] = __builtin_fmaf(acc[r][f][q], scale, sum[r][f][q]);
-            }
+              for (int q = 0; q < 4; ++q) sum[r][f][q] = __builtin_fmaf(acc[r][f][q], by, sum[r][f][q]);
           }
         }
       }
     };
-    if (limit != 0) {
-      if (wave < units) load(0, wave);
-      for (unsigned u = wave; u < units; u += 2 * WAVES) {
-        if (u + WAVES < units) load(1, u + WAVES);
-        multiply(0, u);
-        if (u + WAVES >= units) break;
-        if (u + 2 * WAVES < units) load(0, u + 2 * WAVES);
-        multiply(1, u + WAVES);
+    if (row0) __syncthreads();  // the sums of the pass before have been read
+    if (chunks != 0) {
+      Codes held[UNITS];
+      typename Shape::Side side;
+      request_side(side, 0);
+#pragma unroll
+      for (int j = 0; j < UNITS; ++j) request_codes(held[j], 0, j);
+      stage(side, 0);
+      for (unsigned c = 0; c < chunks; ++c) {
+        __syncthreads();  // chunk c is staged; nobody reads chunk c - 1 any more
+        request_side(side, c + 1);
+#pragma unroll
+        for (int j = 0; j < UNITS; ++j) {
+          __builtin_amdgcn_sched_barrier(0);
+          if (c * kChunk + (j * kWaves + wave) * kUnit < p.k) multiply(held[j], c, j);
+          __builtin_amdgcn_sched_barrier(0);
+          request_codes(held[j], c + 1, j);
+        }
+        stage(side, c + 1);
       }
     }
-    if (row0) __syncthreads();  // the sums of the pass before have been read
+    __syncthreads();
+    float(*const sums)[16 * R][kCols + 1] = reinterpret_cast<float(*)[16 * R][kCols + 1]>(u4_lds_bytes);
 #pragma unroll
     for (int r = 0; r < R; ++r)
 #pragma unroll
       for (int f = 0; f < F; ++f)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) sums_lds[wave][16 * r + 4 * part + q][16 * f + l] = sum[r][f][q];
+        for (int q = 0; q < 4; ++q) sums[wave][16 * r + 4 * part + q][16 * f + l] = sum[r][f][q];
     __syncthreads();
-    for (unsigned i = threadIdx.x; i < 256 * R * F; i += WAVES * 64) {
-      const unsigned row = i / (16 * F), c = i % (16 * F), col = col0 + c;
-      if (row0 + row >= range.rows || col >= p.n) continue;
+    for (unsigned i = threadIdx.x; i < ROWS * kCols; i += kThreads) {
+      const unsigned row = i / kCols, c = i % kCols;
+      if (row0 + row >= range.rows || c >= cols) continue;
       float v = 0.0f;
 #pragma unroll
-      for (int w = 0; w < WAVES; ++w) v = __fadd_rn(v, sums_lds[w][row][c]);
+      for (unsigned w = 0; w < kWaves; ++w) v = __fadd_rn(v, sums[w][row][c]);
       const unsigned out = range.first + row0 + row;
       if (p.rows && (unsigned)p.rows[out] >= limit) v = 0.0f;
-      const size_t at = (size_t)out * p.rsc + col;
+      const size_t at = (size_t)out * p.rsc + col0 + c;
       if (c_single) {
         float *const to = reinterpret_cast<float *>(p.c) + at;
         *to = skl_grouped_result(v, to, p.alpha, p.beta, read_c);
@@ -296,34 +333,43 @@ __global__ void __launch_bounds__(WAVES * 64) gemm_u4_stream_kernel(U4Args p, in
   }
 }
 
-template <typename T, int PER, int F, int R, int WAVES>
+template <typename T, int PER, bool ZEROS, int F, int ROWS, int UNITS, int MIN>
 int launch_stream(const U4Args &p, int c_single) {
-  const dim3 grid(skl_div_up(p.n, 16 * F), p.groups), block(WAVES * 64);
-  if (p.zeros) gemm_u4_stream_kernel<T, PER, true, F, R, WAVES><<<grid, block, 0, skl_current_stream()>>>(p, c_single);
-  else gemm_u4_stream_kernel<T, PER, false, F, R, WAVES><<<grid, block, 0, skl_current_stream()>>>(p, c_single);
+  constexpr unsigned kLds = U4Shape<PER, ZEROS, F, ROWS, UNITS>::kLds;
+  const auto kernel = gemm_u4_stream_kernel<T, PER, ZEROS, F, ROWS, UNITS, MIN>;
+  static std::atomic<int> allowed{0};
+  if (!allowed.load(std::memory_order_relaxed)) {
+    const int rc = skl_check_hip(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kLds), "gemm_u4: LDS size");
+    if (rc != 0) return rc;
+    allowed.store(1, std::memory_order_relaxed);
+  }
+  kernel<<<dim3(skl_div_up(p.n, 16 * F), p.groups), dim3(kThreads), kLds, skl_current_stream()>>>(p, c_single);
   return skl_check_launch("gemm_u4");
 }
 
-template <typename T, int PER>
+template <typename T, int PER, bool ZEROS>
 int stream_by_size(const U4Args &p, int c_single) {
-  if (p.m > 16 * p.groups) return launch_stream<T, PER, 2, 2, 8>(p, c_single);
-  const size_t cols = (size_t)p.n * (p.groups < p.m ? p.groups : p.m);
-  if (cols >= 16384) return launch_stream<T, PER, 4, 1, 8>(p, c_single);
-  return launch_stream<T, PER, 1, 1, 4>(p, c_single);
+  // By the rows there are for a matrix, on average where there are several: rows beyond a pass read the codes again. us, 1 / 4 / 16 rows a pass: 1 x 4096 x 11008 9.8 / 10.5 / -,
+  // 8 tokens to 4 of 32 experts 44 / 26 / 31, 64 tokens 45 with 16 and 61 with 4. Fewer columns and shorter chunks a workgroup, more workgroups: F = 2 rather than 1 costs 1 x 4096 x 11008
+  // 1.2 us, twice the chunk 0.1 to 1.7; with 16 rows, whose operands are read for all columns, F = 2 is the faster one (16 x 8192 x 8192 14.9, F = 1 17.4).
+  if (p.m == 1) return launch_stream<T, PER, ZEROS, 1, 1, 2, 6>(p, c_single);
+  if (p.m <= 4 * (size_t)p.groups) return launch_stream<T, PER, ZEROS, 1, 4, 1, 6>(p, c_single);
+  if (p.m <= 16 * (size_t)p.groups) return launch_stream<T, PER, ZEROS, 2, 16, 1, 4>(p, c_single);
+  return launch_stream<T, PER, ZEROS, 2, 32, 1, 2>(p, c_single);
 }
 
 template <typename T>
 int launch(U4Args p, int c_single) {
   const auto aligned = [](const void *at) { return ((uintptr_t)at & 15) == 0; };
   const bool one = p.group_k >= p.k;
-  if (p.k % 32 == 0 && aligned(p.a) && aligned(p.codes) && p.rsa % 8 == 0 && p.ld % 32 == 0 && p.expert % 32 == 0 &&
-      (one || p.group_k == 32 || p.group_k == 64 || p.group_k == 128 || p.group_k % 256 == 0)) {
-    if (one || p.group_k % 256 == 0) {
+  if (p.k % 32 == 0 && aligned(p.a) && aligned(p.codes) && p.rsa % 8 == 0 && p.ld < (size_t(1) << 25) && p.ld_scales < (size_t(1) << 24) && p.ld % 32 == 0 && p.expert % 32 == 0 &&
+      (one || p.group_k == 32 || p.group_k == 64 || p.group_k % 128 == 0)) {
+    if (one || p.group_k % 128 == 0) {
       if (one) p.group_k = (p.k + kUnit - 1) / kUnit * kUnit;
-      return stream_by_size<T, 1>(p, c_single);
+      return p.zeros ? stream_by_size<T, 1, true>(p, c_single) : stream_by_size<T, 1, false>(p, c_single);
     }
-    if (p.group_k == 32) return stream_by_size<T, 8>(p, c_single);
-    return p.group_k == 64 ? stream_by_size<T, 4>(p, c_single) : stream_by_size<T, 2>(p, c_single);
+    if (p.group_k == 32) return p.zeros ? stream_by_size<T, 4, true>(p, c_single) : stream_by_size<T, 4, false>(p, c_single);
+    return p.zeros ? stream_by_size<T, 2, true>(p, c_single) : stream_by_size<T, 2, false>(p, c_single);
   }
   const dim3 grid(skl_div_up(p.n, 64), p.groups);
   if (c_single) gemm_u4_any_kernel<T, float><<<grid, dim3(256), 0, skl_current_stream()>>>(p);
