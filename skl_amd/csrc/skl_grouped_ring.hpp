@@ -1,0 +1,403 @@
+// skl_grouped_ring.hpp - the streaming kernel's way (skl_gemm_mfma_impl.hpp) with products grouped by expert: operands go from memory to LDS without registers, slices
+// of 64 bytes of K in a ring of four stages, the next slice's reads and a later one's requests dealt out behind the products of this one. What is different: which
+// rows a tile has is known on the GPU alone, an operand's rows may come through an index, C has two types.
+//
+// A tile is 256, 128 or 64 rows by BN columns. Whole tiles of 256 rows are dealt out first, then what is left of each group in the smallest tile that holds it: a group of
+// 300 rows costs 256 + 64, not 512.
+#pragma once
+
+#include "skl_gemm_mfma_impl.hpp"
+#include "skl_groups.hpp"
+
+namespace {
+
+struct GroupedRingArgs {
+  const char *a, *b;
+  const int32_t *offsets, *rows;
+  char *c;
+  size_t a_pitch, b_pitch, b_group;  // bytes: from one line of an operand to the next - rows or columns with K side by side, or steps of K -, from one group's B to the next
+  size_t rsc, gsc;                   // elements
+  unsigned groups, m, n, k, a_rows;  // OVER: k is the number of rows in all
+  unsigned tiles_m, tiles_n;         // OVER: of a group
+  int c_single;
+  skl_scalar alpha, beta;
+};
+
+// Requests of one operand, this wave's share: lines of ROWS rows or columns with K side by side (KC), a pair of slices at a time, or lines of ROWS values across K, a slice at a time. All
+// through a buffer descriptor; what does not exist has an offset beyond its range, for which zeros arrive and no memory is touched.
+template <bool KC, int ROWS, int WAVES>
+struct GroupedLoader {
+  using T = STile<2, KC, ROWS, 4, 16>;
+  static constexpr unsigned kRange = 0xC0000000u, kOutside = 0xE0000000u;
+  static constexpr int kBlocks = (KC ? 2 : 1) * T::kBytes / 1024 / WAVES;  // KiB per wave and unit
+  static_assert(kBlocks >= 1);
+  static constexpr unsigned kBlockStep = KC ? T::kGroup : 1024;
+  static constexpr unsigned kUnitK = KC ? 2 * kRingSlice : kRingSlice / 2;  // bytes or steps of K
+  const char *base;
+  size_t k_step;
+  unsigned off[kBlocks], k_lane[KC ? 2 : kBlocks], k_total, lds;
+
+  __device__ __forceinline__ static const char *scalar(const char *p) {
+    const uintptr_t at = (uintptr_t)p;
+    return (const char *)(((uintptr_t)(unsigned)__builtin_amdgcn_readfirstlane((int)(at >> 32)) << 32) | (unsigned)__builtin_amdgcn_readfirstlane((int)at));
+  }
+  // KC: lines first .. first + count - 1, through `index` where there is one (of `limit` lines); else columns at .. of `count` from there on, steps of K `pitch` apart.
+  // k: bytes (KC) or steps.
+  __device__ __forceinline__ void init(const char *from, size_t pitch, const int32_t *index, unsigned limit, unsigned first, unsigned count, unsigned k) {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    lds = wave * kBlocks * kBlockStep;
+    k_total = k;
+    if constexpr (KC) {
+      base = scalar(index ? from : from + (size_t)first * pitch);
+      k_step = 2 * kRingSlice;
+#pragma unroll
+      for (int i = 0; i < kBlocks; ++i) {
+        const int row = 8 * (wave * kBlocks + i) + ((lane & 31) >> 2), c = (lane & 3) ^ T::turn(row);
+        const unsigned in_k = (lane >> 5) * 64 + c * 16;
+        if (i < 2) k_lane[i] = in_k;  // (the blocks' turns alternate)
+        unsigned line = (unsigned)row < count ? (unsigned)row : ~0u;
+        if (index && line != ~0u) {
+          line = (unsigned)index[first + line];
+          if (line >= limit) line = ~0u;
+        }
+        off[i] = line == ~0u ? kOutside : line * (unsigned)pitch + in_k;
+      }
+    } else {
+      base = scalar(from + (size_t)first * 2);
+      k_step = ((size_t)(unsigned)__builtin_amdgcn_readfirstlane((int)((pitch * kUnitK) >> 32)) << 32) | (unsigned)__builtin_amdgcn_readfirstlane((int)(pitch * kUnitK));
+#pragma unroll
+      for (int i = 0; i < kBlocks; ++i) {
+        constexpr int kLanesPerRow = T::kRowBytes / 16, kRowsPerBlock = 1024 / T::kRowBytes;
+        const int kr = kRowsPerBlock * (wave * kBlocks + i) + lane / kLanesPerRow, mn = ((T::chunk(kr, lane % kLanesPerRow) - kr * T::kRowBytes) >> 4) * 8;
+        k_lane[i] = kr;
+        off[i] = (unsigned)mn < count ? (unsigned)kr * (unsigned)pitch + (unsigned)mn * 2 : kOutside;
+      }
+    }
+  }
+  __device__ __forceinline__ unsigned left_of(unsigned unit) const { return k_total > unit * kUnitK ? k_total - unit * kUnitK : 0; }
+  __device__ __forceinline__ void request(char *region, int stage, unsigned unit, unsigned left, int i) const {
+    unsigned o = k_lane[KC ? i & 1 : i] < left ? off[i] : kOutside;
+    asm volatile("" : "+v"(o));  // (not widened to 64 bits ahead of the loop, see SLoader)
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(__builtin_amdgcn_make_buffer_rsrc((void *)(base + unit * k_step), 0, (int)kRange, 0x00027000),
+                                             (__attribute__((address_space(3))) void *)(region + stage * T::kStageStep + lds + i * kBlockStep), 16, (int)o, 0, 0, 0);
+  }
+};
+
+// C of a wave: acc[i][j] holds, in lane l, four columns from 16 j + 4 (l / 16) on of row 16 i + l % 16. A row of blocks at a time goes through the wave's own 16 x (16 NI + 4) floats of LDS, from
+// where rows leave in runs of 16 bytes a lane.
+template <int MI, int NI>
+constexpr unsigned grouped_space() { return 16 * (16 * NI + 4) * 4; }
+template <typename TC, int MI, int NI>
+__device__ __forceinline__ void grouped_write(TC *c, size_t rsc, const v4f (&acc)[MI][NI], unsigned row0, unsigned col0, unsigned rows, unsigned cols, skl_scalar alpha, skl_scalar beta, char *space) {
+  constexpr int W = 16 * NI, P = W + 4, E = 16 / (int)sizeof(TC);  // a lane's columns
+  constexpr int kLanes = W / E, kDown = 64 / kLanes < 16 ? 64 / kLanes : 16;
+  typedef TC RunC __attribute__((ext_vector_type(E), aligned(sizeof(TC))));
+  const unsigned lane = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u));
+  const bool read_c = !skl_beta_is_zero<float>(beta);
+  float *const stage = reinterpret_cast<float *>(space);
+  const unsigned r_lane = lane / kLanes, col = col0 + lane % kLanes * E;
+#pragma unroll
+  for (int i = 0; i < MI; ++i) {
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int j = 0; j < NI; ++j) *reinterpret_cast<v4f *>(stage + (lane & 15u) * P + 16 * j + 4 * (lane >> 4)) = acc[i][j];
+#pragma unroll
+    for (int d = 0; d < 16; d += kDown) {
+      const unsigned r = d + r_lane, row = row0 + 16 * i + r;
+      if (r >= 16 || row >= rows || col >= cols) continue;
+      TC *const to = c + (size_t)row * rsc + col;
+      float v[E];
+#pragma unroll
+      for (int q = 0; q < E; q += 4) *reinterpret_cast<v4f *>(v + q) = *reinterpret_cast<const v4f *>(stage + r * P + lane % kLanes * E + q);
+      if (col + E <= cols) {
+        RunC old, out;
+        if (read_c) old = *reinterpret_cast<const RunC *>(to);
+#pragma unroll
+        for (int q = 0; q < E; ++q) out[q] = (TC)(read_c ? skl_combine(v[q], (float)old[q], alpha, beta) : skl_initialise_plain(v[q], alpha, beta));
+        *reinterpret_cast<RunC *>(to) = out;
+      } else {
+#pragma unroll
+        for (int q = 0; q < E; ++q)
+          if (col + q < cols) to[q] = skl_grouped_result(v[q], to + q, alpha, beta, read_c);
+      }
+    }
+  }
+}
+
+// One tile. a, b: where its lines begin (GroupedLoader::init), k in bytes where an operand has it side by side, in steps where not; c with its first row and column.
+struct GroupedTile {
+  const char *a, *b;
+  const int32_t *index;
+  unsigned limit, a_first, a_count, b_first, b_count, k;  // k: values
+  char *c;
+  unsigned rows, cols;  // of C from there on
+};
+
+template <int DT, bool A_KC, bool B_KC, int BM, int BN, int WAVES, int WAVES_N>
+struct GroupedRing {
+  using M = RingMma<DT, DT, false>;
+  static constexpr int WAVES_M = WAVES / WAVES_N, WM = BM / WAVES_M, WN = BN / WAVES_N, MI = WM / 16, NI = WN / 16;
+  using LA = GroupedLoader<A_KC, BM, WAVES>;
+  using LB = GroupedLoader<B_KC, BN, WAVES>;
+  using RA = FragReader<2, A_KC, 16, BM, 4, 16, false>;
+  using RB = FragReader<2, B_KC, 16, BN, 4, 16, false>;
+  static constexpr int PA = RA::kPieces, PB = RB::kPieces, kReadsB = NI * PB, kReads = kReadsB + MI * PA, kSlots = MI * NI, kReadSlots = kSlots * 3 / 4 > 0 ? kSlots * 3 / 4 : 1;
+  static constexpr int kPairA = A_KC ? LA::kBlocks : 0, kPairB = B_KC ? LB::kBlocks : 0, kEachA = A_KC ? 0 : LA::kBlocks, kEachB = B_KC ? 0 : LB::kBlocks, kEach = kEachA + kEachB;
+  // Requests of a step, U its parity: pairs of slices s + 3, s + 4 in odd steps, whose stages the barrier in front has freed, and slice s + 4 in every step.
+  static constexpr int kLoads[2] = {kEach, kPairA + kPairB + kEach};
+  // ... that may be under way at the barrier of slice s, where slice s + 1 has to be there: what was requested behind the last of it.
+  static constexpr int in_flight(int u) {
+    int most = 63;
+    if (kPairA + kPairB) {
+      const int x = kLoads[1] - kPairA - kPairB + kLoads[0] + (u == 0 ? kLoads[1] : 0);
+      most = x < most ? x : most;
+    }
+    if (kEach) {
+      const int x = kLoads[0] + kLoads[1];
+      most = x < most ? x : most;
+    }
+    return most;
+  }
+  static constexpr int kInFlight[2] = {in_flight(0), in_flight(1)};
+  static_assert(kInFlight[1] + kLoads[1] < 64, "vmcnt is a 6-bit counter");
+  static constexpr unsigned kRegionA = STile<2, A_KC, BM, 4, 16>::kRegion, kLdsRing = kRegionA + STile<2, B_KC, BN, 4, 16>::kRegion, kLdsRows = WAVES * grouped_space<MI, NI>();
+  static constexpr unsigned kLds = kLdsRing > kLdsRows ? kLdsRing : kLdsRows;
+
+  static constexpr int first_in_slot(int q, int n, int m) { return q >= m ? n : (q * n + m - 1) / m; }
+  static constexpr int first_load(int q, int n, int m) { return q >= m ? n : q * 2 * n <= m ? 0 : (2 * q * n - m + 2 * m - 1) / (2 * m); }
+
+  __device__ __forceinline__ static void run(const GroupedRingArgs &p, const GroupedTile &t, char *smem) {
+    char *const region_a = smem, *const region_b = smem + kRegionA;
+    const unsigned addr_a = (unsigned)(size_t)LDS_PTR(char, smem), addr_b = addr_a + kRegionA;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / WAVES_N * WM, wn = wave % WAVES_N * WN;
+    LA la;
+    LB lb;
+    la.init(t.a, p.a_pitch, t.index, t.limit, t.a_first, t.a_count, A_KC ? t.k * 2 : t.k);
+    lb.init(t.b, p.b_pitch, nullptr, 0, t.b_first, t.b_count, B_KC ? t.k * 2 : t.k);
+    RA ra;
+    RB rb;
+    ra.init(wm);
+    rb.init(wn);
+    v4f acc[MI][NI];
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+      for (int j = 0; j < NI; ++j) acc[i][j] = v4f{0, 0, 0, 0};
+    const unsigned slices = (t.k * 2 + 2 * kRingSlice - 1) / (2 * kRingSlice) * 2, pairs = slices / 2;
+    if (slices != 0) {
+      const auto request_a = [&](unsigned unit, unsigned stage) __attribute__((always_inline)) {
+        const unsigned most = (A_KC ? pairs : slices) - 1, u = unit < most ? unit : most;
+#pragma unroll
+        for (int i = 0; i < LA::kBlocks; ++i) la.request(region_a, (int)stage, u, la.left_of(u), i);
+      };
+      const auto request_b = [&](unsigned unit, unsigned stage) __attribute__((always_inline)) {
+        const unsigned most = (B_KC ? pairs : slices) - 1, u = unit < most ? unit : most;
+#pragma unroll
+        for (int i = 0; i < LB::kBlocks; ++i) lb.request(region_b, (int)stage, u, lb.left_of(u), i);
+      };
+      // What the steps before the first would have requested, in their order.
+#pragma unroll
+      for (int step = -4; step < 0; ++step) {
+        if (A_KC && (step & 1) && step + 3 >= 0) request_a((step + 3) / 2, step + 3);
+        if (B_KC && (step & 1) && step + 3 >= 0) request_b((step + 3) / 2, step + 3);
+        if (!A_KC) request_a(step + 4, step + 4);
+        if (!B_KC) request_b(step + 4, step + 4);
+      }
+      wait_loads_upto<kInFlight[1] + kLoads[1]>();  // slice 0
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+
+      typename RA::Piece pa[2][MI][PA];
+      typename RB::Piece pb[2][NI][PB];
+      const auto read_item = [&](auto rc, auto bufc, unsigned stage_a, unsigned stage_b) __attribute__((always_inline)) {
+        constexpr int R = decltype(rc)::value, BUF = decltype(bufc)::value;
+        if constexpr (R < kReadsB) pb[BUF][R / PB][R % PB] = rb.template read<R / PB, R % PB>(stage_b);
+        else pa[BUF][(R - kReadsB) / PA][(R - kReadsB) % PA] = ra.template read<(R - kReadsB) / PA, (R - kReadsB) % PA>(stage_a);
+      };
+      const auto landed = [&](int buf) __attribute__((always_inline)) {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+          for (int w = 0; w < PA; ++w) asm volatile("" : "+v"(pa[buf][i][w]));
+#pragma unroll
+        for (int j = 0; j < NI; ++j)
+#pragma unroll
+          for (int w = 0; w < PB; ++w) asm volatile("" : "+v"(pb[buf][j][w]));
+      };
+      [&]<int... Rs>(std::integer_sequence<int, Rs...>) __attribute__((always_inline)) {
+        (read_item(std::integral_constant<int, Rs>{}, std::integral_constant<int, 0>{}, addr_a, addr_b), ...);
+      }(std::make_integer_sequence<int, kReads>{});
+
+      unsigned s0 = 0;
+      do {
+        [&]<int... Us>(std::integer_sequence<int, Us...>) __attribute__((always_inline)) {
+          (
+              [&](auto uc) __attribute__((always_inline)) {
+                constexpr int U = decltype(uc)::value, kHere = kLoads[U];
+                const unsigned s = s0 + U;
+                unsigned unit_a, unit_b, next_a, next_b, left_a, left_b;
+                int fill_a, fill_b;
+                // The next slice is there for every wave, and everybody has read the one whose stage is refilled.
+                wait_loads_upto<kInFlight[U]>();
+                landed(U);
+                __builtin_amdgcn_s_barrier();
+                __builtin_amdgcn_sched_barrier(0);
+                [&]<int... Qs>(std::integer_sequence<int, Qs...>) __attribute__((always_inline)) {
+                  (
+                      [&](auto qc) __attribute__((always_inline)) {
+                        constexpr int Q = decltype(qc)::value, i = Q / NI, j = Q % NI;
+                        M::template run<true>(join_pieces<v4i>(pa[U][i]), join_pieces<v4i>(pb[U][j]), acc[i][j]);
+                        __builtin_amdgcn_sched_barrier(0);
+                        if constexpr (Q == 0) {
+                          const auto unit = [&](bool kc) {
+                            const unsigned x = kc ? (s + 3) / 2 : s + 4, most = (kc ? pairs : slices) - 1;
+                            return x < most ? x : most;
+                          };
+                          unit_a = unit(A_KC), unit_b = unit(B_KC);
+                          left_a = la.left_of(unit_a), left_b = lb.left_of(unit_b);
+                          fill_a = (int)((s + (A_KC ? 3 : 4)) % 4), fill_b = (int)((s + (B_KC ? 3 : 4)) % 4);
+                          next_a = addr_a + (s + 1) % 4 * STile<2, A_KC, BM, 4, 16>::kStageStep, next_b = addr_b + (s + 1) % 4 * STile<2, B_KC, BN, 4, 16>::kStageStep;
+                        }
+                        [&]<int... Rs>(std::integer_sequence<int, Rs...>) __attribute__((always_inline)) {
+                          (read_item(std::integral_constant<int, first_in_slot(Q, kReads, kReadSlots) + Rs>{}, std::integral_constant<int, U ^ 1>{}, next_a, next_b), ...);
+                        }(std::make_integer_sequence<int, first_in_slot(Q + 1, kReads, kReadSlots) - first_in_slot(Q, kReads, kReadSlots)>{});
+                        constexpr int L = first_load(Q, kHere, kSlots), kLoadsHere = first_load(Q + 1, kHere, kSlots) - L;
+#pragma unroll
+                        for (int l = L; l < L + kLoadsHere; ++l) {
+                          constexpr int pair_a = U ? kPairA : 0, pair_b = U ? kPairB : 0;
+                          const int each = l - pair_a - pair_b;
+                          if (l < pair_a) la.request(region_a, fill_a, unit_a, left_a, l);
+                          else if (l < pair_a + pair_b) lb.request(region_b, fill_b, unit_b, left_b, l - pair_a);
+                          else if (each < kEachA) la.request(region_a, fill_a, unit_a, left_a, each);
+                          else lb.request(region_b, fill_b, unit_b, left_b, each - kEachA);
+                        }
+                        __builtin_amdgcn_sched_barrier(0);
+                      }(std::integral_constant<int, Qs>{}),
+                      ...);
+                }(std::make_integer_sequence<int, kSlots>{});
+              }(std::integral_constant<int, Us>{}),
+              ...);
+        }(std::make_integer_sequence<int, 2>{});
+        asm volatile("s_nop 7");  // the last product's passes: the compiler, to which it is no matrix instruction, may copy its sums as soon as the loop is left
+        s0 += 2;
+      } while (s0 < slices);
+      __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
+      landed(0);                           // the last step's reads, of a slice that does not exist: their registers are theirs up to here
+      asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
+#pragma unroll
+      for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < NI; ++j) acc[i][j] = fetched<true>(acc[i][j]);
+    }
+    __syncthreads();  // every wave's reads of the stages and requests into them are over
+    char *const space = smem + wave * grouped_space<MI, NI>();
+    if (p.c_single) grouped_write<float, MI, NI>(reinterpret_cast<float *>(t.c), p.rsc, acc, wm, wn, t.rows, t.cols, p.alpha, p.beta, space);
+    else if constexpr (DT == SKL_DT_BF16) grouped_write<__bf16, MI, NI>(reinterpret_cast<__bf16 *>(t.c), p.rsc, acc, wm, wn, t.rows, t.cols, p.alpha, p.beta, space);
+    else grouped_write<_Float16, MI, NI>(reinterpret_cast<_Float16 *>(t.c), p.rsc, acc, wm, wn, t.rows, t.cols, p.alpha, p.beta, space);
+  }
+};
+
+// Which tile of which group a workgroup takes. `whole` tiles of MOST rows come first, group after group, then one for what is left of each group; both are dealt out to the
+// eight dies in runs, so that a die's workgroups share operands. Lane l counts for groups l * each .. + each - 1.
+struct GroupedPlace {
+  unsigned e, first, rows, tile_n;  // rows first .. first + rows - 1 of A and C
+  bool none;
+};
+template <int MOST>
+__device__ __forceinline__ GroupedPlace grouped_place(const int32_t *offsets, unsigned groups, unsigned m, unsigned tiles_n, unsigned id) {
+  const unsigned lane = threadIdx.x & 63u, each = (groups + 63) / 64, g0 = lane * each;
+  unsigned whole = 0, rest = 0;
+  for (unsigned g = g0; g < g0 + each && g < groups; ++g) {
+    const unsigned rows = skl_group_range(offsets, g, m).rows;
+    whole += rows / MOST, rest += rows % MOST != 0;
+  }
+  const unsigned whole_upto = skl_wave_scan(whole), rest_upto = skl_wave_scan(rest);
+  const unsigned all_whole = (unsigned)__builtin_amdgcn_readlane((int)whole_upto, 63) * tiles_n, all_rest = (unsigned)__builtin_amdgcn_readlane((int)rest_upto, 63) * tiles_n;
+  // This die's share of both, one after the other.
+  const unsigned die = id % 8, slot = id / 8;
+  const unsigned whole_first = all_whole / 8 * die + (die < all_whole % 8 ? die : all_whole % 8), whole_mine = all_whole / 8 + (die < all_whole % 8);
+  const unsigned rest_first = all_rest / 8 * die + (die < all_rest % 8 ? die : all_rest % 8), rest_mine = all_rest / 8 + (die < all_rest % 8);
+  GroupedPlace at{0, 0, 0, 0, slot >= whole_mine + rest_mine};
+  if (at.none) return at;
+  const bool is_whole = slot < whole_mine;
+  const unsigned t = is_whole ? whole_first + slot : rest_first + slot - whole_mine, line = t / tiles_n;  // line: row of tiles
+  const unsigned upto = is_whole ? whole_upto : rest_upto, mine = is_whole ? whole : rest;
+  const int owner = (int)__builtin_ctzll(__ballot(line < upto));
+  unsigned before = (unsigned)__builtin_amdgcn_readlane((int)(upto - mine), owner);  // lines of the groups ahead
+  unsigned e = (unsigned)owner * each;
+  SklRange r;
+  unsigned lines;
+  for (;; ++e) {
+    r = skl_group_range(offsets, e, m);
+    lines = is_whole ? r.rows / MOST : r.rows % MOST != 0;
+    if (line < before + lines) break;
+    before += lines;
+  }
+  at.e = e;
+  if (is_whole) {  // up to eight lines of a group column by column
+    const unsigned in = t - before * tiles_n, block = in / (8 * tiles_n), in_block = in - block * (8 * tiles_n), deep = lines - 8 * block < 8 ? lines - 8 * block : 8;
+    at.tile_n = in_block / deep;
+    at.first = r.first + (8 * block + in_block % deep) * MOST;
+    at.rows = MOST;
+  } else {
+    at.tile_n = t % tiles_n;
+    at.first = r.first + r.rows / MOST * MOST;
+    at.rows = r.rows % MOST;
+  }
+  // uniform, and the compiler is told: branches and descriptors go by them
+  at.e = (unsigned)__builtin_amdgcn_readfirstlane((int)at.e), at.first = (unsigned)__builtin_amdgcn_readfirstlane((int)at.first);
+  at.rows = (unsigned)__builtin_amdgcn_readfirstlane((int)at.rows), at.tile_n = (unsigned)__builtin_amdgcn_readfirstlane((int)at.tile_n);
+  return at;
+}
+
+template <int DT, bool B_KC, int MOST, int BN, int WAVES>
+struct GroupedRows {
+  using Full = GroupedRing<DT, true, B_KC, MOST, BN, WAVES, MOST == 64 ? WAVES : MOST == 128 ? WAVES / 2 : 2>;
+  using Half = GroupedRing<DT, true, B_KC, 128, BN, WAVES, WAVES / 2>;
+  using Quarter = GroupedRing<DT, true, B_KC, 64, BN, WAVES, WAVES>;
+  static constexpr unsigned kLds = Full::kLds;
+};
+
+template <int DT, bool B_KC, int MOST, int BN, int WAVES>
+__global__ void __launch_bounds__(WAVES * 64) gemm_grouped_rows_kernel(GroupedRingArgs p) {
+  using Rows = GroupedRows<DT, B_KC, MOST, BN, WAVES>;
+  extern __shared__ __attribute__((aligned(128))) char grouped_smem[];
+  const GroupedPlace at = grouped_place<MOST>(p.offsets, p.groups, p.m, p.tiles_n, blockIdx.x);
+  if (at.none) return;
+  const unsigned col0 = at.tile_n * BN;
+  GroupedTile t;
+  t.a = p.a, t.index = p.rows, t.limit = p.rows ? p.a_rows : p.m, t.a_first = at.first, t.a_count = at.rows;
+  t.b = p.b + (size_t)at.e * p.b_group, t.b_first = col0, t.b_count = p.n - col0, t.k = p.k;
+  t.c = p.c + ((size_t)at.first * p.rsc + col0) * (p.c_single ? 4 : 2), t.rows = at.rows, t.cols = p.n - col0;
+  if constexpr (MOST > 128) {
+    if (at.rows > 128) Rows::Full::run(p, t, grouped_smem);
+    else if (at.rows > 64) Rows::Half::run(p, t, grouped_smem);
+    else Rows::Quarter::run(p, t, grouped_smem);
+  } else {
+    Rows::Full::run(p, t, grouped_smem);
+  }
+}
+
+// Sums over the groups' rows: both operands across K, tiles of BM x BN of each group's C.
+template <int DT, int BM, int BN, int WAVES, int WAVES_N>
+__global__ void __launch_bounds__(WAVES * 64) gemm_grouped_over_kernel(GroupedRingArgs p) {
+  using Ring = GroupedRing<DT, false, false, BM, BN, WAVES, WAVES_N>;
+  extern __shared__ __attribute__((aligned(128))) char grouped_smem[];
+  // a die takes a run of tiles, which are walked in groups of eight rows of tiles, column by column
+  const unsigned all = p.groups * p.tiles_m * p.tiles_n, die = blockIdx.x % 8, slot = blockIdx.x / 8;
+  const unsigned id = all / 8 * die + (die < all % 8 ? die : all % 8) + slot;
+  if (slot >= all / 8 + (die < all % 8)) return;
+  const unsigned e = id / (p.tiles_m * p.tiles_n), in = id % (p.tiles_m * p.tiles_n);
+  const unsigned block = in / (8 * p.tiles_n), in_block = in - block * (8 * p.tiles_n), deep = p.tiles_m - 8 * block < 8 ? p.tiles_m - 8 * block : 8;
+  const unsigned row0 = (8 * block + in_block % deep) * BM, col0 = in_block / deep * BN;
+  SklRange r = skl_group_range(p.offsets, e, p.k);
+  r.first = (unsigned)__builtin_amdgcn_readfirstlane((int)r.first), r.rows = (unsigned)__builtin_amdgcn_readfirstlane((int)r.rows);
+  GroupedTile t;
+  t.a = p.a + (size_t)r.first * p.a_pitch, t.index = nullptr, t.limit = 0, t.a_first = row0, t.a_count = p.m - row0;
+  t.b = p.b + (size_t)r.first * p.b_pitch, t.b_first = col0, t.b_count = p.n - col0, t.k = r.rows;
+  t.c = p.c + ((size_t)e * p.gsc + (size_t)row0 * p.rsc + col0) * (p.c_single ? 4 : 2), t.rows = p.m - row0, t.cols = p.n - col0;
+  Ring::run(p, t, grouped_smem);
+}
+
+}  // namespace
