@@ -2,7 +2,8 @@
 //
 // C = alpha * A[rows] * B_e + beta * C by groups of rows, and C_e = alpha * A[rows]^T * B[rows] + beta * C_e by groups of what is summed over. 128 x 128 tiles
 // of four waves, operands through registers into two stages of 64 k in LDS in the orientation they have in memory.
-#include "skl_grouped_ring.hpp"
+#include "skl_gemm_mfma_impl.hpp"
+#include "skl_groups.hpp"
 #include "../../include/skl-hip.h"
 
 namespace {
@@ -213,93 +214,6 @@ int launch(const GroupedArgs &p, size_t blocks) {
 // Workgroups of a launch: beyond 2^32 threads the runtime takes what is left of the number in 32 bits.
 constexpr size_t kMostBlocks = size_t(1) << 23;
 
-// The streaming kernels: operands and the distances of their lines on 16-byte boundaries, whole 16 bytes of what lies side by side along k, offsets in 32 bits.
-template <typename K>
-int launch_ring(K kernel, std::atomic<int> &allowed, unsigned lds, unsigned threads, const GroupedRingArgs &p, size_t blocks) {
-  if (!allowed.load(std::memory_order_relaxed)) {
-    const int rc = skl_check_hip(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds), "gemm_grouped: LDS size");
-    if (rc != 0) return rc;
-    allowed.store(1, std::memory_order_relaxed);
-  }
-  kernel<<<dim3((unsigned)blocks), dim3(threads), lds, skl_current_stream()>>>(p);
-  return skl_check_launch("gemm_grouped");
-}
-constexpr size_t kMostRingBlocks = size_t(1) << 22;
-constexpr size_t kReach = 0xC0000000u;  // GroupedLoader::kRange
-
-bool aligned16(const void *p, size_t distance) { return ((uintptr_t)p & 15) == 0 && distance % 8 == 0; }
-
-bool ring_takes(const skl_grouped_gemm &g) {
-  const bool kc = g.rsb == 1;
-  const size_t line = kc ? g.csb : g.rsb;
-  return (kc || g.csb == 1) && g.k % 8 == 0 && g.k != 0 && aligned16(g.a, g.rsa) && aligned16(g.b, line) && (g.groups == 1 || g.gsb % 8 == 0) && line < kReach / 1024 && g.rsa < kReach / 1024 &&
-         (!g.rows || (g.a_rows * g.rsa + g.k) * 2 < kReach);
-}
-
-template <int DT, bool B_KC, int MOST, int BN, int WAVES>
-int grouped_rows(const skl_grouped_gemm &g, GroupedRingArgs p) {
-  const size_t lines = g.m / MOST + (g.m < g.groups ? g.m : g.groups);  // of tiles: whole ones, and one more for each group that has a row
-  const size_t most = kMostRingBlocks / (lines + 16) > 0 ? kMostRingBlocks / (lines + 16) : 1, slab = most * BN;
-  static std::atomic<int> allowed{0};
-  for (size_t col = 0; col < g.n; col += slab) {
-    p.n = (unsigned)(g.n - col < slab ? g.n - col : slab);
-    p.tiles_n = skl_div_up(p.n, BN);
-    p.b = (const char *)g.b + col * g.csb * 2;
-    p.c = (char *)g.c + col * (g.c_single ? 4 : 2);
-    const int rc = launch_ring(gemm_grouped_rows_kernel<DT, B_KC, MOST, BN, WAVES>, allowed, GroupedRows<DT, B_KC, MOST, BN, WAVES>::kLds, WAVES * 64, p, (lines * p.tiles_n / 8 + 2) * 8);
-    if (rc != 0) return rc;
-  }
-  return 0;
-}
-template <int DT, bool B_KC>
-int grouped_rows_by_size(const skl_grouped_gemm &g, const GroupedRingArgs &p) {
-  if (g.m <= 64 * g.groups) return grouped_rows<DT, B_KC, 64, 128, 4>(g, p);
-  return grouped_rows<DT, B_KC, 256, 256, 8>(g, p);
-}
-template <int DT>
-int grouped_ring(const skl_grouped_gemm &g) {
-  const bool kc = g.rsb == 1;
-  GroupedRingArgs p{};
-  p.a = (const char *)g.a, p.offsets = g.offsets, p.rows = g.rows;
-  p.a_pitch = g.rsa * 2, p.b_pitch = (kc ? g.csb : g.rsb) * 2, p.b_group = g.gsb * 2;
-  p.rsc = g.rsc, p.groups = (unsigned)g.groups, p.m = (unsigned)g.m, p.k = (unsigned)g.k, p.a_rows = (unsigned)g.a_rows;
-  p.c_single = g.c_single, p.alpha = g.alpha, p.beta = g.beta;
-  return kc ? grouped_rows_by_size<DT, true>(g, p) : grouped_rows_by_size<DT, false>(g, p);
-}
-
-bool ring_takes(const skl_groupedk_gemm &g) {
-  return !g.rows_a && !g.rows_b && aligned16(g.a, g.rsa) && aligned16(g.b, g.rsb) && g.rsa < kReach / 1024 && g.rsb < kReach / 1024;
-}
-template <int DT, int BM, int BN, int WAVES, int WAVES_N>
-int grouped_over(const skl_groupedk_gemm &g, GroupedRingArgs p) {
-  p.tiles_m = skl_div_up(g.m, BM);
-  const size_t all_n = skl_div_up(g.n, BN), left = kMostRingBlocks / p.tiles_m > 0 ? kMostRingBlocks / p.tiles_m : 1;
-  const size_t slab_n = (left < all_n ? left : all_n) * BN, slab = left / all_n > 0 ? left / all_n : 1;
-  static std::atomic<int> allowed{0};
-  for (size_t e = 0; e < g.groups; e += slab) {
-    p.groups = (unsigned)(g.groups - e < slab ? g.groups - e : slab);
-    p.offsets = g.offsets ? g.offsets + e : nullptr;
-    for (size_t col = 0; col < g.n; col += slab_n) {
-      p.n = (unsigned)(g.n - col < slab_n ? g.n - col : slab_n);
-      p.tiles_n = skl_div_up(p.n, BN);
-      p.b = (const char *)g.b + col * 2;
-      p.c = (char *)g.c + (e * g.gsc + col) * (g.c_single ? 4 : 2);
-      const int rc = launch_ring(gemm_grouped_over_kernel<DT, BM, BN, WAVES, WAVES_N>, allowed, GroupedRing<DT, false, false, BM, BN, WAVES, WAVES_N>::kLds, WAVES * 64, p,
-                                 ((size_t)p.groups * p.tiles_m * p.tiles_n + 7) / 8 * 8);
-      if (rc != 0) return rc;
-    }
-  }
-  return 0;
-}
-template <int DT>
-int grouped_over_ring(const skl_groupedk_gemm &g) {
-  GroupedRingArgs p{};
-  p.a = (const char *)g.a, p.a_pitch = g.rsa * 2, p.b_pitch = g.rsb * 2;
-  p.rsc = g.rsc, p.gsc = g.gsc, p.m = (unsigned)g.m, p.k = (unsigned)g.total;
-  p.c_single = g.c_single, p.alpha = g.alpha, p.beta = g.beta;
-  return grouped_over<DT, 256, 256, 8, 2>(g, p);
-}
-
 template <int DT, typename T>
 int grouped(const skl_grouped_gemm &g, GroupedArgs p) {
   const auto by_layout = [&](auto c, size_t blocks) {
@@ -345,7 +259,7 @@ int groupedk(const skl_groupedk_gemm &g, GroupedArgs p) {
 }  // namespace
 
 int skl_hip_launch_gemm_grouped(const skl_grouped_gemm *g) {
-  if (ring_takes(*g)) return g->dt == SKL_DT_BF16 ? grouped_ring<SKL_DT_BF16>(*g) : grouped_ring<SKL_DT_F16>(*g);
+  if (skl_grouped_ring_takes(*g)) return g->dt == SKL_DT_BF16 ? skl_launch_grouped_ring_bf16(*g) : skl_launch_grouped_ring_f16(*g);
   GroupedArgs p{};
   p.a = (const uint16_t *)g->a, p.offsets = g->offsets, p.rows_a = g->rows;
   p.rsa = g->rsa, p.rsb = g->rsb, p.csb = g->csb, p.gsb = g->gsb, p.rsc = g->rsc;
@@ -355,7 +269,7 @@ int skl_hip_launch_gemm_grouped(const skl_grouped_gemm *g) {
 }
 
 int skl_hip_launch_gemm_groupedk(const skl_groupedk_gemm *g) {
-  if (ring_takes(*g)) return g->dt == SKL_DT_BF16 ? grouped_over_ring<SKL_DT_BF16>(*g) : grouped_over_ring<SKL_DT_F16>(*g);
+  if (skl_groupedk_ring_takes(*g)) return g->dt == SKL_DT_BF16 ? skl_launch_groupedk_ring_bf16(*g) : skl_launch_groupedk_ring_f16(*g);
   GroupedArgs p{};
   p.a = (const uint16_t *)g->a, p.rows_a = g->rows_a, p.rows_b = g->rows_b;
   p.rsa = g->rsa, p.rsb = g->rsb, p.rsc = g->rsc, p.gsc = g->gsc;

@@ -8,16 +8,17 @@
 
 #include "skl_gemm_mfma_impl.hpp"
 #include "skl_groups.hpp"
+#include "../../include/skl-hip.h"
 
 namespace {
 
 struct GroupedRingArgs {
   const char *a, *b;
-  const int32_t *offsets, *rows;
+  const int32_t *offsets, *rows, *rows_b;  // rows: of A
   char *c;
   size_t a_pitch, b_pitch, b_group;  // bytes: from one line of an operand to the next - rows or columns with K side by side, or steps of K -, from one group's B to the next
   size_t rsc, gsc;                   // elements
-  unsigned groups, m, n, k, a_rows;  // OVER: k is the number of rows in all
+  unsigned groups, m, n, k, a_rows, b_rows;  // OVER: k is the number of rows in all
   unsigned tiles_m, tiles_n;         // OVER: of a group
   int c_single;
   skl_scalar alpha, beta;
@@ -25,7 +26,8 @@ struct GroupedRingArgs {
 
 // Requests of one operand, this wave's share: lines of ROWS rows or columns with K side by side (KC), a pair of slices at a time, or lines of ROWS values across K, a slice at a time. All
 // through a buffer descriptor; what does not exist has an offset beyond its range, for which zeros arrive and no memory is touched.
-template <bool KC, int ROWS, int WAVES>
+// INDEXED (not KC): the steps of K are rows through an index. A wave's part of a slice is a few rows, whose numbers come as scalars a step ahead of the requests.
+template <bool KC, int ROWS, int WAVES, bool INDEXED>
 struct GroupedLoader {
   using T = STile<2, KC, ROWS, 4, 16>;
   static constexpr unsigned kRange = 0xC0000000u, kOutside = 0xE0000000u;
@@ -33,9 +35,14 @@ struct GroupedLoader {
   static_assert(kBlocks >= 1);
   static constexpr unsigned kBlockStep = KC ? T::kGroup : 1024;
   static constexpr unsigned kUnitK = KC ? 2 * kRingSlice : kRingSlice / 2;  // bytes or steps of K
+  static constexpr int kLanesPerRow = KC ? 1 : T::kRowBytes / 16, kRowsPerBlock = KC ? 1 : 1024 / T::kRowBytes, kRows = kBlocks * kRowsPerBlock;
   const char *base;
   size_t k_step;
   unsigned off[kBlocks], k_lane[KC ? 2 : kBlocks], k_total, lds;
+  const __attribute__((address_space(4))) char *index;  // this wave's first row's; read by scalar loads
+  unsigned index_left, index_limit, index_pitch;        // index_left: rows from there on less one
+  typedef int Lines __attribute__((ext_vector_type(kRows < 2 ? 2 : kRows)));
+  Lines ahead, line;  // rows of the next step's unit; offsets of this step's (vectors: arrays in here are kept in memory)
 
   __device__ __forceinline__ static const char *scalar(const char *p) {
     const uintptr_t at = (uintptr_t)p;
@@ -43,7 +50,8 @@ struct GroupedLoader {
   }
   // KC: lines first .. first + count - 1, through `index` where there is one (of `limit` lines); else columns at .. of `count` from there on, steps of K `pitch` apart.
   // k: bytes (KC) or steps.
-  __device__ __forceinline__ void init(const char *from, size_t pitch, const int32_t *index, unsigned limit, unsigned first, unsigned count, unsigned k) {
+  // INDEXED: step r is row index[index_at + r] of `limit`.
+  __device__ __forceinline__ void init(const char *from, size_t pitch, const int32_t *index, unsigned index_at, unsigned limit, unsigned first, unsigned count, unsigned k) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     lds = wave * kBlocks * kBlockStep;
     k_total = k;
@@ -57,7 +65,7 @@ struct GroupedLoader {
         if (i < 2) k_lane[i] = in_k;  // (the blocks' turns alternate)
         unsigned line = (unsigned)row < count ? (unsigned)row : ~0u;
         if (index && line != ~0u) {
-          line = (unsigned)index[first + line];
+          line = (unsigned)index[index_at + line];
           if (line >= limit) line = ~0u;
         }
         off[i] = line == ~0u ? kOutside : line * (unsigned)pitch + in_k;
@@ -67,16 +75,44 @@ struct GroupedLoader {
       k_step = ((size_t)(unsigned)__builtin_amdgcn_readfirstlane((int)((pitch * kUnitK) >> 32)) << 32) | (unsigned)__builtin_amdgcn_readfirstlane((int)(pitch * kUnitK));
 #pragma unroll
       for (int i = 0; i < kBlocks; ++i) {
-        constexpr int kLanesPerRow = T::kRowBytes / 16, kRowsPerBlock = 1024 / T::kRowBytes;
         const int kr = kRowsPerBlock * (wave * kBlocks + i) + lane / kLanesPerRow, mn = ((T::chunk(kr, lane % kLanesPerRow) - kr * T::kRowBytes) >> 4) * 8;
         k_lane[i] = kr;
-        off[i] = (unsigned)mn < count ? (unsigned)kr * (unsigned)pitch + (unsigned)mn * 2 : kOutside;
+        off[i] = (unsigned)mn < count ? (INDEXED ? 0u : (unsigned)kr * (unsigned)pitch) + (unsigned)mn * 2 : kOutside;
       }
+      if constexpr (INDEXED) {
+        const unsigned mine = (unsigned)wave * kRows;
+        this->index = (const __attribute__((address_space(4))) char *)(uintptr_t)scalar((const char *)(index + index_at + (mine < k ? mine : k - 1)));
+        index_left = mine < k ? k - 1 - mine : 0, index_limit = limit, index_pitch = (unsigned)pitch;
+        k_step = 0;
+      }
+    }
+  }
+  // The rows of the part of `unit` that is this wave's; beyond the last one that one again.
+  __device__ __forceinline__ void look_ahead(unsigned unit) {
+    if constexpr (INDEXED) {
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) {
+        const unsigned at = unit * kUnitK + r;
+        ahead[r] = *(const __attribute__((address_space(4))) int32_t *)(index + (at < index_left ? at : index_left) * 4u);
+      }
+    }
+  }
+  __device__ __forceinline__ void look() {
+    if constexpr (INDEXED) {
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) line[r] = (int)((unsigned)ahead[r] < index_limit ? (unsigned)ahead[r] * index_pitch : kOutside);
     }
   }
   __device__ __forceinline__ unsigned left_of(unsigned unit) const { return k_total > unit * kUnitK ? k_total - unit * kUnitK : 0; }
   __device__ __forceinline__ void request(char *region, int stage, unsigned unit, unsigned left, int i) const {
     unsigned o = k_lane[KC ? i & 1 : i] < left ? off[i] : kOutside;
+    if constexpr (INDEXED) {
+      const unsigned lane = threadIdx.x & 63u;
+      unsigned of_line = (unsigned)line[i * kRowsPerBlock];
+#pragma unroll
+      for (int r = 1; r < kRowsPerBlock; ++r) of_line = lane >= (unsigned)(r * kLanesPerRow) ? (unsigned)line[i * kRowsPerBlock + r] : of_line;
+      o = o == kOutside || of_line == kOutside ? kOutside : o + of_line;
+    }
     asm volatile("" : "+v"(o));  // (not widened to 64 bits ahead of the loop, see SLoader)
     __builtin_amdgcn_raw_ptr_buffer_load_lds(__builtin_amdgcn_make_buffer_rsrc((void *)(base + unit * k_step), 0, (int)kRange, 0x00027000),
                                              (__attribute__((address_space(3))) void *)(region + stage * T::kStageStep + lds + i * kBlockStep), 16, (int)o, 0, 0, 0);
@@ -127,18 +163,18 @@ __device__ __forceinline__ void grouped_write(TC *c, size_t rsc, const v4f (&acc
 // One tile. a, b: where its lines begin (GroupedLoader::init), k in bytes where an operand has it side by side, in steps where not; c with its first row and column.
 struct GroupedTile {
   const char *a, *b;
-  const int32_t *index;
-  unsigned limit, a_first, a_count, b_first, b_count, k;  // k: values
+  const int32_t *index, *index_b;
+  unsigned index_at, limit, limit_b, a_first, a_count, b_first, b_count, k;  // k: values
   char *c;
   unsigned rows, cols;  // of C from there on
 };
 
-template <int DT, bool A_KC, bool B_KC, int BM, int BN, int WAVES, int WAVES_N>
+template <int DT, bool A_KC, bool B_KC, int BM, int BN, int WAVES, int WAVES_N, bool A_INDEXED = false, bool B_INDEXED = false>
 struct GroupedRing {
   using M = RingMma<DT, DT, false>;
   static constexpr int WAVES_M = WAVES / WAVES_N, WM = BM / WAVES_M, WN = BN / WAVES_N, MI = WM / 16, NI = WN / 16;
-  using LA = GroupedLoader<A_KC, BM, WAVES>;
-  using LB = GroupedLoader<B_KC, BN, WAVES>;
+  using LA = GroupedLoader<A_KC, BM, WAVES, A_INDEXED>;
+  using LB = GroupedLoader<B_KC, BN, WAVES, B_INDEXED>;
   using RA = FragReader<2, A_KC, 16, BM, 4, 16, false>;
   using RB = FragReader<2, B_KC, 16, BN, 4, 16, false>;
   static constexpr int PA = RA::kPieces, PB = RB::kPieces, kReadsB = NI * PB, kReads = kReadsB + MI * PA, kSlots = MI * NI, kReadSlots = kSlots * 3 / 4 > 0 ? kSlots * 3 / 4 : 1;
@@ -172,8 +208,8 @@ struct GroupedRing {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / WAVES_N * WM, wn = wave % WAVES_N * WN;
     LA la;
     LB lb;
-    la.init(t.a, p.a_pitch, t.index, t.limit, t.a_first, t.a_count, A_KC ? t.k * 2 : t.k);
-    lb.init(t.b, p.b_pitch, nullptr, 0, t.b_first, t.b_count, B_KC ? t.k * 2 : t.k);
+    la.init(t.a, p.a_pitch, t.index, t.index_at, t.limit, t.a_first, t.a_count, A_KC ? t.k * 2 : t.k);
+    lb.init(t.b, p.b_pitch, t.index_b, t.index_at, t.limit_b, t.b_first, t.b_count, B_KC ? t.k * 2 : t.k);
     RA ra;
     RB rb;
     ra.init(wm);
@@ -187,11 +223,15 @@ struct GroupedRing {
     if (slices != 0) {
       const auto request_a = [&](unsigned unit, unsigned stage) __attribute__((always_inline)) {
         const unsigned most = (A_KC ? pairs : slices) - 1, u = unit < most ? unit : most;
+        la.look_ahead(u);
+        la.look();
 #pragma unroll
         for (int i = 0; i < LA::kBlocks; ++i) la.request(region_a, (int)stage, u, la.left_of(u), i);
       };
       const auto request_b = [&](unsigned unit, unsigned stage) __attribute__((always_inline)) {
         const unsigned most = (B_KC ? pairs : slices) - 1, u = unit < most ? unit : most;
+        lb.look_ahead(u);
+        lb.look();
 #pragma unroll
         for (int i = 0; i < LB::kBlocks; ++i) lb.request(region_b, (int)stage, u, lb.left_of(u), i);
       };
@@ -203,6 +243,8 @@ struct GroupedRing {
         if (!A_KC) request_a(step + 4, step + 4);
         if (!B_KC) request_b(step + 4, step + 4);
       }
+      la.look_ahead(4 < slices - 1 ? 4 : slices - 1);
+      lb.look_ahead(4 < slices - 1 ? 4 : slices - 1);
       wait_loads_upto<kInFlight[1] + kLoads[1]>();  // slice 0
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       __builtin_amdgcn_s_barrier();
@@ -247,7 +289,7 @@ struct GroupedRing {
                   (
                       [&](auto qc) __attribute__((always_inline)) {
                         constexpr int Q = decltype(qc)::value, i = Q / NI, j = Q % NI;
-                        M::template run<true>(join_pieces<v4i>(pa[U][i]), join_pieces<v4i>(pb[U][j]), acc[i][j]);
+                        M::template run<ring_sum_in_a<MI, NI, v4f>(i, j)>(join_pieces<v4i>(pa[U][i]), join_pieces<v4i>(pb[U][j]), acc[i][j]);
                         __builtin_amdgcn_sched_barrier(0);
                         if constexpr (Q == 0) {
                           const auto unit = [&](bool kc) {
@@ -256,6 +298,8 @@ struct GroupedRing {
                           };
                           unit_a = unit(A_KC), unit_b = unit(B_KC);
                           left_a = la.left_of(unit_a), left_b = lb.left_of(unit_b);
+                          la.look(), lb.look();  // (in front of this step's reads: the compiler waits for both together)
+                          la.look_ahead(unit_a + 1 < slices ? unit_a + 1 : unit_a), lb.look_ahead(unit_b + 1 < slices ? unit_b + 1 : unit_b);
                           fill_a = (int)((s + (A_KC ? 3 : 4)) % 4), fill_b = (int)((s + (B_KC ? 3 : 4)) % 4);
                           next_a = addr_a + (s + 1) % 4 * STile<2, A_KC, BM, 4, 16>::kStageStep, next_b = addr_b + (s + 1) % 4 * STile<2, B_KC, BN, 4, 16>::kStageStep;
                         }
@@ -285,10 +329,9 @@ struct GroupedRing {
       __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
       landed(0);                           // the last step's reads, of a slice that does not exist: their registers are theirs up to here
       asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
-#pragma unroll
-      for (int i = 0; i < MI; ++i)
-#pragma unroll
-        for (int j = 0; j < NI; ++j) acc[i][j] = fetched<true>(acc[i][j]);
+      [&]<int... Bs>(std::integer_sequence<int, Bs...>) __attribute__((always_inline)) {
+        ((acc[Bs / NI][Bs % NI] = fetched<ring_sum_in_a<MI, NI, v4f>(Bs / NI, Bs % NI)>(acc[Bs / NI][Bs % NI])), ...);
+      }(std::make_integer_sequence<int, MI * NI>{});
     }
     __syncthreads();  // every wave's reads of the stages and requests into them are over
     char *const space = smem + wave * grouped_space<MI, NI>();
@@ -367,7 +410,7 @@ __global__ void __launch_bounds__(WAVES * 64) gemm_grouped_rows_kernel(GroupedRi
   if (at.none) return;
   const unsigned col0 = at.tile_n * BN;
   GroupedTile t;
-  t.a = p.a, t.index = p.rows, t.limit = p.rows ? p.a_rows : p.m, t.a_first = at.first, t.a_count = at.rows;
+  t.a = p.a, t.index = p.rows, t.index_b = nullptr, t.index_at = at.first, t.limit = p.a_rows, t.limit_b = 0, t.a_first = at.first, t.a_count = at.rows;
   t.b = p.b + (size_t)at.e * p.b_group, t.b_first = col0, t.b_count = p.n - col0, t.k = p.k;
   t.c = p.c + ((size_t)at.first * p.rsc + col0) * (p.c_single ? 4 : 2), t.rows = at.rows, t.cols = p.n - col0;
   if constexpr (MOST > 128) {
@@ -379,25 +422,111 @@ __global__ void __launch_bounds__(WAVES * 64) gemm_grouped_rows_kernel(GroupedRi
   }
 }
 
+// The group that comes at place `place` by its length, longest first (up to 64 groups; more as they lie, which evens out by itself).
+__device__ __forceinline__ unsigned grouped_by_length(const int32_t *offsets, unsigned groups, unsigned most, unsigned place) {
+  if (groups > 64 || groups == 1) return place;
+  const unsigned lane = threadIdx.x & 63u, mine = lane < groups ? skl_group_range(offsets, lane, most).rows : 0u;
+  unsigned ahead = 0;
+  for (unsigned g = 0; g < groups; ++g) {
+    const unsigned other = (unsigned)__builtin_amdgcn_readlane((int)mine, (int)g);
+    ahead += other > mine || (other == mine && g < lane);
+  }
+  return (unsigned)__builtin_ctzll(__ballot(lane < groups && ahead == place));
+}
+
 // Sums over the groups' rows: both operands across K, tiles of BM x BN of each group's C.
-template <int DT, int BM, int BN, int WAVES, int WAVES_N>
+template <int DT, int BM, int BN, int WAVES, int WAVES_N, bool A_INDEXED, bool B_INDEXED>
 __global__ void __launch_bounds__(WAVES * 64) gemm_grouped_over_kernel(GroupedRingArgs p) {
-  using Ring = GroupedRing<DT, false, false, BM, BN, WAVES, WAVES_N>;
+  using Ring = GroupedRing<DT, false, false, BM, BN, WAVES, WAVES_N, A_INDEXED, B_INDEXED>;
   extern __shared__ __attribute__((aligned(128))) char grouped_smem[];
-  // a die takes a run of tiles, which are walked in groups of eight rows of tiles, column by column
-  const unsigned all = p.groups * p.tiles_m * p.tiles_n, die = blockIdx.x % 8, slot = blockIdx.x / 8;
-  const unsigned id = all / 8 * die + (die < all % 8 ? die : all % 8) + slot;
-  if (slot >= all / 8 + (die < all % 8)) return;
-  const unsigned e = id / (p.tiles_m * p.tiles_n), in = id % (p.tiles_m * p.tiles_n);
+  // Each die takes a run of every group's tiles - a group's length decides how long they take -, the longest group first, walked in blocks of eight rows of tiles, column by column.
+  const unsigned tiles = p.tiles_m * p.tiles_n, run = (tiles + 7) / 8, die = blockIdx.x % 8, slot = blockIdx.x / 8;
+  const unsigned in = die * run + slot % run, e = grouped_by_length(p.offsets, p.groups, p.k, slot / run);
+  if (in >= tiles) return;
   const unsigned block = in / (8 * p.tiles_n), in_block = in - block * (8 * p.tiles_n), deep = p.tiles_m - 8 * block < 8 ? p.tiles_m - 8 * block : 8;
   const unsigned row0 = (8 * block + in_block % deep) * BM, col0 = in_block / deep * BN;
   SklRange r = skl_group_range(p.offsets, e, p.k);
   r.first = (unsigned)__builtin_amdgcn_readfirstlane((int)r.first), r.rows = (unsigned)__builtin_amdgcn_readfirstlane((int)r.rows);
   GroupedTile t;
-  t.a = p.a + (size_t)r.first * p.a_pitch, t.index = nullptr, t.limit = 0, t.a_first = row0, t.a_count = p.m - row0;
-  t.b = p.b + (size_t)r.first * p.b_pitch, t.b_first = col0, t.b_count = p.n - col0, t.k = r.rows;
+  t.index = p.rows, t.index_b = p.rows_b, t.index_at = r.first, t.limit = p.a_rows, t.limit_b = p.b_rows;
+  t.a = A_INDEXED ? p.a : p.a + (size_t)r.first * p.a_pitch, t.a_first = row0, t.a_count = p.m - row0;
+  t.b = B_INDEXED ? p.b : p.b + (size_t)r.first * p.b_pitch, t.b_first = col0, t.b_count = p.n - col0, t.k = r.rows;
   t.c = p.c + ((size_t)e * p.gsc + (size_t)row0 * p.rsc + col0) * (p.c_single ? 4 : 2), t.rows = p.m - row0, t.cols = p.n - col0;
   Ring::run(p, t, grouped_smem);
+}
+
+template <typename K>
+int launch_ring(K kernel, std::atomic<int> &allowed, unsigned lds, unsigned threads, const GroupedRingArgs &p, size_t blocks) {
+  if (!allowed.load(std::memory_order_relaxed)) {
+    const int rc = skl_check_hip(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds), "gemm_grouped: LDS size");
+    if (rc != 0) return rc;
+    allowed.store(1, std::memory_order_relaxed);
+  }
+  kernel<<<dim3((unsigned)blocks), dim3(threads), lds, skl_current_stream()>>>(p);
+  return skl_check_launch("gemm_grouped");
+}
+constexpr size_t kMostRingBlocks = size_t(1) << 22;
+template <int DT, bool B_KC, int MOST, int BN, int WAVES>
+int grouped_rows(const skl_grouped_gemm &g, GroupedRingArgs p) {
+  const size_t lines = g.m / MOST + (g.m < g.groups ? g.m : g.groups);  // of tiles: whole ones, and one more for each group that has a row
+  const size_t most = kMostRingBlocks / (lines + 16) > 0 ? kMostRingBlocks / (lines + 16) : 1, slab = most * BN;
+  static std::atomic<int> allowed{0};
+  for (size_t col = 0; col < g.n; col += slab) {
+    p.n = (unsigned)(g.n - col < slab ? g.n - col : slab);
+    p.tiles_n = skl_div_up(p.n, BN);
+    p.b = (const char *)g.b + col * g.csb * 2;
+    p.c = (char *)g.c + col * (g.c_single ? 4 : 2);
+    const int rc = launch_ring(gemm_grouped_rows_kernel<DT, B_KC, MOST, BN, WAVES>, allowed, GroupedRows<DT, B_KC, MOST, BN, WAVES>::kLds, WAVES * 64, p, (lines * p.tiles_n / 8 + 2) * 8);
+    if (rc != 0) return rc;
+  }
+  return 0;
+}
+template <int DT, bool B_KC>
+int grouped_rows_by_size(const skl_grouped_gemm &g, const GroupedRingArgs &p) {
+  if (g.m <= 64 * g.groups) return grouped_rows<DT, B_KC, 64, 128, 4>(g, p);
+  return grouped_rows<DT, B_KC, 256, 256, 8>(g, p);
+}
+template <int DT>
+int grouped_ring(const skl_grouped_gemm &g) {
+  const bool kc = g.rsb == 1;
+  GroupedRingArgs p{};
+  p.a = (const char *)g.a, p.offsets = g.offsets, p.rows = g.rows;
+  p.a_pitch = g.rsa * 2, p.b_pitch = (kc ? g.csb : g.rsb) * 2, p.b_group = g.gsb * 2;
+  p.rsc = g.rsc, p.groups = (unsigned)g.groups, p.m = (unsigned)g.m, p.k = (unsigned)g.k, p.a_rows = (unsigned)g.a_rows;
+  p.c_single = g.c_single, p.alpha = g.alpha, p.beta = g.beta;
+  return kc ? grouped_rows_by_size<DT, true>(g, p) : grouped_rows_by_size<DT, false>(g, p);
+}
+
+template <int DT, int BM, int BN, int WAVES, int WAVES_N, bool A_INDEXED, bool B_INDEXED>
+int grouped_over(const skl_groupedk_gemm &g, GroupedRingArgs p) {
+  p.tiles_m = skl_div_up(g.m, BM);
+  const size_t all_n = skl_div_up(g.n, BN), left = kMostRingBlocks / p.tiles_m > 0 ? kMostRingBlocks / p.tiles_m : 1;
+  const size_t slab_n = (left < all_n ? left : all_n) * BN, slab = left / all_n > 0 ? left / all_n : 1;
+  static std::atomic<int> allowed{0};
+  for (size_t e = 0; e < g.groups; e += slab) {
+    p.groups = (unsigned)(g.groups - e < slab ? g.groups - e : slab);
+    p.offsets = g.offsets ? g.offsets + e : nullptr;
+    for (size_t col = 0; col < g.n; col += slab_n) {
+      p.n = (unsigned)(g.n - col < slab_n ? g.n - col : slab_n);
+      p.tiles_n = skl_div_up(p.n, BN);
+      p.b = (const char *)g.b + col * 2;
+      p.c = (char *)g.c + (e * g.gsc + col) * (g.c_single ? 4 : 2);
+      const int rc = launch_ring(gemm_grouped_over_kernel<DT, BM, BN, WAVES, WAVES_N, A_INDEXED, B_INDEXED>, allowed, GroupedRing<DT, false, false, BM, BN, WAVES, WAVES_N>::kLds, WAVES * 64, p,
+                                 (size_t)p.groups * (((size_t)p.tiles_m * p.tiles_n + 7) / 8) * 8);
+      if (rc != 0) return rc;
+    }
+  }
+  return 0;
+}
+template <int DT>
+int grouped_over_ring(const skl_groupedk_gemm &g) {
+  GroupedRingArgs p{};
+  p.a = (const char *)g.a, p.a_pitch = g.rsa * 2, p.b_pitch = g.rsb * 2;
+  p.rows = g.rows_a, p.rows_b = g.rows_b, p.a_rows = (unsigned)g.a_rows, p.b_rows = (unsigned)g.b_rows;
+  p.rsc = g.rsc, p.gsc = g.gsc, p.m = (unsigned)g.m, p.k = (unsigned)g.total;
+  p.c_single = g.c_single, p.alpha = g.alpha, p.beta = g.beta;
+  if (g.rows_a) return g.rows_b ? grouped_over<DT, 256, 256, 8, 2, true, true>(g, p) : grouped_over<DT, 256, 256, 8, 2, true, false>(g, p);
+  return g.rows_b ? grouped_over<DT, 256, 256, 8, 2, false, true>(g, p) : grouped_over<DT, 256, 256, 8, 2, false, false>(g, p);
 }
 
 }  // namespace

@@ -5,6 +5,23 @@
 #include "skl_device.hpp"
 #include "skl_grouped.h"
 
+// The streaming kernels (skl_grouped_ring.hpp), and what they take: operands and the distances of their lines on 16-byte boundaries, whole 16 bytes of what lies
+// side by side along k, offsets in 32 bits.
+int skl_launch_grouped_ring_bf16(const skl_grouped_gemm &g);
+int skl_launch_grouped_ring_f16(const skl_grouped_gemm &g);
+int skl_launch_groupedk_ring_bf16(const skl_groupedk_gemm &g);
+int skl_launch_groupedk_ring_f16(const skl_groupedk_gemm &g);
+constexpr size_t kGroupedReach = 0xC0000000u;  // bytes that an offset covers
+static inline bool skl_grouped_aligned(const void *p, size_t distance) { return ((uintptr_t)p & 15) == 0 && distance % 8 == 0 && distance < kGroupedReach / 1024; }
+static inline bool skl_grouped_ring_takes(const skl_grouped_gemm &g) {
+  const bool kc = g.rsb == 1;
+  return (kc || g.csb == 1) && g.k % 8 == 0 && g.k != 0 && skl_grouped_aligned(g.a, g.rsa) && skl_grouped_aligned(g.b, kc ? g.csb : g.rsb) && (g.groups == 1 || g.gsb % 8 == 0) &&
+         (!g.rows || (g.a_rows * g.rsa + g.k) * 2 < kGroupedReach);
+}
+static inline bool skl_groupedk_ring_takes(const skl_groupedk_gemm &g) {
+  return skl_grouped_aligned(g.a, g.rsa) && skl_grouped_aligned(g.b, g.rsb) && (!g.rows_a || (g.a_rows * g.rsa + g.m) * 2 < kGroupedReach) && (!g.rows_b || (g.b_rows * g.rsb + g.n) * 2 < kGroupedReach);
+}
+
 namespace {
 
 // Inclusive sum over the lanes of a wave up to this one.
