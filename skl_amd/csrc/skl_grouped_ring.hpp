@@ -12,6 +12,14 @@
 
 namespace {
 
+// 64 values across K: eight chunks of a k-row of 128 bytes, two of which fill the banks. 32 lanes of a tr16 read take k-rows r .. r + 3 and r + 8 .. r + 11, two chunks of each: rows of one
+// parity are parted by their second and fourth bits.
+template <int NS>
+struct STile<2, false, 64, NS, 16> {
+  static constexpr int kStages = NS, kBytes = 64 * kRingSlice, kRegion = kBytes * NS, kRowBytes = 128, kStageStep = kBytes, kGroup = NS * 512;
+  __device__ static __forceinline__ int chunk(int r, int c) { return r * 128 + ((c ^ ((r & 2) | (r >> 1 & 4))) << 4); }
+};
+
 struct GroupedRingArgs {
   const char *a, *b;
   const int32_t *offsets, *rows, *rows_b;  // rows: of A
@@ -27,9 +35,9 @@ struct GroupedRingArgs {
 // Requests of one operand, this wave's share: lines of ROWS rows or columns with K side by side (KC), a pair of slices at a time, or lines of ROWS values across K, a slice at a time. All
 // through a buffer descriptor; what does not exist has an offset beyond its range, for which zeros arrive and no memory is touched.
 // INDEXED (not KC): the steps of K are rows through an index. A wave's part of a slice is a few rows, whose numbers come as scalars a step ahead of the requests.
-template <bool KC, int ROWS, int WAVES, bool INDEXED>
+template <bool KC, int ROWS, int WAVES, int NS, bool INDEXED>
 struct GroupedLoader {
-  using T = STile<2, KC, ROWS, 4, 16>;
+  using T = STile<2, KC, ROWS, NS, 16>;
   static constexpr unsigned kRange = 0xC0000000u, kOutside = 0xE0000000u;
   static constexpr int kBlocks = (KC ? 2 : 1) * T::kBytes / 1024 / WAVES;  // KiB per wave and unit
   static_assert(kBlocks >= 1);
@@ -150,7 +158,7 @@ __device__ __forceinline__ void grouped_write(TC *c, size_t rsc, const v4f (&acc
         if (read_c) old = *reinterpret_cast<const RunC *>(to);
 #pragma unroll
         for (int q = 0; q < E; ++q) out[q] = (TC)(read_c ? skl_combine(v[q], (float)old[q], alpha, beta) : skl_initialise_plain(v[q], alpha, beta));
-        *reinterpret_cast<RunC *>(to) = out;
+        __builtin_nontemporal_store(out, reinterpret_cast<RunC *>(to));
       } else {
 #pragma unroll
         for (int q = 0; q < E; ++q)
@@ -169,34 +177,36 @@ struct GroupedTile {
   unsigned rows, cols;  // of C from there on
 };
 
-template <int DT, bool A_KC, bool B_KC, int BM, int BN, int WAVES, int WAVES_N, bool A_INDEXED = false, bool B_INDEXED = false>
+template <int DT, bool A_KC, bool B_KC, int BM, int BN, int WAVES, int WAVES_N, int NS, bool A_INDEXED = false, bool B_INDEXED = false>
 struct GroupedRing {
   using M = RingMma<DT, DT, false>;
   static constexpr int WAVES_M = WAVES / WAVES_N, WM = BM / WAVES_M, WN = BN / WAVES_N, MI = WM / 16, NI = WN / 16;
-  using LA = GroupedLoader<A_KC, BM, WAVES, A_INDEXED>;
-  using LB = GroupedLoader<B_KC, BN, WAVES, B_INDEXED>;
-  using RA = FragReader<2, A_KC, 16, BM, 4, 16, false>;
-  using RB = FragReader<2, B_KC, 16, BN, 4, 16, false>;
+  using LA = GroupedLoader<A_KC, BM, WAVES, NS, A_INDEXED>;
+  using LB = GroupedLoader<B_KC, BN, WAVES, NS, B_INDEXED>;
+  using RA = FragReader<2, A_KC, 16, BM, NS, 16, false>;
+  using RB = FragReader<2, B_KC, 16, BN, NS, 16, false>;
   static constexpr int PA = RA::kPieces, PB = RB::kPieces, kReadsB = NI * PB, kReads = kReadsB + MI * PA, kSlots = MI * NI, kReadSlots = kSlots * 3 / 4 > 0 ? kSlots * 3 / 4 : 1;
   static constexpr int kPairA = A_KC ? LA::kBlocks : 0, kPairB = B_KC ? LB::kBlocks : 0, kEachA = A_KC ? 0 : LA::kBlocks, kEachB = B_KC ? 0 : LB::kBlocks, kEach = kEachA + kEachB;
-  // Requests of a step, U its parity: pairs of slices s + 3, s + 4 in odd steps, whose stages the barrier in front has freed, and slice s + 4 in every step.
+  static_assert(NS % 4 == 0);
+  // Requests of a step, U its parity: pairs of slices s + NS - 1, s + NS in odd steps, whose stages the barrier in front has freed, and slice s + NS in every step.
   static constexpr int kLoads[2] = {kEach, kPairA + kPairB + kEach};
   // ... that may be under way at the barrier of slice s, where slice s + 1 has to be there: what was requested behind the last of it.
   static constexpr int in_flight(int u) {
+    const int both = kLoads[0] + kLoads[1];
     int most = 63;
-    if (kPairA + kPairB) {
-      const int x = kLoads[1] - kPairA - kPairB + kLoads[0] + (u == 0 ? kLoads[1] : 0);
+    if (kPairA + kPairB) {  // since step s - NS + 1, or s - NS + 2
+      const int x = kLoads[1] - kPairA - kPairB + (NS / 2 - 1) * both - (u == 0 ? 0 : kLoads[1]);
       most = x < most ? x : most;
     }
-    if (kEach) {
-      const int x = kLoads[0] + kLoads[1];
+    if (kEach) {  // since step s - NS + 1
+      const int x = (NS / 2 - 1) * both;
       most = x < most ? x : most;
     }
     return most;
   }
   static constexpr int kInFlight[2] = {in_flight(0), in_flight(1)};
   static_assert(kInFlight[1] + kLoads[1] < 64, "vmcnt is a 6-bit counter");
-  static constexpr unsigned kRegionA = STile<2, A_KC, BM, 4, 16>::kRegion, kLdsRing = kRegionA + STile<2, B_KC, BN, 4, 16>::kRegion, kLdsRows = WAVES * grouped_space<MI, NI>();
+  static constexpr unsigned kRegionA = STile<2, A_KC, BM, NS, 16>::kRegion, kLdsRing = kRegionA + STile<2, B_KC, BN, NS, 16>::kRegion, kLdsRows = WAVES * grouped_space<MI, NI>();
   static constexpr unsigned kLds = kLdsRing > kLdsRows ? kLdsRing : kLdsRows;
 
   static constexpr int first_in_slot(int q, int n, int m) { return q >= m ? n : (q * n + m - 1) / m; }
@@ -237,14 +247,14 @@ struct GroupedRing {
       };
       // What the steps before the first would have requested, in their order.
 #pragma unroll
-      for (int step = -4; step < 0; ++step) {
-        if (A_KC && (step & 1) && step + 3 >= 0) request_a((step + 3) / 2, step + 3);
-        if (B_KC && (step & 1) && step + 3 >= 0) request_b((step + 3) / 2, step + 3);
-        if (!A_KC) request_a(step + 4, step + 4);
-        if (!B_KC) request_b(step + 4, step + 4);
+      for (int step = -NS; step < 0; ++step) {
+        if (A_KC && (step & 1) && step + NS - 1 >= 0) request_a((step + NS - 1) / 2, step + NS - 1);
+        if (B_KC && (step & 1) && step + NS - 1 >= 0) request_b((step + NS - 1) / 2, step + NS - 1);
+        if (!A_KC) request_a(step + NS, step + NS);
+        if (!B_KC) request_b(step + NS, step + NS);
       }
-      la.look_ahead(4 < slices - 1 ? 4 : slices - 1);
-      lb.look_ahead(4 < slices - 1 ? 4 : slices - 1);
+      la.look_ahead(NS < slices - 1 ? NS : slices - 1);
+      lb.look_ahead(NS < slices - 1 ? NS : slices - 1);
       wait_loads_upto<kInFlight[1] + kLoads[1]>();  // slice 0
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       __builtin_amdgcn_s_barrier();
@@ -293,15 +303,15 @@ struct GroupedRing {
                         __builtin_amdgcn_sched_barrier(0);
                         if constexpr (Q == 0) {
                           const auto unit = [&](bool kc) {
-                            const unsigned x = kc ? (s + 3) / 2 : s + 4, most = (kc ? pairs : slices) - 1;
+                            const unsigned x = kc ? (s + NS - 1) / 2 : s + NS, most = (kc ? pairs : slices) - 1;
                             return x < most ? x : most;
                           };
                           unit_a = unit(A_KC), unit_b = unit(B_KC);
                           left_a = la.left_of(unit_a), left_b = lb.left_of(unit_b);
                           la.look(), lb.look();  // (in front of this step's reads: the compiler waits for both together)
                           la.look_ahead(unit_a + 1 < slices ? unit_a + 1 : unit_a), lb.look_ahead(unit_b + 1 < slices ? unit_b + 1 : unit_b);
-                          fill_a = (int)((s + (A_KC ? 3 : 4)) % 4), fill_b = (int)((s + (B_KC ? 3 : 4)) % 4);
-                          next_a = addr_a + (s + 1) % 4 * STile<2, A_KC, BM, 4, 16>::kStageStep, next_b = addr_b + (s + 1) % 4 * STile<2, B_KC, BN, 4, 16>::kStageStep;
+                          fill_a = (int)((s + (A_KC ? NS - 1 : NS)) % NS), fill_b = (int)((s + (B_KC ? NS - 1 : NS)) % NS);
+                          next_a = addr_a + (s + 1) % NS * STile<2, A_KC, BM, NS, 16>::kStageStep, next_b = addr_b + (s + 1) % NS * STile<2, B_KC, BN, NS, 16>::kStageStep;
                         }
                         [&]<int... Rs>(std::integer_sequence<int, Rs...>) __attribute__((always_inline)) {
                           (read_item(std::integral_constant<int, first_in_slot(Q, kReads, kReadSlots) + Rs>{}, std::integral_constant<int, U ^ 1>{}, next_a, next_b), ...);
@@ -341,70 +351,17 @@ struct GroupedRing {
   }
 };
 
-// Which tile of which group a workgroup takes. `whole` tiles of MOST rows come first, group after group, then one for what is left of each group; both are dealt out to the
-// eight dies in runs, so that a die's workgroups share operands. Lane l counts for groups l * each .. + each - 1.
-struct GroupedPlace {
-  unsigned e, first, rows, tile_n;  // rows first .. first + rows - 1 of A and C
-  bool none;
-};
-template <int MOST>
-__device__ __forceinline__ GroupedPlace grouped_place(const int32_t *offsets, unsigned groups, unsigned m, unsigned tiles_n, unsigned id) {
-  const unsigned lane = threadIdx.x & 63u, each = (groups + 63) / 64, g0 = lane * each;
-  unsigned whole = 0, rest = 0;
-  for (unsigned g = g0; g < g0 + each && g < groups; ++g) {
-    const unsigned rows = skl_group_range(offsets, g, m).rows;
-    whole += rows / MOST, rest += rows % MOST != 0;
-  }
-  const unsigned whole_upto = skl_wave_scan(whole), rest_upto = skl_wave_scan(rest);
-  const unsigned all_whole = (unsigned)__builtin_amdgcn_readlane((int)whole_upto, 63) * tiles_n, all_rest = (unsigned)__builtin_amdgcn_readlane((int)rest_upto, 63) * tiles_n;
-  // This die's share of both, one after the other.
-  const unsigned die = id % 8, slot = id / 8;
-  const unsigned whole_first = all_whole / 8 * die + (die < all_whole % 8 ? die : all_whole % 8), whole_mine = all_whole / 8 + (die < all_whole % 8);
-  const unsigned rest_first = all_rest / 8 * die + (die < all_rest % 8 ? die : all_rest % 8), rest_mine = all_rest / 8 + (die < all_rest % 8);
-  GroupedPlace at{0, 0, 0, 0, slot >= whole_mine + rest_mine};
-  if (at.none) return at;
-  const bool is_whole = slot < whole_mine;
-  const unsigned t = is_whole ? whole_first + slot : rest_first + slot - whole_mine, line = t / tiles_n;  // line: row of tiles
-  const unsigned upto = is_whole ? whole_upto : rest_upto, mine = is_whole ? whole : rest;
-  const int owner = (int)__builtin_ctzll(__ballot(line < upto));
-  unsigned before = (unsigned)__builtin_amdgcn_readlane((int)(upto - mine), owner);  // lines of the groups ahead
-  unsigned e = (unsigned)owner * each;
-  SklRange r;
-  unsigned lines;
-  for (;; ++e) {
-    r = skl_group_range(offsets, e, m);
-    lines = is_whole ? r.rows / MOST : r.rows % MOST != 0;
-    if (line < before + lines) break;
-    before += lines;
-  }
-  at.e = e;
-  if (is_whole) {  // up to eight lines of a group column by column
-    const unsigned in = t - before * tiles_n, block = in / (8 * tiles_n), in_block = in - block * (8 * tiles_n), deep = lines - 8 * block < 8 ? lines - 8 * block : 8;
-    at.tile_n = in_block / deep;
-    at.first = r.first + (8 * block + in_block % deep) * MOST;
-    at.rows = MOST;
-  } else {
-    at.tile_n = t % tiles_n;
-    at.first = r.first + r.rows / MOST * MOST;
-    at.rows = r.rows % MOST;
-  }
-  // uniform, and the compiler is told: branches and descriptors go by them
-  at.e = (unsigned)__builtin_amdgcn_readfirstlane((int)at.e), at.first = (unsigned)__builtin_amdgcn_readfirstlane((int)at.first);
-  at.rows = (unsigned)__builtin_amdgcn_readfirstlane((int)at.rows), at.tile_n = (unsigned)__builtin_amdgcn_readfirstlane((int)at.tile_n);
-  return at;
-}
-
-template <int DT, bool B_KC, int MOST, int BN, int WAVES>
+template <int DT, bool B_KC, int MOST, int BN, int WAVES, int NS>
 struct GroupedRows {
-  using Full = GroupedRing<DT, true, B_KC, MOST, BN, WAVES, MOST == 64 ? WAVES : MOST == 128 ? WAVES / 2 : 2>;
-  using Half = GroupedRing<DT, true, B_KC, 128, BN, WAVES, WAVES / 2>;
-  using Quarter = GroupedRing<DT, true, B_KC, 64, BN, WAVES, WAVES>;
+  using Full = GroupedRing<DT, true, B_KC, MOST, BN, WAVES, MOST == 64 ? (BN / 16 < WAVES ? BN / 16 : WAVES) : 2, NS>;
+  using Half = GroupedRing<DT, true, B_KC, 128, BN, WAVES, WAVES / 2, NS>;
+  using Quarter = GroupedRing<DT, true, B_KC, 64, BN, WAVES, WAVES, NS>;
   static constexpr unsigned kLds = Full::kLds;
 };
 
-template <int DT, bool B_KC, int MOST, int BN, int WAVES>
+template <int DT, bool B_KC, int MOST, int BN, int WAVES, int NS>
 __global__ void __launch_bounds__(WAVES * 64) gemm_grouped_rows_kernel(GroupedRingArgs p) {
-  using Rows = GroupedRows<DT, B_KC, MOST, BN, WAVES>;
+  using Rows = GroupedRows<DT, B_KC, MOST, BN, WAVES, NS>;
   extern __shared__ __attribute__((aligned(128))) char grouped_smem[];
   const GroupedPlace at = grouped_place<MOST>(p.offsets, p.groups, p.m, p.tiles_n, blockIdx.x);
   if (at.none) return;
@@ -437,7 +394,7 @@ __device__ __forceinline__ unsigned grouped_by_length(const int32_t *offsets, un
 // Sums over the groups' rows: both operands across K, tiles of BM x BN of each group's C.
 template <int DT, int BM, int BN, int WAVES, int WAVES_N, bool A_INDEXED, bool B_INDEXED>
 __global__ void __launch_bounds__(WAVES * 64) gemm_grouped_over_kernel(GroupedRingArgs p) {
-  using Ring = GroupedRing<DT, false, false, BM, BN, WAVES, WAVES_N, A_INDEXED, B_INDEXED>;
+  using Ring = GroupedRing<DT, false, false, BM, BN, WAVES, WAVES_N, 4, A_INDEXED, B_INDEXED>;
   extern __shared__ __attribute__((aligned(128))) char grouped_smem[];
   // Each die takes a run of every group's tiles - a group's length decides how long they take -, the longest group first, walked in blocks of eight rows of tiles, column by column.
   const unsigned tiles = p.tiles_m * p.tiles_n, run = (tiles + 7) / 8, die = blockIdx.x % 8, slot = blockIdx.x / 8;
@@ -466,7 +423,7 @@ int launch_ring(K kernel, std::atomic<int> &allowed, unsigned lds, unsigned thre
   return skl_check_launch("gemm_grouped");
 }
 constexpr size_t kMostRingBlocks = size_t(1) << 22;
-template <int DT, bool B_KC, int MOST, int BN, int WAVES>
+template <int DT, bool B_KC, int MOST, int BN, int WAVES, int NS>
 int grouped_rows(const skl_grouped_gemm &g, GroupedRingArgs p) {
   const size_t lines = g.m / MOST + (g.m < g.groups ? g.m : g.groups);  // of tiles: whole ones, and one more for each group that has a row
   const size_t most = kMostRingBlocks / (lines + 16) > 0 ? kMostRingBlocks / (lines + 16) : 1, slab = most * BN;
@@ -476,15 +433,20 @@ int grouped_rows(const skl_grouped_gemm &g, GroupedRingArgs p) {
     p.tiles_n = skl_div_up(p.n, BN);
     p.b = (const char *)g.b + col * g.csb * 2;
     p.c = (char *)g.c + col * (g.c_single ? 4 : 2);
-    const int rc = launch_ring(gemm_grouped_rows_kernel<DT, B_KC, MOST, BN, WAVES>, allowed, GroupedRows<DT, B_KC, MOST, BN, WAVES>::kLds, WAVES * 64, p, (lines * p.tiles_n / 8 + 2) * 8);
+    const int rc = launch_ring(gemm_grouped_rows_kernel<DT, B_KC, MOST, BN, WAVES, NS>, allowed, GroupedRows<DT, B_KC, MOST, BN, WAVES, NS>::kLds, WAVES * 64, p, (lines * p.tiles_n / 8 + 2) * 8);
     if (rc != 0) return rc;
   }
   return 0;
 }
 template <int DT, bool B_KC>
 int grouped_rows_by_size(const skl_grouped_gemm &g, const GroupedRingArgs &p) {
-  if (g.m <= 64 * g.groups) return grouped_rows<DT, B_KC, 64, 128, 4>(g, p);
-  return grouped_rows<DT, B_KC, 256, 256, 8>(g, p);
+  // By how many rows a group has on average and how many tiles there are: the largest tile that is mostly filled and fills the chip. us, 256 x 256 / 128 x 128 / 64 x 64: 32 groups of
+  // 2816 x 2048 with 256, 512, 1024 and 3000 tokens to four of them -, 84, 78; 92, 85, 93; 107, 116, 140; 167, 200, 315; two groups of 1024 x 1024 with 2000 rows 27, 15, 13. One token to four of
+  // 32 groups: 64 x 64 with eight slices of k in the ring 12.5, 64 x 128 with four 28.
+  const size_t groups = g.m < g.groups ? g.m : g.groups, lines = g.m / 256 + groups / 2, lines_half = g.m / 128 + groups / 2;  // half of the last tiles of the groups are small ones
+  if (g.m >= 112 * groups && lines * skl_div_up(g.n, 256) >= 160) return grouped_rows<DT, B_KC, 256, 256, 8, 4>(g, p);
+  if (g.m >= 56 * groups && lines_half * skl_div_up(g.n, 128) >= 160) return grouped_rows<DT, B_KC, 128, 128, 8, 4>(g, p);
+  return grouped_rows<DT, B_KC, 64, 64, 4, 8>(g, p);
 }
 template <int DT>
 int grouped_ring(const skl_grouped_gemm &g) {
@@ -511,7 +473,7 @@ int grouped_over(const skl_groupedk_gemm &g, GroupedRingArgs p) {
       p.tiles_n = skl_div_up(p.n, BN);
       p.b = (const char *)g.b + col * 2;
       p.c = (char *)g.c + (e * g.gsc + col) * (g.c_single ? 4 : 2);
-      const int rc = launch_ring(gemm_grouped_over_kernel<DT, BM, BN, WAVES, WAVES_N, A_INDEXED, B_INDEXED>, allowed, GroupedRing<DT, false, false, BM, BN, WAVES, WAVES_N>::kLds, WAVES * 64, p,
+      const int rc = launch_ring(gemm_grouped_over_kernel<DT, BM, BN, WAVES, WAVES_N, A_INDEXED, B_INDEXED>, allowed, GroupedRing<DT, false, false, BM, BN, WAVES, WAVES_N, 4>::kLds, WAVES * 64, p,
                                  (size_t)p.groups * (((size_t)p.tiles_m * p.tiles_n + 7) / 8) * 8);
       if (rc != 0) return rc;
     }

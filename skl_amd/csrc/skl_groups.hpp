@@ -48,6 +48,59 @@ __device__ __forceinline__ SklRange skl_group_range(const int32_t *offsets, unsi
   return {b, f > b ? f - b : 0u};
 }
 
+// Which tile of which group a workgroup takes. `whole` tiles of MOST rows come first, group after group, then one for what is left of each group; both are dealt out to the
+// eight dies in runs, so that a die's workgroups share operands. Lane l counts for groups l * each .. + each - 1.
+struct GroupedPlace {
+  unsigned e, first, rows, tile_n;  // rows first .. first + rows - 1 of A and C
+  bool none;
+};
+template <int MOST>
+__device__ __forceinline__ GroupedPlace grouped_place(const int32_t *offsets, unsigned groups, unsigned m, unsigned tiles_n, unsigned id) {
+  const unsigned lane = threadIdx.x & 63u, each = (groups + 63) / 64, g0 = lane * each;
+  unsigned whole = 0, rest = 0;
+  for (unsigned g = g0; g < g0 + each && g < groups; ++g) {
+    const unsigned rows = skl_group_range(offsets, g, m).rows;
+    whole += rows / MOST, rest += rows % MOST != 0;
+  }
+  const unsigned whole_upto = skl_wave_scan(whole), rest_upto = skl_wave_scan(rest);
+  const unsigned all_whole = (unsigned)__builtin_amdgcn_readlane((int)whole_upto, 63) * tiles_n, all_rest = (unsigned)__builtin_amdgcn_readlane((int)rest_upto, 63) * tiles_n;
+  // This die's share of both, one after the other.
+  const unsigned die = id % 8, slot = id / 8;
+  const unsigned whole_first = all_whole / 8 * die + (die < all_whole % 8 ? die : all_whole % 8), whole_mine = all_whole / 8 + (die < all_whole % 8);
+  const unsigned rest_first = all_rest / 8 * die + (die < all_rest % 8 ? die : all_rest % 8), rest_mine = all_rest / 8 + (die < all_rest % 8);
+  GroupedPlace at{0, 0, 0, 0, slot >= whole_mine + rest_mine};
+  if (at.none) return at;
+  const bool is_whole = slot < whole_mine;
+  const unsigned t = is_whole ? whole_first + slot : rest_first + slot - whole_mine, line = t / tiles_n;  // line: row of tiles
+  const unsigned upto = is_whole ? whole_upto : rest_upto, mine = is_whole ? whole : rest;
+  const int owner = (int)__builtin_ctzll(__ballot(line < upto));
+  unsigned before = (unsigned)__builtin_amdgcn_readlane((int)(upto - mine), owner);  // lines of the groups ahead
+  unsigned e = (unsigned)owner * each;
+  SklRange r;
+  unsigned lines;
+  for (;; ++e) {
+    r = skl_group_range(offsets, e, m);
+    lines = is_whole ? r.rows / MOST : r.rows % MOST != 0;
+    if (line < before + lines) break;
+    before += lines;
+  }
+  at.e = e;
+  if (is_whole) {  // up to eight lines of a group column by column
+    const unsigned in = t - before * tiles_n, block = in / (8 * tiles_n), in_block = in - block * (8 * tiles_n), deep = lines - 8 * block < 8 ? lines - 8 * block : 8;
+    at.tile_n = in_block / deep;
+    at.first = r.first + (8 * block + in_block % deep) * MOST;
+    at.rows = MOST;
+  } else {
+    at.tile_n = t % tiles_n;
+    at.first = r.first + r.rows / MOST * MOST;
+    at.rows = r.rows % MOST;
+  }
+  // uniform, and the compiler is told: branches and descriptors go by them
+  at.e = (unsigned)__builtin_amdgcn_readfirstlane((int)at.e), at.first = (unsigned)__builtin_amdgcn_readfirstlane((int)at.first);
+  at.rows = (unsigned)__builtin_amdgcn_readfirstlane((int)at.rows), at.tile_n = (unsigned)__builtin_amdgcn_readfirstlane((int)at.tile_n);
+  return at;
+}
+
 __device__ __forceinline__ float skl_widen(uint16_t v, bool bf16) { return bf16 ? __uint_as_float((unsigned)v << 16) : (float)__builtin_bit_cast(_Float16, v); }
 
 // The result for one element of C: TC is float, __bf16 or _Float16; a 16-bit C is widened, combined in fp32 and rounded once, to the nearest.
