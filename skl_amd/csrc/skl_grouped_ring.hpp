@@ -49,7 +49,7 @@ struct GroupedLoader {
   unsigned off[kBlocks], k_lane[KC ? 2 : kBlocks], k_total, lds;
   const __attribute__((address_space(4))) char *index;  // this wave's first row's; read by scalar loads
   unsigned index_left, index_limit, index_pitch;        // index_left: rows from there on less one
-  typedef int Lines __attribute__((ext_vector_type(kRows < 2 ? 2 : kRows)));
+  typedef int Lines __attribute__((ext_vector_type(INDEXED ? kRows : 2)));
   Lines ahead, line;  // rows of the next step's unit; offsets of this step's (vectors: arrays in here are kept in memory)
 
   __device__ __forceinline__ static const char *scalar(const char *p) {
@@ -96,19 +96,21 @@ struct GroupedLoader {
     }
   }
   // The rows of the part of `unit` that is this wave's; beyond the last one that one again.
-  __device__ __forceinline__ void look_ahead(unsigned unit) {
+  __device__ __forceinline__ Lines look_up(unsigned unit) const {
+    Lines rows = 0;
     if constexpr (INDEXED) {
 #pragma unroll
       for (int r = 0; r < kRows; ++r) {
         const unsigned at = unit * kUnitK + r;
-        ahead[r] = *(const __attribute__((address_space(4))) int32_t *)(index + (at < index_left ? at : index_left) * 4u);
+        rows[r] = *(const __attribute__((address_space(4))) int32_t *)(index + (at < index_left ? at : index_left) * 4u);
       }
     }
+    return rows;
   }
-  __device__ __forceinline__ void look() {
+  __device__ __forceinline__ void take(Lines rows) {  // for the requests of a step
     if constexpr (INDEXED) {
 #pragma unroll
-      for (int r = 0; r < kRows; ++r) line[r] = (int)((unsigned)ahead[r] < index_limit ? (unsigned)ahead[r] * index_pitch : kOutside);
+      for (int r = 0; r < kRows; ++r) line[r] = (int)((unsigned)rows[r] < index_limit ? (unsigned)rows[r] * index_pitch : kOutside);
     }
   }
   __device__ __forceinline__ unsigned left_of(unsigned unit) const { return k_total > unit * kUnitK ? k_total - unit * kUnitK : 0; }
@@ -231,21 +233,31 @@ struct GroupedRing {
       for (int j = 0; j < NI; ++j) acc[i][j] = v4f{0, 0, 0, 0};
     const unsigned slices = (t.k * 2 + 2 * kRingSlice - 1) / (2 * kRingSlice) * 2, pairs = slices / 2;
     if (slices != 0) {
+      const auto unit_of = [&](bool kc, unsigned unit) {
+        const unsigned most = (kc ? pairs : slices) - 1;
+        return unit < most ? unit : most;
+      };
+      // What the steps before the first would have requested, in their order (the rows of all of it looked up ahead).
+      typename LA::Lines rows_a[A_INDEXED ? NS : 1];
+      typename LB::Lines rows_b[B_INDEXED ? NS : 1];
+      if constexpr (A_INDEXED)
+#pragma unroll
+        for (int u = 0; u < NS; ++u) rows_a[u] = la.look_up(unit_of(false, u));
+      if constexpr (B_INDEXED)
+#pragma unroll
+        for (int u = 0; u < NS; ++u) rows_b[u] = lb.look_up(unit_of(false, u));
       const auto request_a = [&](unsigned unit, unsigned stage) __attribute__((always_inline)) {
-        const unsigned most = (A_KC ? pairs : slices) - 1, u = unit < most ? unit : most;
-        la.look_ahead(u);
-        la.look();
+        const unsigned u = unit_of(A_KC, unit);
+        if constexpr (A_INDEXED) la.take(rows_a[stage]);
 #pragma unroll
         for (int i = 0; i < LA::kBlocks; ++i) la.request(region_a, (int)stage, u, la.left_of(u), i);
       };
       const auto request_b = [&](unsigned unit, unsigned stage) __attribute__((always_inline)) {
-        const unsigned most = (B_KC ? pairs : slices) - 1, u = unit < most ? unit : most;
-        lb.look_ahead(u);
-        lb.look();
+        const unsigned u = unit_of(B_KC, unit);
+        if constexpr (B_INDEXED) lb.take(rows_b[stage]);
 #pragma unroll
         for (int i = 0; i < LB::kBlocks; ++i) lb.request(region_b, (int)stage, u, lb.left_of(u), i);
       };
-      // What the steps before the first would have requested, in their order.
 #pragma unroll
       for (int step = -NS; step < 0; ++step) {
         if (A_KC && (step & 1) && step + NS - 1 >= 0) request_a((step + NS - 1) / 2, step + NS - 1);
@@ -253,8 +265,7 @@ struct GroupedRing {
         if (!A_KC) request_a(step + NS, step + NS);
         if (!B_KC) request_b(step + NS, step + NS);
       }
-      la.look_ahead(NS < slices - 1 ? NS : slices - 1);
-      lb.look_ahead(NS < slices - 1 ? NS : slices - 1);
+      la.ahead = la.look_up(unit_of(false, NS)), lb.ahead = lb.look_up(unit_of(false, NS));
       wait_loads_upto<kInFlight[1] + kLoads[1]>();  // slice 0
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       __builtin_amdgcn_s_barrier();
@@ -308,8 +319,8 @@ struct GroupedRing {
                           };
                           unit_a = unit(A_KC), unit_b = unit(B_KC);
                           left_a = la.left_of(unit_a), left_b = lb.left_of(unit_b);
-                          la.look(), lb.look();  // (in front of this step's reads: the compiler waits for both together)
-                          la.look_ahead(unit_a + 1 < slices ? unit_a + 1 : unit_a), lb.look_ahead(unit_b + 1 < slices ? unit_b + 1 : unit_b);
+                          la.take(la.ahead), lb.take(lb.ahead);  // (in front of this step's reads: the compiler waits for both together)
+                          la.ahead = la.look_up(unit_a + 1 < slices ? unit_a + 1 : unit_a), lb.ahead = lb.look_up(unit_b + 1 < slices ? unit_b + 1 : unit_b);
                           fill_a = (int)((s + (A_KC ? NS - 1 : NS)) % NS), fill_b = (int)((s + (B_KC ? NS - 1 : NS)) % NS);
                           next_a = addr_a + (s + 1) % NS * STile<2, A_KC, BM, NS, 16>::kStageStep, next_b = addr_b + (s + 1) % NS * STile<2, B_KC, BN, NS, 16>::kStageStep;
                         }
@@ -379,16 +390,29 @@ __global__ void __launch_bounds__(WAVES * 64) gemm_grouped_rows_kernel(GroupedRi
   }
 }
 
-// The group that comes at place `place` by its length, longest first (up to 64 groups; more as they lie, which evens out by itself).
-__device__ __forceinline__ unsigned grouped_by_length(const int32_t *offsets, unsigned groups, unsigned most, unsigned place) {
-  if (groups > 64 || groups == 1) return place;
-  const unsigned lane = threadIdx.x & 63u, mine = lane < groups ? skl_group_range(offsets, lane, most).rows : 0u;
+// The group that comes at place `place`, the longest one first, and its rows. Finding out among 64 groups takes 1 us, so that short ones are taken as they lie unless there are few.
+struct GroupedTurn {
+  unsigned e;
+  SklRange rows;
+};
+template <unsigned MOST>
+__device__ __forceinline__ GroupedTurn grouped_longest_first(const int32_t *offsets, unsigned groups, unsigned most, unsigned place) {
+  const unsigned lane = threadIdx.x & 63u;
+  const SklRange mine = lane < groups ? skl_group_range(offsets, lane, most) : SklRange{0, 0};
   unsigned ahead = 0;
-  for (unsigned g = 0; g < groups; ++g) {
-    const unsigned other = (unsigned)__builtin_amdgcn_readlane((int)mine, (int)g);
-    ahead += other > mine || (other == mine && g < lane);
+#pragma unroll
+  for (unsigned g = 0; g < MOST; ++g) {  // (lanes beyond the groups hold none and come last)
+    const unsigned other = (unsigned)__builtin_amdgcn_readlane((int)mine.rows, (int)g);
+    ahead += other > mine.rows || (other == mine.rows && g < lane);
   }
-  return (unsigned)__builtin_ctzll(__ballot(lane < groups && ahead == place));
+  const int owner = (int)__builtin_ctzll(__ballot(lane < groups && ahead == place));
+  return {(unsigned)owner, {(unsigned)__builtin_amdgcn_readlane((int)mine.first, owner), (unsigned)__builtin_amdgcn_readlane((int)mine.rows, owner)}};
+}
+__device__ __forceinline__ GroupedTurn grouped_by_length(const int32_t *offsets, unsigned groups, unsigned most, unsigned place) {
+  if (groups > 1 && groups <= 16) return grouped_longest_first<16>(offsets, groups, most, place);
+  if (groups > 1 && groups <= 64 && most >= 512 * groups) return grouped_longest_first<64>(offsets, groups, most, place);
+  SklRange r = skl_group_range(offsets, place, most);
+  return {place, {(unsigned)__builtin_amdgcn_readfirstlane((int)r.first), (unsigned)__builtin_amdgcn_readfirstlane((int)r.rows)}};
 }
 
 // Sums over the groups' rows: both operands across K, tiles of BM x BN of each group's C.
@@ -398,12 +422,13 @@ __global__ void __launch_bounds__(WAVES * 64) gemm_grouped_over_kernel(GroupedRi
   extern __shared__ __attribute__((aligned(128))) char grouped_smem[];
   // Each die takes a run of every group's tiles - a group's length decides how long they take -, the longest group first, walked in blocks of eight rows of tiles, column by column.
   const unsigned tiles = p.tiles_m * p.tiles_n, run = (tiles + 7) / 8, die = blockIdx.x % 8, slot = blockIdx.x / 8;
-  const unsigned in = die * run + slot % run, e = grouped_by_length(p.offsets, p.groups, p.k, slot / run);
+  const unsigned in = die * run + slot % run;
   if (in >= tiles) return;
+  const GroupedTurn turn = grouped_by_length(p.offsets, p.groups, p.k, slot / run);
+  const unsigned e = turn.e;
+  const SklRange r = turn.rows;
   const unsigned block = in / (8 * p.tiles_n), in_block = in - block * (8 * p.tiles_n), deep = p.tiles_m - 8 * block < 8 ? p.tiles_m - 8 * block : 8;
   const unsigned row0 = (8 * block + in_block % deep) * BM, col0 = in_block / deep * BN;
-  SklRange r = skl_group_range(p.offsets, e, p.k);
-  r.first = (unsigned)__builtin_amdgcn_readfirstlane((int)r.first), r.rows = (unsigned)__builtin_amdgcn_readfirstlane((int)r.rows);
   GroupedTile t;
   t.index = p.rows, t.index_b = p.rows_b, t.index_at = r.first, t.limit = p.a_rows, t.limit_b = p.b_rows;
   t.a = A_INDEXED ? p.a : p.a + (size_t)r.first * p.a_pitch, t.a_first = row0, t.a_count = p.m - row0;
@@ -480,6 +505,11 @@ int grouped_over(const skl_groupedk_gemm &g, GroupedRingArgs p) {
   }
   return 0;
 }
+template <int DT, int BM, int BN, int WAVES, int WAVES_N>
+int grouped_over_indexed(const skl_groupedk_gemm &g, const GroupedRingArgs &p) {
+  if (g.rows_a) return g.rows_b ? grouped_over<DT, BM, BN, WAVES, WAVES_N, true, true>(g, p) : grouped_over<DT, BM, BN, WAVES, WAVES_N, true, false>(g, p);
+  return g.rows_b ? grouped_over<DT, BM, BN, WAVES, WAVES_N, false, true>(g, p) : grouped_over<DT, BM, BN, WAVES, WAVES_N, false, false>(g, p);
+}
 template <int DT>
 int grouped_over_ring(const skl_groupedk_gemm &g) {
   GroupedRingArgs p{};
@@ -487,8 +517,8 @@ int grouped_over_ring(const skl_groupedk_gemm &g) {
   p.rows = g.rows_a, p.rows_b = g.rows_b, p.a_rows = (unsigned)g.a_rows, p.b_rows = (unsigned)g.b_rows;
   p.rsc = g.rsc, p.gsc = g.gsc, p.m = (unsigned)g.m, p.k = (unsigned)g.total;
   p.c_single = g.c_single, p.alpha = g.alpha, p.beta = g.beta;
-  if (g.rows_a) return g.rows_b ? grouped_over<DT, 256, 256, 8, 2, true, true>(g, p) : grouped_over<DT, 256, 256, 8, 2, true, false>(g, p);
-  return g.rows_b ? grouped_over<DT, 256, 256, 8, 2, false, true>(g, p) : grouped_over<DT, 256, 256, 8, 2, false, false>(g, p);
+  // (Smaller tiles with two workgroups to a compute unit are slower at every length, short ones among them: us, 256 x 256 / 128 x 128, 64 groups of 2048 x 1408 with 96 rows on average 165 / 217.)
+  return grouped_over_indexed<DT, 256, 256, 8, 2>(g, p);
 }
 
 }  // namespace

@@ -58,9 +58,10 @@ template <int MOST>
 __device__ __forceinline__ GroupedPlace grouped_place(const int32_t *offsets, unsigned groups, unsigned m, unsigned tiles_n, unsigned id) {
   const unsigned lane = threadIdx.x & 63u, each = (groups + 63) / 64, g0 = lane * each;
   unsigned whole = 0, rest = 0;
+  SklRange mine_last{0, 0};  // with one group to a lane, the lane's
   for (unsigned g = g0; g < g0 + each && g < groups; ++g) {
-    const unsigned rows = skl_group_range(offsets, g, m).rows;
-    whole += rows / MOST, rest += rows % MOST != 0;
+    mine_last = skl_group_range(offsets, g, m);
+    whole += mine_last.rows / MOST, rest += mine_last.rows % MOST != 0;
   }
   const unsigned whole_upto = skl_wave_scan(whole), rest_upto = skl_wave_scan(rest);
   const unsigned all_whole = (unsigned)__builtin_amdgcn_readlane((int)whole_upto, 63) * tiles_n, all_rest = (unsigned)__builtin_amdgcn_readlane((int)rest_upto, 63) * tiles_n;
@@ -78,11 +79,16 @@ __device__ __forceinline__ GroupedPlace grouped_place(const int32_t *offsets, un
   unsigned e = (unsigned)owner * each;
   SklRange r;
   unsigned lines;
-  for (;; ++e) {
-    r = skl_group_range(offsets, e, m);
+  if (each == 1) {  // (what the lane holds: no second trip to memory)
+    r = {(unsigned)__builtin_amdgcn_readlane((int)mine_last.first, owner), (unsigned)__builtin_amdgcn_readlane((int)mine_last.rows, owner)};
     lines = is_whole ? r.rows / MOST : r.rows % MOST != 0;
-    if (line < before + lines) break;
-    before += lines;
+  } else {
+    for (;; ++e) {
+      r = skl_group_range(offsets, e, m);
+      lines = is_whole ? r.rows / MOST : r.rows % MOST != 0;
+      if (line < before + lines) break;
+      before += lines;
+    }
   }
   at.e = e;
   if (is_whole) {  // up to eight lines of a group column by column
