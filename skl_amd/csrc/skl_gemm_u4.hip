@@ -169,6 +169,7 @@ struct U4Shape {
   static constexpr unsigned kEntries = kChunk / kUnit * PER, kEach = (kCols * kEntries + kThreads - 1) / kThreads;  // scales of a column and chunk, of a thread
   static constexpr unsigned kBytesA = ROWS * kPitch, kStage = (kBytesA + (kEntries + 1) * kCols * 4 + 15) / 16 * 16;
   static constexpr unsigned kSums = kWaves * 16 * kR * (kCols + 1) * 4, kLds = 2 * kStage > kSums ? 2 * kStage : kSums;
+  static_assert(kLds <= 160 * 1024);
   struct Side {  // what goes to LDS, on its way
     v4i a[kPieces];
     unsigned scale[kEach], zero[ZEROS ? kEach : 1];
@@ -384,8 +385,8 @@ int skl_hip_launch_gemm_u4(const skl_grouped_u4 *u) {
   U4Args p{};
   p.a = (const uint16_t *)g->a, p.rsa = g->rsa, p.offsets = g->offsets, p.rows = g->rows;
   p.groups = (unsigned)g->groups, p.m = (unsigned)g->m, p.n = (unsigned)g->n, p.k = (unsigned)g->k, p.a_rows = (unsigned)g->a_rows, p.group_k = (unsigned)u->group_k;
-  p.codes = u->codes, p.ld = u->ld, p.expert = u->expert;
-  p.scales = (const uint16_t *)u->scales, p.zeros = u->zeros, p.ld_scales = u->ld_scales, p.expert_scales = u->expert_scales;
+  p.codes = u->codes, p.ld = u->ld, p.expert = g->groups > 1 ? u->expert : 0;
+  p.scales = (const uint16_t *)u->scales, p.zeros = u->zeros, p.ld_scales = u->ld_scales, p.expert_scales = g->groups > 1 ? u->expert_scales : 0;
   p.c = g->c, p.rsc = g->rsc, p.alpha = g->alpha, p.beta = g->beta;
   // Columns of a launch: beyond 2^32 threads the runtime takes what is left of the number in 32 bits.
   const size_t slab = size_t(1) << 26;

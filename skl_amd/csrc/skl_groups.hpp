@@ -74,7 +74,10 @@ __device__ __forceinline__ GroupedPlace grouped_place(const int32_t *offsets, un
   const bool is_whole = slot < whole_mine;
   const unsigned t = is_whole ? whole_first + slot : rest_first + slot - whole_mine, line = t / tiles_n;  // line: row of tiles
   const unsigned upto = is_whole ? whole_upto : rest_upto, mine = is_whole ? whole : rest;
-  const int owner = (int)__builtin_ctzll(__ballot(line < upto));
+  const unsigned long long behind = __ballot(line < upto);
+  at.none = behind == 0;  // (sums beyond 32 bits, of offsets that fall back)
+  if (at.none) return at;
+  const int owner = (int)__builtin_ctzll(behind);
   unsigned before = (unsigned)__builtin_amdgcn_readlane((int)(upto - mine), owner);  // lines of the groups ahead
   unsigned e = (unsigned)owner * each;
   SklRange r;
@@ -86,7 +89,7 @@ __device__ __forceinline__ GroupedPlace grouped_place(const int32_t *offsets, un
     for (;; ++e) {
       r = skl_group_range(offsets, e, m);
       lines = is_whole ? r.rows / MOST : r.rows % MOST != 0;
-      if (line < before + lines) break;
+      if (line < before + lines || e + 1 >= groups) break;
       before += lines;
     }
   }
