@@ -219,7 +219,7 @@ SKL_GROUPEDK(skl_gemm_groupedk_f16c_f16_f16_gfx950, SKL_DT_F16, skl_f16_t, 0, sk
 static int u4_ok(const skl_gfx950_u4_t *b, size_t groups, size_t n, size_t k) {
   size_t blocks;
   if (!b || b->group_k == 0 || (b->group_k % 32 != 0 && b->group_k < k) || !b->codes || !b->scales) return 0;
-  blocks = (k + b->group_k - 1) / b->group_k;
+  blocks = k / b->group_k + (k % b->group_k != 0);
   if (n > 1 && (b->ld % 2 != 0 || b->ld < k || b->ld_scales < blocks)) return 0;
   return groups <= 1 || b->expert % 2 == 0;
 }

@@ -233,12 +233,9 @@ __global__ void __launch_bounds__(256, 2) gemm_grouped_kernel(GroupedArgs p) {
 template <int DT, typename TC, bool OVER, int AMODE, int BMODE>
 int launch(const GroupedArgs &p, size_t blocks) {
   constexpr int kLds = 2 * (Operand<AMODE>::T::kBytes + Operand<BMODE>::T::kBytes);
-  static std::atomic<int> allowed{0};
-  if (!allowed.load(std::memory_order_relaxed)) {
-    const int rc = skl_check_hip(hipFuncSetAttribute(reinterpret_cast<const void *>(&gemm_grouped_kernel<DT, TC, OVER, AMODE, BMODE>), hipFuncAttributeMaxDynamicSharedMemorySize, kLds), "gemm_grouped: LDS size");
-    if (rc != 0) return rc;
-    allowed.store(1, std::memory_order_relaxed);
-  }
+  static std::atomic<unsigned long long> allowed{0};
+  const int rc = skl_allow_lds(reinterpret_cast<const void *>(&gemm_grouped_kernel<DT, TC, OVER, AMODE, BMODE>), kLds, allowed);
+  if (rc != 0) return rc;
   gemm_grouped_kernel<DT, TC, OVER, AMODE, BMODE><<<dim3((unsigned)blocks), dim3(256), kLds, skl_current_stream()>>>(p);
   return skl_check_launch("gemm_grouped");
 }

@@ -338,12 +338,9 @@ template <typename T, int PER, bool ZEROS, int F, int ROWS, int UNITS, int MIN>
 int launch_stream(const U4Args &p, int c_single) {
   constexpr unsigned kLds = U4Shape<PER, ZEROS, F, ROWS, UNITS>::kLds;
   const auto kernel = gemm_u4_stream_kernel<T, PER, ZEROS, F, ROWS, UNITS, MIN>;
-  static std::atomic<int> allowed{0};
-  if (!allowed.load(std::memory_order_relaxed)) {
-    const int rc = skl_check_hip(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kLds), "gemm_u4: LDS size");
-    if (rc != 0) return rc;
-    allowed.store(1, std::memory_order_relaxed);
-  }
+  static std::atomic<unsigned long long> allowed{0};
+  const int rc = skl_allow_lds(reinterpret_cast<const void *>(kernel), kLds, allowed);
+  if (rc != 0) return rc;
   kernel<<<dim3(skl_div_up(p.n, 16 * F), p.groups), dim3(kThreads), kLds, skl_current_stream()>>>(p, c_single);
   return skl_check_launch("gemm_u4");
 }

@@ -150,11 +150,8 @@ int skl_hip_launch_group_rows(size_t count, const int32_t *ids, size_t per_row, 
     group_count_kernel<<<dim3((unsigned)blocks), dim3(waves * 64), groups * 4, skl_current_stream()>>>(p);
     rc = skl_check_launch("group_rows: counts");
   }
-  static std::atomic<int> allowed{0};
-  if (rc == 0 && !allowed.load(std::memory_order_relaxed)) {
-    rc = skl_check_hip(hipFuncSetAttribute(reinterpret_cast<const void *>(&group_rows_kernel), hipFuncAttributeMaxDynamicSharedMemorySize, 18 * 2048 * 4), "group_rows: LDS size");
-    if (rc == 0) allowed.store(1, std::memory_order_relaxed);
-  }
+  static std::atomic<unsigned long long> allowed{0};
+  if (rc == 0) rc = skl_allow_lds(reinterpret_cast<const void *>(&group_rows_kernel), 18 * 2048 * 4, allowed);
   if (rc == 0) {
     group_rows_kernel<<<dim3((unsigned)blocks), dim3(waves * 64), lds, skl_current_stream()>>>(p);
     rc = skl_check_launch("group_rows");

@@ -438,12 +438,9 @@ __global__ void __launch_bounds__(WAVES * 64) gemm_grouped_over_kernel(GroupedRi
 }
 
 template <typename K>
-int launch_ring(K kernel, std::atomic<int> &allowed, unsigned lds, unsigned threads, const GroupedRingArgs &p, size_t blocks) {
-  if (!allowed.load(std::memory_order_relaxed)) {
-    const int rc = skl_check_hip(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds), "gemm_grouped: LDS size");
-    if (rc != 0) return rc;
-    allowed.store(1, std::memory_order_relaxed);
-  }
+int launch_ring(K kernel, std::atomic<unsigned long long> &allowed, unsigned lds, unsigned threads, const GroupedRingArgs &p, size_t blocks) {
+  const int rc = skl_allow_lds(reinterpret_cast<const void *>(kernel), lds, allowed);
+  if (rc != 0) return rc;
   kernel<<<dim3((unsigned)blocks), dim3(threads), lds, skl_current_stream()>>>(p);
   return skl_check_launch("gemm_grouped");
 }
@@ -452,7 +449,7 @@ template <int DT, bool B_KC, int MOST, int BN, int WAVES, int NS>
 int grouped_rows(const skl_grouped_gemm &g, GroupedRingArgs p) {
   const size_t lines = g.m / MOST + (g.m < g.groups ? g.m : g.groups);  // of tiles: whole ones, and one more for each group that has a row
   const size_t most = kMostRingBlocks / (lines + 16) > 0 ? kMostRingBlocks / (lines + 16) : 1, slab = most * BN;
-  static std::atomic<int> allowed{0};
+  static std::atomic<unsigned long long> allowed{0};
   for (size_t col = 0; col < g.n; col += slab) {
     p.n = (unsigned)(g.n - col < slab ? g.n - col : slab);
     p.tiles_n = skl_div_up(p.n, BN);
@@ -489,7 +486,7 @@ int grouped_over(const skl_groupedk_gemm &g, GroupedRingArgs p) {
   p.tiles_m = skl_div_up(g.m, BM);
   const size_t all_n = skl_div_up(g.n, BN), left = kMostRingBlocks / p.tiles_m > 0 ? kMostRingBlocks / p.tiles_m : 1;
   const size_t slab_n = (left < all_n ? left : all_n) * BN, slab = left / all_n > 0 ? left / all_n : 1;
-  static std::atomic<int> allowed{0};
+  static std::atomic<unsigned long long> allowed{0};
   for (size_t e = 0; e < g.groups; e += slab) {
     p.groups = (unsigned)(g.groups - e < slab ? g.groups - e : slab);
     p.offsets = g.offsets ? g.offsets + e : nullptr;

@@ -2,8 +2,11 @@
 // 16 bits, and the last step of a result (not installed).
 #pragma once
 
+#include <atomic>
+
 #include "skl_device.hpp"
 #include "skl_grouped.h"
+#include "../../include/skl-hip.h"
 
 // The streaming kernels (skl_grouped_ring.hpp), and what they take: operands and the distances of their lines on 16-byte boundaries, whole 16 bytes of what lies
 // side by side along k, offsets in 32 bits.
@@ -23,6 +26,17 @@ static inline bool skl_groupedk_ring_takes(const skl_groupedk_gemm &g) {
 }
 
 namespace {
+
+// Lets `kernel` have `bytes` of LDS on the current device, once on each: `devices` has a bit for those where it may. (Racing threads ask for the same.)
+inline int skl_allow_lds(const void *kernel, unsigned bytes, std::atomic<unsigned long long> &devices) {
+  int device = 0;
+  int rc = skl_check_hip(hipGetDevice(&device), "hipGetDevice");
+  const unsigned long long bit = device < 64 ? 1ull << device : 0;
+  if (rc != 0 || (devices.load(std::memory_order_relaxed) & bit)) return rc;
+  rc = skl_check_hip(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes), "products grouped by expert: LDS size");
+  if (rc == 0) devices.fetch_or(bit, std::memory_order_relaxed);
+  return rc;
+}
 
 // Inclusive sum over the lanes of a wave up to this one.
 __device__ __forceinline__ unsigned skl_wave_scan(unsigned v) {
