@@ -3,7 +3,7 @@
 // A counting sort that keeps the order of equals. Every wave owns a run of picks and has a row of counters in LDS; a pick's place is where its group begins, the
 // picks of that group in earlier workgroups and waves, those of earlier steps of its own wave - all in the counters - and those in lower lanes of its step, which are the
 // lanes that agree with it in every bit of the group's number: a ballot for each bit. No order comes from an atomic: those only count.
-// Up to 8192 picks one workgroup does it in a launch; more are counted by a first launch, whose counts each workgroup of the second adds up for itself.
+// Up to 2048 picks one workgroup does it in a launch; more are counted by a first launch, whose counts each workgroup of the second adds up for itself.
 #include <hip/hip_runtime.h>
 
 #include <atomic>
@@ -17,7 +17,7 @@ struct GroupRowsArgs {
   const int32_t *ids;
   unsigned count, per_row, groups, bits;
   unsigned each;      // picks of a wave
-  unsigned *counts;   // [groups][workgroups], from the launch before; NULL: there is one workgroup
+  unsigned *counts;   // [workgroups][groups], from the launch before; NULL: there is one workgroup
   int32_t *offsets, *order, *rows, *place;
 };
 
@@ -39,37 +39,42 @@ __global__ void __launch_bounds__(1024) group_count_kernel(GroupRowsArgs p) {
     if (g < p.groups) atomicAdd(&count_lds[g], 1u);
   }
   __syncthreads();
-  for (unsigned g = threadIdx.x; g < p.groups; g += blockDim.x) p.counts[(size_t)g * gridDim.x + blockIdx.x] = count_lds[g];
+  for (unsigned g = threadIdx.x; g < p.groups; g += blockDim.x) p.counts[(size_t)blockIdx.x * p.groups + g] = count_lds[g];
 }
-
-__device__ __forceinline__ unsigned wave_sum(unsigned v) { return (unsigned)__builtin_amdgcn_readlane((int)skl_wave_scan(v), 63); }
 
 __global__ void __launch_bounds__(1024) group_rows_kernel(GroupRowsArgs p) {
   extern __shared__ unsigned rows_lds[];  // [waves][groups] next places; [groups] where a group begins; [groups] its picks in earlier workgroups
   __shared__ unsigned sums[16];
   const unsigned threads = blockDim.x, waves = threads / 64, lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, groups = p.groups;
   unsigned *const next = rows_lds, *const begin = next + waves * groups, *const before = begin + groups;
-  for (unsigned g = threadIdx.x; g < waves * groups; g += threads) next[g] = 0;
+  for (unsigned at = threadIdx.x; at < (waves + 2) * groups; at += threads) next[at] = 0;
   unsigned first, end;
   run_of(p, wave, waves, first, end);
-  unsigned held = first + lane < end ? (unsigned)p.ids[first + lane] : ~0u;  // the first step's, looked at again below
+  // The first two steps' picks, looked at again below.
+  const unsigned held = first + lane < end ? (unsigned)p.ids[first + lane] : ~0u, held_next = first + 64 + lane < end ? (unsigned)p.ids[first + 64 + lane] : ~0u;
   __syncthreads();
-  if (p.counts) {  // a wave per group: 64 workgroups' counts at a time
-    for (unsigned g = wave; g < groups; g += waves) {
+  if (p.counts) {  // a thread per group and part of the workgroups, eight counts under way at a time
+    const unsigned parts = threads / groups > 0 ? threads / groups : 1;
+    for (unsigned at = threadIdx.x; at < parts * groups; at += threads) {
+      const unsigned g = at % groups;
       unsigned all = 0, lower = 0;
-      for (unsigned b = lane; b < gridDim.x; b += 64) {
-        const unsigned c = p.counts[(size_t)g * gridDim.x + b];
+#pragma unroll 8
+      for (unsigned b = at / groups; b < gridDim.x; b += parts) {
+        const unsigned c = p.counts[(size_t)b * groups + g];
         all += c;
         lower += b < blockIdx.x ? c : 0u;
       }
-      all = wave_sum(all), lower = wave_sum(lower);
-      if (lane == 0) begin[g] = all, before[g] = lower;
+      atomicAdd(&begin[g], all);
+      atomicAdd(&before[g], lower);
     }
   }
   unsigned *const mine = next + wave * groups;
-  for (unsigned i = first + lane; i < end; i += 64) {
-    const unsigned g = i < first + 64 ? held : (unsigned)p.ids[i];
-    if (g < groups) atomicAdd(&mine[g], 1u);
+  const auto pick = [&](unsigned i0) { return i0 < end && end - i0 > lane ? (unsigned)p.ids[i0 + lane] : ~0u; };
+  unsigned chosen = held, chosen_next = held_next;  // two steps ahead
+  for (unsigned i0 = first; i0 < end; i0 += 64) {
+    const unsigned after = pick(i0 + 128);
+    if (chosen < groups) atomicAdd(&mine[chosen], 1u);
+    chosen = chosen_next, chosen_next = after;
   }
   __syncthreads();
   // Thread t: groups t * per .. + per - 1.
@@ -79,7 +84,7 @@ __global__ void __launch_bounds__(1024) group_rows_kernel(GroupRowsArgs p) {
     if (!p.counts) {
       unsigned all = 0;
       for (unsigned w = 0; w < waves; ++w) all += next[w * groups + g];
-      begin[g] = all, before[g] = 0;
+      begin[g] = all;
     }
     sum += begin[g];
   }
@@ -92,34 +97,37 @@ __global__ void __launch_bounds__(1024) group_rows_kernel(GroupRowsArgs p) {
     const unsigned all = begin[g];
     if (blockIdx.x == 0) p.offsets[g] = (int)at;
     unsigned to = at + before[g];
-    for (unsigned w = 0; w < waves; ++w) {
-      const unsigned c = next[w * groups + g];
-      next[w * groups + g] = to;
-      to += c;
+    for (unsigned w = 0; w < waves; w += 4) {  // (4 or 16 of them: four reads at a time)
+      unsigned *const four = next + w * groups + g;
+      const unsigned c0 = four[0], c1 = four[groups], c2 = four[2 * groups], c3 = four[3 * groups];
+      four[0] = to, four[groups] = to + c0, four[2 * groups] = to + c0 + c1, four[3 * groups] = to + c0 + c1 + c2;
+      to += c0 + c1 + c2 + c3;
     }
     at += all;
   }
   if (blockIdx.x == 0 && g1 == groups && g0 < groups) p.offsets[groups] = (int)at;
   __syncthreads();
+  chosen = held, chosen_next = held_next;
   for (unsigned i0 = first; i0 < end; i0 += 64) {
-    const unsigned i = i0 + lane, g = i0 == first ? held : i < end ? (unsigned)p.ids[i] : ~0u;
-    const bool in = g < groups;
+    const unsigned i = i0 + lane, after = pick(i0 + 128);
+    const bool in = chosen < groups;
     unsigned long long same = __ballot(in);
     for (unsigned b = 0; b < p.bits; ++b) {
-      const bool set = (g >> b) & 1u;
+      const bool set = (chosen >> b) & 1u;
       const unsigned long long of_bit = __ballot(set);
       same &= set ? of_bit : ~of_bit;
     }
     const unsigned lower = __builtin_amdgcn_mbcnt_hi((unsigned)(same >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)same, 0u));
     unsigned to = 0;
     if (in) {
-      volatile unsigned *const here = &mine[g];  // other lanes write it
+      volatile unsigned *const here = &mine[chosen];  // other lanes write it
       to = *here + lower;
-      if (p.order) p.order[to] = (int)i;
-      if (p.rows) p.rows[to] = (int)(i / p.per_row);
+      if (p.order && to < p.count) p.order[to] = (int)i;  // (true unless somebody else writes into this stream's scratch memory meanwhile)
+      if (p.rows && to < p.count) p.rows[to] = (int)(i / p.per_row);
       if (lower + 1 == (unsigned)__popcll(same)) *here = to + 1;  // the last of them; a wave's accesses are in order
     }
     if (p.place && i < end) p.place[i] = in ? (int)to : -1;
+    chosen = chosen_next, chosen_next = after;
   }
 }
 
@@ -134,10 +142,13 @@ int skl_hip_launch_group_rows(size_t count, const int32_t *ids, size_t per_row, 
   while ((size_t(1) << p.bits) < groups) ++p.bits;
   const unsigned waves = groups <= 2048 ? 16 : 4;  // their counters fit LDS
   const unsigned lds = (waves + 2) * p.groups * 4;
-  // Workgroups: 2048 picks each and no more than the compute units; what each adds up, groups x workgroups, at most 1 MiB.
-  size_t blocks = count <= 8192 ? 1 : (count + 2047) / 2048;
-  if (blocks > 256) blocks = 256;
-  if (blocks > 262144 / groups) blocks = 262144 / groups;
+  // Workgroups: a launch costs about 2 us, one workgroup 1 us for 1000 picks. What each goes through, its picks and everybody's counts, is least with sqrt(8 count / groups) of them (measured: of
+  // 131072 picks 128 / 64 / 32 workgroups with 64 groups 8.9 / 8.7 / 10.8 us, with 256 16 / 12.9 / 13.7; 32 / 16 / 8 with 2048 34 / 33 / 43); of fewer than 1024 picks each nothing is won.
+  size_t blocks = 1;
+  if (count > 2048) {
+    while (blocks < 256 && (blocks + 1) * (blocks + 1) * groups <= 8 * count) ++blocks;
+    if (blocks > (count + 1023) / 1024) blocks = (count + 1023) / 1024;
+  }
   const bool sequence = blocks > 1;
   if (sequence) {
     skl_hip_sequence_begin();

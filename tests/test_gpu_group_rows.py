@@ -48,6 +48,12 @@ def test_against_the_definition(gpu, mode, count, per_row, groups):
     check(call(gpu, ids, per_row, groups, mode=mode), ids, per_row, groups)
 
 
+@pytest.mark.parametrize("count,groups", [(2047, 40), (2048, 40), (2049, 40), (2049, 4096), (3000, 1), (300000, 3), (300000, 300), (700001, 2048)])
+def test_one_workgroup_and_more(gpu, count, groups):
+    ids = np.random.default_rng(count).integers(-1, groups, count)
+    check(call(gpu, ids, 1, groups), ids, 1, groups)
+
+
 @pytest.mark.parametrize("count", (5, 3000, 40000))
 def test_one_group_takes_all_or_nothing(gpu, count):
     for ids, groups in ((np.zeros(count), 1), (np.full(count, 6), 7), (np.full(count, -1), 7), (np.arange(count) % 2 * 63, 64)):
