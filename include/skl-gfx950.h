@@ -547,8 +547,8 @@ typedef struct skl_gfx950_u4 {
   size_t ld_scales, expert_scales;
 } skl_gfx950_u4_t;
 /* C = alpha * A * B_e + beta * C with such a B, the rest as in skl_gemm_grouped_bf16_bf16rc_f32_gfx950; groups == 1 and offsets == NULL is an ordinary layer. q - z is
- * an integer that bf16 and f16 hold, its products with A are exact, they are summed in fp32 within 32 to 128 values of one group, and those sums are scaled and added up in fp32.
- * Made for few rows: a group's codes are read once for up to 16 of its rows; more rows take more passes over them. */
+ * an integer that bf16 and f16 hold, its products with A are exact, they are summed in fp32 over at most 128 values of one group, and those sums are scaled and added up in fp32.
+ * Made for few rows: an expert's codes are read once for up to 4, 16 or 32 of its rows, by how many there are on average; more rows take more passes over them. */
 void skl_gemm_grouped_bf16_u4c_f32_gfx950(size_t groups, const int32_t *offsets, size_t m, size_t n, size_t k, float alpha, const skl_bf16_t *a, size_t rsa,
                                           const int32_t *rows, size_t a_rows, const skl_gfx950_u4_t *b, float beta, float *c, size_t rsc);
 void skl_gemm_grouped_bf16_u4c_bf16_gfx950(size_t groups, const int32_t *offsets, size_t m, size_t n, size_t k, float alpha, const skl_bf16_t *a, size_t rsa,

@@ -158,11 +158,12 @@ __device__ __forceinline__ v4i quarters_transposed(v4i v) {
   return v4i{(int)c[0], (int)c[1], (int)d[0], (int)d[1]};
 }
 
-constexpr unsigned kUnit = 128, kWaves = 8, kThreads = kWaves * 64;  // of k
+constexpr unsigned kUnit = 128;  // of k
 
 // What a kernel holds. PER: groups of a unit, 4, 2 or 1; F: 16 columns each; ROWS: of A, staged in LDS for a chunk of UNITS units per wave.
-template <int PER, bool ZEROS, int F, int ROWS, int UNITS>
+template <int PER, bool ZEROS, int F, int ROWS, int UNITS, int WAVES>
 struct U4Shape {
+  static constexpr unsigned kWaves = WAVES, kThreads = kWaves * 64;
   static constexpr unsigned kR = (ROWS + 15) / 16, kCols = 16 * F, kChunk = kUnit * kWaves * UNITS;
   static constexpr unsigned kPitch = kChunk * 2 + 16;  // bytes of a row of A: 16 rows meet in no bank
   static constexpr unsigned kPieces = (ROWS * kChunk / 8 + kThreads - 1) / kThreads, kRowPieces = kChunk / 8;
@@ -176,9 +177,10 @@ struct U4Shape {
   };
 };
 
-template <typename T, int PER, bool ZEROS, int F, int ROWS, int UNITS, int MIN>
-__global__ void __launch_bounds__(kThreads, MIN) gemm_u4_stream_kernel(U4Args p, int c_single) {
-  using Shape = U4Shape<PER, ZEROS, F, ROWS, UNITS>;
+template <typename T, int PER, bool ZEROS, int F, int ROWS, int UNITS, int MIN, int WAVES>
+__global__ void __launch_bounds__(WAVES * 64, MIN) gemm_u4_stream_kernel(U4Args p, int c_single) {
+  using Shape = U4Shape<PER, ZEROS, F, ROWS, UNITS, WAVES>;
+  constexpr unsigned kWaves = Shape::kWaves, kThreads = Shape::kThreads;
   constexpr bool kFine = PER > 1;       // groups smaller than the 128 k whose codes the quarters of a wave hold side by side
   constexpr unsigned kCols = Shape::kCols, kChunk = Shape::kChunk, kEntries = Shape::kEntries, kEach = Shape::kEach, kPitch = Shape::kPitch, kPieces = Shape::kPieces, kRowPieces = Shape::kRowPieces;
   constexpr int R = Shape::kR;
@@ -244,7 +246,8 @@ __global__ void __launch_bounds__(kThreads, MIN) gemm_u4_stream_kernel(U4Args p,
 #pragma unroll
       for (int i = 0; i < (int)kEach; ++i) {  // [column][entry]: a scale with its zero point above
         const unsigned at = threadIdx.x + i * kThreads;
-        if (kCols * kEntries % kThreads == 0 || at < kCols * kEntries) reinterpret_cast<unsigned *>(to + Shape::kBytesA)[at / kEntries * (kEntries + 1) + at % kEntries] = from.scale[i] | (ZEROS ? from.zero[ZEROS ? i : 0] : 8u) << 16;
+        if (kCols * kEntries % kThreads == 0 || at < kCols * kEntries) reinterpret_cast<unsigned *>(to + Shape::kBytesA)[at / kEntries * (kEntries + 1) + at % kEntries] =
+            (kFine && at % kEntries + c * kEntries > last_group ? 0u : from.scale[i]) | (ZEROS ? from.zero[ZEROS ? i : 0] : 8u) << 16;  // (behind k no scale that is infinite, for sums that are zero)
       }
     };
     v4f sum[R][F];
@@ -334,26 +337,31 @@ __global__ void __launch_bounds__(kThreads, MIN) gemm_u4_stream_kernel(U4Args p,
   }
 }
 
-template <typename T, int PER, bool ZEROS, int F, int ROWS, int UNITS, int MIN>
+template <typename T, int PER, bool ZEROS, int F, int ROWS, int UNITS, int MIN, int WAVES>
 int launch_stream(const U4Args &p, int c_single) {
-  constexpr unsigned kLds = U4Shape<PER, ZEROS, F, ROWS, UNITS>::kLds;
-  const auto kernel = gemm_u4_stream_kernel<T, PER, ZEROS, F, ROWS, UNITS, MIN>;
+  constexpr unsigned kLds = U4Shape<PER, ZEROS, F, ROWS, UNITS, WAVES>::kLds;
+  const auto kernel = gemm_u4_stream_kernel<T, PER, ZEROS, F, ROWS, UNITS, MIN, WAVES>;
   static std::atomic<unsigned long long> allowed{0};
   const int rc = skl_allow_lds(reinterpret_cast<const void *>(kernel), kLds, allowed);
   if (rc != 0) return rc;
-  kernel<<<dim3(skl_div_up(p.n, 16 * F), p.groups), dim3(kThreads), kLds, skl_current_stream()>>>(p, c_single);
+  kernel<<<dim3(skl_div_up(p.n, 16 * F), p.groups), dim3(WAVES * 64), kLds, skl_current_stream()>>>(p, c_single);
   return skl_check_launch("gemm_u4");
 }
 
 template <typename T, int PER, bool ZEROS>
 int stream_by_size(const U4Args &p, int c_single) {
-  // By the rows there are for a matrix, on average where there are several: rows beyond a pass read the codes again. us, 1 / 4 / 16 rows a pass: 1 x 4096 x 11008 9.8 / 10.5 / -,
-  // 8 tokens to 4 of 32 experts 44 / 26 / 31, 64 tokens 45 with 16 and 61 with 4. Fewer columns and shorter chunks a workgroup, more workgroups: F = 2 rather than 1 costs 1 x 4096 x 11008
-  // 1.2 us, twice the chunk 0.1 to 1.7; with 16 rows, whose operands are read for all columns, F = 2 is the faster one (16 x 8192 x 8192 14.9, F = 1 17.4).
-  if (p.m == 1) return launch_stream<T, PER, ZEROS, 1, 1, 2, 6>(p, c_single);
-  if (p.m <= 4 * (size_t)p.groups) return launch_stream<T, PER, ZEROS, 1, 4, 1, 6>(p, c_single);
-  if (p.m <= 16 * (size_t)p.groups) return launch_stream<T, PER, ZEROS, 2, 16, 1, 4>(p, c_single);
-  return launch_stream<T, PER, ZEROS, 2, 32, 1, 2>(p, c_single);
+  // By the rows there are for a matrix, on average where there are several: rows beyond a pass read the codes again, and what a pass has room for is computed. us, 4 / 16 / 32 rows a pass: one
+  // row 9.8 (1 row) / 10.5 (4) for 4096 x 11008; 32 matrices of 2048 x 2816 with 32 rows 23.6 / 24.9 / -, 128 rows 47.9 / 34.4 / -, 256 rows 61 / 36.3 / 54.4.
+  // And by the workgroups there are, each with all of k: eight waves for a column's k where they hardly fill the chip, four where more workgroups, of half the LDS, then overlap. us,
+  // eight / four: one row 4096 x 11008 9.9 / 9.5, 11008 x 4096 9.5 / 12.3, 4096 x 28672 19.4 / 17.1; 48 rows for 64 of 4096 x 1408 35.4 / 27.7; 16 rows 8192 x 8192 14.8 / 20.4, 256 rows
+  // for 32 of 2048 x 2816 44.5 / 36.3, 128 rows for 8 of 4096 x 4096 39.1 / 38.6; 64 rows 4096 x 11008 40.8 / 36.4, 8192 x 8192 37.4 / 46.0.
+  // Fewer columns and shorter chunks a workgroup, more workgroups: F = 2 rather than 1 costs one row 4096 x 11008 1.2 us, twice the chunk 0.1 to 1.7; with 16 rows, whose operands are read for
+  // all columns, F = 2 is the faster one (16 x 8192 x 8192 14.9, F = 1 17.4).
+  const size_t m = p.m, groups = p.groups, runs = (size_t)skl_div_up(p.n, 16) * groups;
+  if (m == 1) return runs >= 640 ? launch_stream<T, PER, ZEROS, 1, 1, 2, 4, 4>(p, c_single) : launch_stream<T, PER, ZEROS, 1, 1, 2, 6, 8>(p, c_single);
+  if (m <= 4 || m <= 2 * groups) return runs >= 512 ? launch_stream<T, PER, ZEROS, 1, 4, 2, 4, 4>(p, c_single) : launch_stream<T, PER, ZEROS, 1, 4, 1, 6, 8>(p, c_single);
+  if (m <= 16 * groups) return runs >= 4096 ? launch_stream<T, PER, ZEROS, 2, 16, 1, 2, 4>(p, c_single) : launch_stream<T, PER, ZEROS, 2, 16, 1, 4, 8>(p, c_single);
+  return runs >= 640 ? launch_stream<T, PER, ZEROS, 2, 32, 1, 2, 4>(p, c_single) : launch_stream<T, PER, ZEROS, 2, 32, 1, 2, 8>(p, c_single);
 }
 
 template <typename T>

@@ -147,3 +147,31 @@ def test_the_same_bits_on_every_run(gpu):
     first = run_u4(gpu, "bf16", "f32", 7, 2000, 4096, 128, seed=1)
     for _ in range(3):
         assert np.array_equal(first.view(np.uint32), run_u4(gpu, "bf16", "f32", 7, 2000, 4096, 128, seed=1).view(np.uint32))
+
+
+@pytest.mark.parametrize("k,group_k", [(96, 32), (160, 32), (192, 64), (1120, 32), (2112, 64), (40, 64)])
+@pytest.mark.parametrize("m", (1, 3, 20))
+def test_an_infinite_scale_at_the_end(gpu, m, k, group_k):
+    """The last group's scale is infinite and its sums are not zero: infinities of their sign, as the definition has it - nothing behind k joins in."""
+    n, blocks = 33, -(-k // group_k)
+    a = gs.bits(np.ones((m, k)), "bf16")
+    q = np.full((n, k), 11, np.uint8)
+    q[1::2] = 3
+    scales = np.ones((n, blocks), np.float32)
+    scales[:, -1] = np.inf
+    bufs = [DeviceBuffer.from_array(v) for v in (a, gs.u4_store(q, k), gs.bits(scales, "bf16"))]
+    c = DeviceBuffer(4 * m * n)
+    w = U4Weights(group_k=group_k, codes=bufs[1], ld=k, expert=0, scales=bufs[2], zeros=None, ld_scales=blocks, expert_scales=0)
+    gpu.skl_gemm_grouped_bf16_u4c_f32_gfx950(1, None, m, n, k, 1.0, bufs[0], k, None, 0, w, 0.0, c, n)
+    got = c.download(np.float32).reshape(m, n)
+    skl_amd.check_error()
+    assert np.all(got[:, 0::2] == np.inf) and np.all(got[:, 1::2] == -np.inf)
+
+
+@pytest.mark.parametrize("m,n,groups", [(1, 10300, 1), (3, 8300, 1), (4, 520, 16), (40, 400, 40), (200, 1100, 64), (30, 10300, 1), (70, 5200, 2)])
+@pytest.mark.parametrize("k,group_k,zeros", [(544, 32, "some"), (1600, 64, None), (1184, 2000, "far"), (1280, 128, "some")])
+def test_many_workgroups(gpu, m, n, groups, k, group_k, zeros):
+    """Sizes at which four waves, not eight, share a column's k."""
+    rng = np.random.default_rng(m + n)
+    offsets = None if groups == 1 else split(rng, m, groups)
+    run_u4(gpu, "f16" if k == 1600 else "bf16", "f32", m, n, k, group_k, offsets=offsets, groups=groups, zeros=zeros, seed=n)
