@@ -28,7 +28,7 @@ struct GroupedRingArgs {
   size_t rsc, gsc;                   // elements
   unsigned groups, m, n, k, a_rows, b_rows;  // OVER: k is the number of rows in all
   unsigned tiles_m, tiles_n;         // OVER: of a group
-  int c_single, by_group;            // by_group: a group's tiles are taken together
+  int c_single;
   skl_scalar alpha, beta;
 };
 
@@ -377,8 +377,7 @@ template <int DT, bool B_KC, int MOST, int BN, int WAVES, int NS>
 __global__ void __launch_bounds__(WAVES * 64) gemm_grouped_rows_kernel(GroupedRingArgs p) {
   using Rows = GroupedRows<DT, B_KC, MOST, BN, WAVES, NS>;
   extern __shared__ __attribute__((aligned(128))) char grouped_smem[];
-  const GroupedPlace at = MOST == 256 && p.by_group ? grouped_place_by_group(p.offsets, p.groups, p.m, p.tiles_n, blockIdx.x, gridDim.x / 8)
-                                                    : grouped_place<MOST>(p.offsets, p.groups, p.m, p.tiles_n, blockIdx.x);
+  const GroupedPlace at = grouped_place<MOST>(p.offsets, p.groups, p.m, p.tiles_n, blockIdx.x);
   if (at.none) return;
   const unsigned col0 = at.tile_n * BN;
   GroupedTile t;
@@ -459,25 +458,18 @@ int grouped_rows(const skl_grouped_gemm &g, GroupedRingArgs p) {
     p.tiles_n = skl_div_up(p.n, BN);
     p.b = (const char *)g.b + col * g.csb * 2;
     p.c = (char *)g.c + col * (g.c_single ? 4 : 2);
-    const int rc = launch_ring(gemm_grouped_rows_kernel<DT, B_KC, MOST, BN, WAVES, NS>, allowed, GroupedRows<DT, B_KC, MOST, BN, WAVES, NS>::kLds, WAVES * 64, p,
-                               (lines * p.tiles_n / 8 * (p.by_group ? 9 : 8) / 8 + 2) * 8);
+    const int rc = launch_ring(gemm_grouped_rows_kernel<DT, B_KC, MOST, BN, WAVES, NS>, allowed, GroupedRows<DT, B_KC, MOST, BN, WAVES, NS>::kLds, WAVES * 64, p, (lines * p.tiles_n / 8 + 2) * 8);
     if (rc != 0) return rc;
   }
   return 0;
 }
 template <int DT, bool B_KC>
-int grouped_rows_by_size(const skl_grouped_gemm &g, GroupedRingArgs p) {
+int grouped_rows_by_size(const skl_grouped_gemm &g, const GroupedRingArgs &p) {
   // By how many rows a group has on average and how many tiles there are: the largest tile that is mostly filled and fills the chip. us, 256 x 256 / 128 x 128 / 64 x 64: 32 groups of
   // 2816 x 2048 with 256, 512, 1024 and 3000 tokens to four of them -, 84, 78; 92, 85, 93; 107, 116, 140; 167, 200, 315; two groups of 1024 x 1024 with 2000 rows 27, 15, 13. One token to four of
   // 32 groups: 64 x 64 with eight slices of k in the ring 12.5, 64 x 128 with four 28.
   const size_t groups = g.m < g.groups ? g.m : g.groups, lines = g.m / 256 + groups / 2, lines_half = g.m / 128 + groups / 2;  // half of the last tiles of the groups are small ones
-  if (g.m >= 112 * groups && lines * skl_div_up(g.n, 256) >= 160) {
-    // Where there are many tiles a group's are taken together; where not, its small tiles behind everybody's whole ones, which leaves less for the last of them to wait for. us, together / behind:
-    // 8 groups of 14336 x 4096 with 8192 rows (8 tiles to a compute unit) 822 / 868, 64 of 2048 x 1408 with 32768 rows (5) 260 / 269, of 1408 x 2048 (4) 236 / 230, 8 of 4096 x 14336 with 4096
-    // rows (1.4) 725 / 703.
-    p.by_group = lines * skl_div_up(g.n, 256) >= 1152;
-    return grouped_rows<DT, B_KC, 256, 256, 8, 4>(g, p);
-  }
+  if (g.m >= 112 * groups && lines * skl_div_up(g.n, 256) >= 160) return grouped_rows<DT, B_KC, 256, 256, 8, 4>(g, p);
   if (g.m >= 56 * groups && lines_half * skl_div_up(g.n, 128) >= 160) return grouped_rows<DT, B_KC, 128, 128, 8, 4>(g, p);
   return grouped_rows<DT, B_KC, 64, 64, 4, 8>(g, p);
 }

@@ -62,20 +62,27 @@ __device__ __forceinline__ SklRange skl_group_range(const int32_t *offsets, unsi
   return {b, f > b ? f - b : 0u};
 }
 
-// Which tile of which group a workgroup takes. `whole` tiles of MOST rows come first, group after group, then one for what is left of each group; both are dealt out to the
-// eight dies in runs, so that a die's workgroups share operands. Lane l counts for groups l * each .. + each - 1.
+// Which tile of which group a workgroup takes. A group's rows are lines of MOST; the last one, if it is a small tile - for MOST == 256 of up to 128 rows -, comes behind everybody's others, so that
+// what ends last ends soon. Both kinds go group after group, up to eight lines of a group column by column so that B comes once for them, and are dealt out to the eight dies in runs, so that a die's
+// workgroups share operands. (Last lines of more than 128 rows behind the whole ones, too, read B once more: 8 groups of 14336 x 4096 with 8192 rows 926 us against 870, 64 of 2048 x 1408 with 32768
+// 270 against 250; all of a group's lines together and the dies' runs cut by cost 869 and 259, of 4096 x 4096 16 groups with 32768 rows 940 against 900.) Lane l counts for groups
+// l * each .. + each - 1.
 struct GroupedPlace {
   unsigned e, first, rows, tile_n;  // rows first .. first + rows - 1 of A and C
   bool none;
 };
 template <int MOST>
 __device__ __forceinline__ GroupedPlace grouped_place(const int32_t *offsets, unsigned groups, unsigned m, unsigned tiles_n, unsigned id) {
+  // Lines of tiles of (nearly) MOST rows, and whether a smaller one is left.
+  constexpr unsigned kSmall = MOST == 256 ? 128 : MOST - 1;
+  const auto whole_of = [](unsigned rows) { return rows / MOST + (rows % MOST > kSmall); };
+  const auto rest_of = [](unsigned rows) { return (unsigned)(rows % MOST != 0 && rows % MOST <= kSmall); };
   const unsigned lane = threadIdx.x & 63u, each = (groups + 63) / 64, g0 = lane * each;
   unsigned whole = 0, rest = 0;
   SklRange mine_last{0, 0};  // with one group to a lane, the lane's
   for (unsigned g = g0; g < g0 + each && g < groups; ++g) {
     mine_last = skl_group_range(offsets, g, m);
-    whole += mine_last.rows / MOST, rest += mine_last.rows % MOST != 0;
+    whole += whole_of(mine_last.rows), rest += rest_of(mine_last.rows);
   }
   const unsigned whole_upto = skl_wave_scan(whole), rest_upto = skl_wave_scan(rest);
   const unsigned all_whole = (unsigned)__builtin_amdgcn_readlane((int)whole_upto, 63) * tiles_n, all_rest = (unsigned)__builtin_amdgcn_readlane((int)rest_upto, 63) * tiles_n;
@@ -98,11 +105,11 @@ __device__ __forceinline__ GroupedPlace grouped_place(const int32_t *offsets, un
   unsigned lines;
   if (each == 1) {  // (what the lane holds: no second trip to memory)
     r = {(unsigned)__builtin_amdgcn_readlane((int)mine_last.first, owner), (unsigned)__builtin_amdgcn_readlane((int)mine_last.rows, owner)};
-    lines = is_whole ? r.rows / MOST : r.rows % MOST != 0;
+    lines = is_whole ? whole_of(r.rows) : rest_of(r.rows);
   } else {
     for (;; ++e) {
       r = skl_group_range(offsets, e, m);
-      lines = is_whole ? r.rows / MOST : r.rows % MOST != 0;
+      lines = is_whole ? whole_of(r.rows) : rest_of(r.rows);
       if (line < before + lines || e + 1 >= groups) break;
       before += lines;
     }
@@ -112,80 +119,12 @@ __device__ __forceinline__ GroupedPlace grouped_place(const int32_t *offsets, un
     const unsigned in = t - before * tiles_n, block = in / (8 * tiles_n), in_block = in - block * (8 * tiles_n), deep = lines - 8 * block < 8 ? lines - 8 * block : 8;
     at.tile_n = in_block / deep;
     at.first = r.first + (8 * block + in_block % deep) * MOST;
-    at.rows = MOST;
+    at.rows = r.rows - (at.first - r.first) < MOST ? r.rows - (at.first - r.first) : MOST;
   } else {
     at.tile_n = t % tiles_n;
     at.first = r.first + r.rows / MOST * MOST;
     at.rows = r.rows % MOST;
   }
-  // uniform, and the compiler is told: branches and descriptors go by them
-  at.e = (unsigned)__builtin_amdgcn_readfirstlane((int)at.e), at.first = (unsigned)__builtin_amdgcn_readfirstlane((int)at.first);
-  at.rows = (unsigned)__builtin_amdgcn_readfirstlane((int)at.rows), at.tile_n = (unsigned)__builtin_amdgcn_readfirstlane((int)at.tile_n);
-  return at;
-}
-
-// The other order, of tiles of 256 rows and what is left as smaller ones: a group's tiles together, up to eight lines at a time column by column, so that B comes once for all of them.
-// Each die's run is as long by what its tiles cost as the grid's `slots` for a die let it be. Its last tiles may be large ones: for many tiles (grouped_rows_by_size).
-__device__ __forceinline__ GroupedPlace grouped_place_by_group(const int32_t *offsets, unsigned groups, unsigned m, unsigned tiles_n, unsigned id, unsigned slots) {
-  constexpr unsigned MOST = 256;
-  const auto lines_of = [](unsigned rows) { return (rows + MOST - 1) / MOST; };
-  const unsigned lane = threadIdx.x & 63u, each = (groups + 63) / 64, g0 = lane * each;
-  unsigned count = 0, cost = 0;
-  SklRange last{0, 0};  // with one group to a lane, the lane's
-  for (unsigned g = g0; g < g0 + each && g < groups; ++g) {
-    last = skl_group_range(offsets, g, m);
-    count += lines_of(last.rows);
-    const unsigned rest = last.rows % MOST;
-    cost += last.rows / MOST * 8 + (rest > 128 ? 8 : rest > 64 ? 5 : rest > 0 ? 4 : 0);
-  }
-  const unsigned upto = skl_wave_scan(count), all = (unsigned)__builtin_amdgcn_readlane((int)upto, 63) * tiles_n;
-  const unsigned die = id % 8, slot = id / 8;
-  const unsigned cost_upto = skl_wave_scan(cost), whole_cost = (unsigned)__builtin_amdgcn_readlane((int)cost_upto, 63);
-  unsigned first = 0, end = 0;  // this die's run
-  for (unsigned d = 0; d <= die; ++d) {
-    first = end;
-    // In the lane where d + 1 eighths of the cost are reached, as far into its tiles as into its cost; the dies behind have to hold the others.
-    const float reached = (float)whole_cost * (float)(d + 1) * 0.125f;
-    const unsigned long long behind = __ballot((float)cost_upto > reached);
-    end = all;
-    if (behind && d < 7) {
-      const int at = (int)__builtin_ctzll(behind);
-      const float ahead = (float)__builtin_amdgcn_readlane((int)(cost_upto - cost), at), mine = (float)__builtin_amdgcn_readlane((int)cost, at);
-      const unsigned lines = (unsigned)__builtin_amdgcn_readlane((int)count, at), before = (unsigned)__builtin_amdgcn_readlane((int)(upto - count), at);
-      const float part = (reached - ahead) / mine * (float)(lines * tiles_n);
-      end = before * tiles_n + (part > 0 ? (unsigned)part : 0u);
-    }
-    const unsigned behind_hold = (7 - d) * slots;
-    end = end < first ? first : end - first > slots ? first + slots : end;
-    if (all > behind_hold && end < all - behind_hold) end = all - behind_hold;
-  }
-  const unsigned t = first + slot, line = t / tiles_n;  // line: row of tiles
-  GroupedPlace at{0, 0, 0, 0, t >= end};
-  if (at.none) return at;
-  const unsigned long long behind = __ballot(line < upto);
-  at.none = behind == 0;  // (sums beyond 32 bits, of offsets that fall back)
-  if (at.none) return at;
-  const int owner = (int)__builtin_ctzll(behind);
-  unsigned before = (unsigned)__builtin_amdgcn_readlane((int)(upto - count), owner);  // lines of the groups ahead
-  unsigned e = (unsigned)owner * each;
-  SklRange r;
-  unsigned lines;
-  if (each == 1) {  // (what the lane holds: no second trip to memory)
-    r = {(unsigned)__builtin_amdgcn_readlane((int)last.first, owner), (unsigned)__builtin_amdgcn_readlane((int)last.rows, owner)};
-    lines = lines_of(r.rows);
-  } else {
-    for (;; ++e) {
-      r = skl_group_range(offsets, e, m);
-      lines = lines_of(r.rows);
-      if (line < before + lines || e + 1 >= groups) break;
-      before += lines;
-    }
-  }
-  at.none = line - before >= lines;
-  if (at.none) return at;
-  const unsigned in = t - before * tiles_n, block = in / (8 * tiles_n), in_block = in - block * (8 * tiles_n), deep = lines - 8 * block < 8 ? lines - 8 * block : 8;
-  const unsigned in_group = (8 * block + in_block % deep) * MOST;
-  at.e = e, at.tile_n = in_block / deep, at.first = r.first + in_group, at.rows = r.rows - in_group < MOST ? r.rows - in_group : MOST;
   // uniform, and the compiler is told: branches and descriptors go by them
   at.e = (unsigned)__builtin_amdgcn_readfirstlane((int)at.e), at.first = (unsigned)__builtin_amdgcn_readfirstlane((int)at.first);
   at.rows = (unsigned)__builtin_amdgcn_readfirstlane((int)at.rows), at.tile_n = (unsigned)__builtin_amdgcn_readfirstlane((int)at.tile_n);

@@ -58,13 +58,13 @@ def test_many_groups(gpu, groups):
 
 @pytest.mark.parametrize("groups,n,layout", ((64, 5118, "col"), (130, 2560, "row")))
 def test_many_tiles_of_uneven_groups(gpu, groups, n, layout):
-    """Enough tiles of 256 rows for a group's to be taken together: the dies' runs of them are dealt out by what they cost."""
+    """Many tiles of 256 rows, last lines of every length."""
     rng = np.random.default_rng(groups)
     share = rng.exponential(size=groups) ** 2 * (rng.random(groups) > 0.1)
     sizes = np.floor(share / share.sum() * 113 * groups).astype(int)
     sizes[groups // 2] += 113 * groups - sizes.sum()
     run_grouped(gpu, "bf16", "bf16", int(sizes.sum()) + 3, n, 16, offsets_of(sizes, 3), groups, layout=layout, seed=groups)
-    # all in one group, the last: one lane holds the tiles and their cost
+    # all in one group, the last: one lane holds all tiles
     sizes[:], sizes[-1] = 0, 113 * groups
     run_grouped(gpu, "bf16", "bf16", int(sizes.sum()), n, 8, offsets_of(sizes), groups, layout=layout, seed=groups)
 
