@@ -519,7 +519,7 @@ void skl_gemm_grouped_f16_f16rc_f16_gfx950(size_t groups, const int32_t *offsets
  * dW_e = dY^T X with A = dY, B = X. A has m columns and B n, both row-major; ra(r) = rows_a[r], or r where rows_a is NULL, likewise rb; of `total` rows in all
  * (offsets are cut off at 0 and total; rows_a == NULL: A has them all). C_e(i, j) at c[e * gsc + i * rsc + j]. An empty group makes C_e = beta * C_e. Everything else as above:
  * a row whose index is outside [0, a_rows) or [0, b_rows) counts as zeros, offsets may be NULL with groups == 1, total is at most 2^30. A sum is taken in the order of its
- * rows' places in tiles whose size depends on m, n, groups and total alone. */
+ * rows' places; where C has few values and groups many rows, in parts, by m, n, groups and total and by whether the stream holds scratch memory. */
 void skl_gemm_groupedk_bf16c_bf16_f32_gfx950(size_t groups, const int32_t *offsets, size_t m, size_t n, size_t total, float alpha, const skl_bf16_t *a,
                                              size_t rsa, const int32_t *rows_a, size_t a_rows, const skl_bf16_t *b, size_t rsb, const int32_t *rows_b,
                                              size_t b_rows, float beta, float *c, size_t rsc, size_t gsc);
@@ -548,6 +548,7 @@ typedef struct skl_gfx950_u4 {
 } skl_gfx950_u4_t;
 /* C = alpha * A * B_e + beta * C with such a B, the rest as in skl_gemm_grouped_bf16_bf16rc_f32_gfx950; groups == 1 and offsets == NULL is an ordinary layer. q - z is
  * an integer that bf16 and f16 hold, its products with A are exact, they are summed in fp32 over at most 128 values of one group, and those sums are scaled and added up in fp32.
+ * (An infinite scale thus meets the sum, not each product: no NaN from a code that equals its zero point.)
  * Made for few rows: an expert's codes are read once for up to 4, 16 or 32 of its rows, by how many there are on average; more rows take more passes over them. */
 void skl_gemm_grouped_bf16_u4c_f32_gfx950(size_t groups, const int32_t *offsets, size_t m, size_t n, size_t k, float alpha, const skl_bf16_t *a, size_t rsa,
                                           const int32_t *rows, size_t a_rows, const skl_gfx950_u4_t *b, float beta, float *c, size_t rsc);

@@ -28,6 +28,7 @@ struct GroupedRingArgs {
   size_t rsc, gsc;                   // elements
   unsigned groups, m, n, k, a_rows, b_rows;  // OVER: k is the number of rows in all
   unsigned tiles_m, tiles_n;         // OVER: of a group
+  unsigned parts;                    // OVER: a group's rows are shared out over so many; more than 1: C is each part's own
   int c_single;
   skl_scalar alpha, beta;
 };
@@ -427,9 +428,17 @@ __global__ void __launch_bounds__(WAVES * 64) gemm_grouped_over_kernel(GroupedRi
   const unsigned tiles = p.tiles_m * p.tiles_n, run = (tiles + 7) / 8, die = blockIdx.x % 8, slot = blockIdx.x / 8;
   const unsigned in = die * run + slot % run;
   if (in >= tiles) return;
-  const GroupedTurn turn = grouped_by_length(p.offsets, p.groups, p.k, slot / run);
-  const unsigned e = turn.e;
-  const SklRange r = turn.rows;
+  unsigned e = slot / run;  // its part, too
+  SklRange r;
+  if (p.parts == 1) {
+    const GroupedTurn turn = grouped_by_length(p.offsets, p.groups, p.k, e);
+    e = turn.e, r = turn.rows;
+  } else {
+    r = skl_group_range(p.offsets, e / p.parts, p.k);
+    const unsigned each = (r.rows + p.parts * 64 - 1) / (p.parts * 64) * 64, before = e % p.parts * each;  // whole slices but for the last one's
+    r.first = (unsigned)__builtin_amdgcn_readfirstlane((int)(r.first + (before < r.rows ? before : r.rows)));
+    r.rows = (unsigned)__builtin_amdgcn_readfirstlane((int)(before < r.rows ? (r.rows - before < each ? r.rows - before : each) : 0u));
+  }
   const unsigned block = in / (8 * p.tiles_n), in_block = in - block * (8 * p.tiles_n), deep = p.tiles_m - 8 * block < 8 ? p.tiles_m - 8 * block : 8;
   const unsigned row0 = (8 * block + in_block % deep) * BM, col0 = in_block / deep * BN;
   GroupedTile t;
@@ -438,6 +447,39 @@ __global__ void __launch_bounds__(WAVES * 64) gemm_grouped_over_kernel(GroupedRi
   t.b = B_INDEXED ? p.b : p.b + (size_t)r.first * p.b_pitch, t.b_first = col0, t.b_count = p.n - col0, t.k = r.rows;
   t.c = p.c + ((size_t)e * p.gsc + (size_t)row0 * p.rsc + col0) * (p.c_single ? 4 : 2), t.rows = p.m - row0, t.cols = p.n - col0;
   Ring::run(p, t, grouped_smem);
+}
+
+// Sums of parts, added up in their order: C_e = alpha * (part 0 + part 1 + ..) + beta * C_e.
+struct GroupedJoin {
+  const float *from;  // [groups][parts][m][n]
+  void *c;
+  size_t rsc, gsc;
+  unsigned groups, m, n, parts;
+  int c_single;
+  skl_scalar alpha, beta;
+};
+template <typename TC>
+__global__ void __launch_bounds__(256) gemm_grouped_join_kernel(GroupedJoin p) {
+  const size_t size = (size_t)p.m * p.n;
+  const bool read_c = !skl_beta_is_zero<float>(p.beta);
+  for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < size * p.groups; i += (size_t)gridDim.x * 256) {
+    const unsigned e = (unsigned)(i / size), in = (unsigned)(i % size), row = in / p.n, col = in % p.n;
+    const float *const from = p.from + (size_t)e * p.parts * size + in;
+    float sum = from[0];
+#pragma unroll 4
+    for (unsigned part = 1; part < p.parts; ++part) sum = __fadd_rn(sum, from[part * size]);
+    TC *const to = reinterpret_cast<TC *>(p.c) + (size_t)e * p.gsc + (size_t)row * p.rsc + col;
+    *to = skl_grouped_result(sum, to, p.alpha, p.beta, read_c);
+  }
+}
+template <int DT>
+int launch_join(const GroupedJoin &j) {
+  const size_t blocks = skl_div_up((size_t)j.m * j.n * j.groups, 256);
+  const dim3 grid((unsigned)(blocks < 4096 ? blocks : 4096));
+  if (j.c_single) gemm_grouped_join_kernel<float><<<grid, dim3(256), 0, skl_current_stream()>>>(j);
+  else if (DT == SKL_DT_BF16) gemm_grouped_join_kernel<__bf16><<<grid, dim3(256), 0, skl_current_stream()>>>(j);
+  else gemm_grouped_join_kernel<_Float16><<<grid, dim3(256), 0, skl_current_stream()>>>(j);
+  return skl_check_launch("gemm_grouped: join");
 }
 
 template <typename K>
@@ -490,6 +532,18 @@ int grouped_over(const skl_groupedk_gemm &g, GroupedRingArgs p) {
   const size_t all_n = skl_div_up(g.n, BN), left = kMostRingBlocks / p.tiles_m > 0 ? kMostRingBlocks / p.tiles_m : 1;
   const size_t slab_n = (left < all_n ? left : all_n) * BN, slab = left / all_n > 0 ? left / all_n : 1;
   static std::atomic<unsigned long long> allowed{0};
+  const auto launch = [&](size_t blocks) {
+    return launch_ring(gemm_grouped_over_kernel<DT, BM, BN, WAVES, WAVES_N, A_INDEXED, B_INDEXED>, allowed, GroupedRing<DT, false, false, BM, BN, WAVES, WAVES_N, 4>::kLds, WAVES * 64, p, blocks);
+  };
+  if (p.parts > 1) {  // (few tiles, one launch) C of every part into scratch memory, where the join finds them
+    const GroupedJoin j{(const float *)p.c, g.c, g.rsc, g.gsc, (unsigned)g.groups, p.m, (unsigned)g.n, p.parts, g.c_single, g.alpha, g.beta};
+    p.n = (unsigned)g.n, p.tiles_n = (unsigned)all_n, p.offsets = g.offsets, p.groups = (unsigned)g.groups;
+    p.b = (const char *)g.b;
+    p.rsc = g.n, p.gsc = g.m * g.n, p.c_single = 1;
+    p.alpha.f = 1.0f, p.beta.fz.value = 0.0f, p.beta.fz.skip_c_read = SKL_C_UNTOUCHED;
+    const int rc = launch(g.groups * p.parts * ((p.tiles_m * all_n + 7) / 8) * 8);
+    return rc != 0 ? rc : launch_join<DT>(j);
+  }
   for (size_t e = 0; e < g.groups; e += slab) {
     p.groups = (unsigned)(g.groups - e < slab ? g.groups - e : slab);
     p.offsets = g.offsets ? g.offsets + e : nullptr;
@@ -498,8 +552,7 @@ int grouped_over(const skl_groupedk_gemm &g, GroupedRingArgs p) {
       p.tiles_n = skl_div_up(p.n, BN);
       p.b = (const char *)g.b + col * 2;
       p.c = (char *)g.c + (e * g.gsc + col) * (g.c_single ? 4 : 2);
-      const int rc = launch_ring(gemm_grouped_over_kernel<DT, BM, BN, WAVES, WAVES_N, A_INDEXED, B_INDEXED>, allowed, GroupedRing<DT, false, false, BM, BN, WAVES, WAVES_N, 4>::kLds, WAVES * 64, p,
-                                 (size_t)p.groups * (((size_t)p.tiles_m * p.tiles_n + 7) / 8) * 8);
+      const int rc = launch((size_t)p.groups * (((size_t)p.tiles_m * p.tiles_n + 7) / 8) * 8);
       if (rc != 0) return rc;
     }
   }
@@ -517,8 +570,28 @@ int grouped_over_ring(const skl_groupedk_gemm &g) {
   p.rows = g.rows_a, p.rows_b = g.rows_b, p.a_rows = (unsigned)g.a_rows, p.b_rows = (unsigned)g.b_rows;
   p.rsc = g.rsc, p.gsc = g.gsc, p.m = (unsigned)g.m, p.k = (unsigned)g.total;
   p.c_single = g.c_single, p.alpha = g.alpha, p.beta = g.beta;
-  // (Smaller tiles with two workgroups to a compute unit are slower at every length, short ones among them: us, 256 x 256 / 128 x 128, 64 groups of 2048 x 1408 with 96 rows on average 165 / 217.)
-  return grouped_over_indexed<DT, 256, 256, 8, 2>(g, p);
+  p.parts = 1;
+  // Tiles of 256 x 256 where they fill half the chip. (Smaller ones with two workgroups to a compute unit are slower at every length, short ones among them: us, 256 x 256 / 128 x 128,
+  // 64 groups of 2048 x 1408 with 96 rows on average 165 / 217.) Fewer of them share out their rows among workgroups, if there are enough, or are 128 x 128, or both; the parts meet in scratch
+  // memory. us, 256 x 256 / the same with parts / 128 x 128 / the same with parts: 4 groups of 1024 x 1024 with 32768 rows 284 / 107 / 157 / 132, 2 of 1024 x 4096 with 16384 239 / 157 / - / -,
+  // 2 of 512 x 256 with 32768 356 / 62 / 197 / 32, 16 of 256 x 512 with 32000 106 / 79 / 60 / 37, 3 of 1152 x 832 with 1002 21 / 29 / 11 / 23, 2 of 512 x 512 with 64 12.4 / - / 6.6 / -.
+  const size_t tiles = g.groups * skl_div_up(g.m, 256) * skl_div_up(g.n, 256), each = g.total / g.groups;
+  if (tiles > 128) return grouped_over_indexed<DT, 256, 256, 8, 2>(g, p);
+  const size_t small = g.groups * skl_div_up(g.m, 128) * skl_div_up(g.n, 128);
+  size_t parts = 256 / tiles < each / 1024 ? 256 / tiles : each / 1024;
+  const bool large = tiles == 128 || (tiles >= 64 && parts >= 2);
+  if (!large) parts = 512 / small < each / 256 ? 512 / small : each / 256;
+  const size_t one = g.groups * g.m * g.n * 4, most = (size_t(1) << 26) / one < 64 ? (size_t(1) << 26) / one : 64;  // the workspace's 64 MiB
+  if (parts > most) parts = most;
+  const bool sequence = parts >= 2;
+  if (sequence) {
+    skl_hip_sequence_begin();
+    p.c = (char *)skl_workspace(parts * one, true);
+    if (p.c) p.parts = (unsigned)parts;  // no scratch memory: in one part
+  }
+  const int rc = large ? grouped_over_indexed<DT, 256, 256, 8, 2>(g, p) : grouped_over_indexed<DT, 128, 128, 8, 2>(g, p);
+  if (sequence) skl_hip_sequence_end();
+  return rc;
 }
 
 }  // namespace

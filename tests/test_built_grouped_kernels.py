@@ -23,7 +23,7 @@ def kernels(code_objects):  # noqa: F811
             name = re.match(r"[0-9a-f]{16} <([^>]*)>:", part)
             if name and GROUPED.search(name.group(1)):
                 out[name.group(1)] = [line.split("//")[0].strip() for line in part.split("\n")[1:] if line.startswith("\t")]
-    assert len(out) == 20  # two types: three sizes of tile for two layouts of B; four ways of sums
+    assert len(out) == 28  # two types: three sizes of tile for two layouts of B; four ways of sums in two sizes
     return out
 
 

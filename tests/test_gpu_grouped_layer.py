@@ -302,7 +302,7 @@ def test_two_streams_at_once(gpu, hip):
 
 
 def test_without_a_scratch_slot(gpu, hip):
-    """A stream beyond those that hold scratch memory: the order comes from one workgroup, and is the same."""
+    """A stream beyond those that hold scratch memory: the order comes from one workgroup, and is the same; gradients of few weights are summed in one part, which is another order."""
     work = Pass(4)
     gpu.skl_hip_set_pointer_mode(1)
     streams = []
@@ -317,6 +317,16 @@ def test_without_a_scratch_slot(gpu, hip):
         work.enqueue(gpu)
         got = work.take(gpu)
         assert gpu.skl_hip_last_error() == 0
+        L = work.layer
+        n, rows = int(want["offsets"].view(np.int32)[-1]), want["rows"].view(np.int32)
+        ranges = gs.cut(want["offsets"].view(np.int32), L.picks, L.experts)
+        load = lambda buf, cols: gs.values(buf.download(np.uint16).reshape(-1, cols), "bf16")  # noqa: E731
+        index = np.append(rows[:n], np.full(L.picks - n, -1))
+        sums = {"dup": gs.over(load(L.dpre, L.inter), load(L.x, L.hidden), np.zeros((L.experts, L.inter, L.hidden)), 1.0, 0.0, ranges, None, index, total=L.picks),
+                "ddown": gs.over(load(L.dout, L.hidden), load(L.act, L.inter), np.zeros((L.experts, L.hidden, L.inter)), 1.0, 0.0, ranges, total=L.picks)}
+        for name, (exact, bound) in sums.items():
+            for side in (got, want):
+                assert np.all(np.abs(side.pop(name).view(np.float32).reshape(exact.shape) - exact) <= bound), name
         same(got, want)
     finally:
         gpu.skl_hip_set_stream(None)

@@ -85,6 +85,27 @@ def test_sums_of_every_length(gpu, kind, indexed):
     run_groupedk(gpu, kind, kind, 264, 256, total, offsets_of(LENGTHS, 3), len(LENGTHS), index[0], 90 if indexed[0] else 0, index[1], 90 if indexed[1] else 0, alpha=-2.0, beta=0.5, pads=(0, 8, 4), seed=9)
 
 
+# (m, n, lengths of the groups): few tiles with many rows, whose sums are taken in parts of 256 x 256 and of 128 x 128 tiles, or in one of the latter
+IN_PARTS = ((264, 264, [700, 0, 333, 1, 65, 5000]), (128, 128, [3000]), (520, 1000, [2100, 2100, 2100, 2100, 2100, 0, 6000, 64]), (100, 300, [0, 0, 1300, 20, 257]), (72, 80, [12000, 1]),
+            (520, 264, [40, 100, 3]))
+
+
+@pytest.mark.parametrize("indexed", ((False, False), (True, True)), ids=str)
+@pytest.mark.parametrize("m,n,lengths", IN_PARTS, ids=str)
+def test_sums_in_parts(gpu, m, n, lengths, indexed):
+    total = sum(lengths) + 5
+    rng = np.random.default_rng(total)
+    index = [rng.integers(-1, 90, total) if i else None for i in indexed]
+    rows = [90 if i else 0 for i in indexed]
+    for kind, out, alpha, beta in (("bf16", "f32", 1.0, 0.0), ("f16", "f16", 0.5, -1.0), ("bf16", "bf16", 1.0, 0.0), ("f16", "f32", -1.0, 2.0)):
+        run_groupedk(gpu, kind, out, m, n, total, offsets_of(lengths, 3), len(lengths), index[0], rows[0], index[1], rows[1], alpha=alpha, beta=beta, pads=(-m % 8, -n % 8, 4), seed=m)
+
+
+def test_the_same_bits_of_sums_in_parts(gpu):
+    first, second = (run_groupedk(gpu, "bf16", "f32", 256, 256, 9000, offsets_of([4000, 5000]), 2, seed=5) for _ in range(2))
+    assert np.array_equal(first.view(np.uint32), second.view(np.uint32))
+
+
 def test_few_columns_of_a_sum(gpu):
     """Fewer than the eight values that are loaded at once."""
     for m, n in ((1, 7), (7, 1), (8, 7), (7, 200), (200, 3), (9, 9)):
