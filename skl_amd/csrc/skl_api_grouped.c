@@ -113,7 +113,7 @@ static void stage_rows(staged *s, const skl_grouped_gemm *g, skl_grouped_gemm *d
 
 static void grouped(skl_grouped_gemm g, const char *who) {
   const size_t k = g.k;
-  const void *given[5] = {g.offsets, k ? g.a : NULL, k ? g.rows : NULL, k ? g.b : NULL, g.c};
+  const void *given[5] = {g.offsets, g.a, g.rows, k ? g.b : NULL, g.c};
   int where;
   if (g.m == 0 || g.n == 0 || g.groups == 0) return; /* nothing is addressed */
   if (!rows_ok(&g) || (k && !g.b)) {
@@ -142,7 +142,7 @@ static skl_grouped_gemm grouped_problem(int dt, int c_single, size_t groups, con
   skl_grouped_gemm g;
   memset(&g, 0, sizeof g);
   g.dt = dt, g.c_single = c_single, g.groups = groups, g.offsets = offsets, g.m = m, g.n = n, g.k = k;
-  g.a = a, g.rsa = rsa, g.rows = rows, g.a_rows = a_rows, g.c = c, g.rsc = rsc;
+  g.a = k ? a : NULL, g.rsa = rsa, g.rows = k ? rows : NULL, g.a_rows = a_rows, g.c = c, g.rsc = rsc; /* k == 0: kernels look rows up all the same */
   g.alpha = alpha_of(alpha), g.beta = beta_of(beta);
   return g;
 }
@@ -241,7 +241,7 @@ static void grouped_u4(skl_grouped_gemm g, const skl_gfx950_u4_t *b, const char 
     u.scales = b->scales, u.zeros = b->zeros, u.ld_scales = b->ld_scales, u.expert_scales = b->expert_scales;
   }
   {
-    const void *given[7] = {g.offsets, k ? g.a : NULL, k ? g.rows : NULL, u.codes, u.scales, u.zeros, g.c};
+    const void *given[7] = {g.offsets, g.a, g.rows, u.codes, u.scales, u.zeros, g.c};
     where = skl_classify(given, 7, who);
   }
   if (where < 0) return;
