@@ -500,8 +500,8 @@ void skl_group_rows_gfx950(size_t count, const int32_t *ids, size_t per_row, siz
  * offsets have to ascend; they are cut off at 0 and m, nothing outside C's m rows is written whatever they are, and which of its rows are written is open where
  * they do not ascend. offsets may be NULL with groups == 1: all m rows are the group. groups is 1 to 4096; m, n, k and a_rows are at most 2^30.
  * Products are exact, sums in fp32 on the matrix cores, the result rounded once where C has 16 bits. The order of a sum depends on k and the layouts and, through the
- * tiles chosen, on groups, m and n, not on the offsets' values: the same call gives the same bits. k == 0: C = beta * C on the groups' rows. beta == 0 leaves C unread
- * (an old C counts as +0) unless skl_hip_set_beta_zero_mode asks for the reference's evaluation. C overlaps neither A nor B. */
+ * tiles chosen, on groups, m and n, not on the offsets' values: the same call gives the same bits. k == 0, or an index into an A of no rows (a_rows == 0): C = beta * C on the groups'
+ * rows, neither A, B nor rows is read. beta == 0 leaves C unread (an old C counts as +0) unless skl_hip_set_beta_zero_mode asks for the reference's evaluation. C overlaps neither A nor B. */
 void skl_gemm_grouped_bf16_bf16rc_f32_gfx950(size_t groups, const int32_t *offsets, size_t m, size_t n, size_t k, float alpha, const skl_bf16_t *a,
                                              size_t rsa, const int32_t *rows, size_t a_rows, const skl_bf16_t *b, size_t rsb, size_t csb, size_t gsb,
                                              float beta, float *c, size_t rsc);
@@ -517,7 +517,7 @@ void skl_gemm_grouped_f16_f16rc_f16_gfx950(size_t groups, const int32_t *offsets
 
 /* C_e[i][j] = alpha * sum_r A[ra(r)][i] * B[rb(r)][j] + beta * C_e[i][j], the sum over the rows r of group e: the gradient of such a layer's weights,
  * dW_e = dY^T X with A = dY, B = X. A has m columns and B n, both row-major; ra(r) = rows_a[r], or r where rows_a is NULL, likewise rb; of `total` rows in all
- * (offsets are cut off at 0 and total; rows_a == NULL: A has them all). C_e(i, j) at c[e * gsc + i * rsc + j]. An empty group makes C_e = beta * C_e. Everything else as above:
+ * (offsets are cut off at 0 and total; rows_a == NULL: A has them all). C_e(i, j) at c[e * gsc + i * rsc + j]. An empty group makes C_e = beta * C_e, and so does an index into an operand of no rows. Everything else as above:
  * a row whose index is outside [0, a_rows) or [0, b_rows) counts as zeros, offsets may be NULL with groups == 1, total is at most 2^30. A sum is taken in the order of its
  * rows' places; where C has few values and groups many rows, in parts, by m, n, groups and total and by whether the stream holds scratch memory. */
 void skl_gemm_groupedk_bf16c_bf16_f32_gfx950(size_t groups, const int32_t *offsets, size_t m, size_t n, size_t total, float alpha, const skl_bf16_t *a,

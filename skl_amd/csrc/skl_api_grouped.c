@@ -111,16 +111,24 @@ static void stage_rows(staged *s, const skl_grouped_gemm *g, skl_grouped_gemm *d
   d->c = stage(s, g->c, bytes_of_c(g)); /* its whole span travels both ways: what no group covers comes back unchanged */
 }
 
+/* With k == 0, or an A of no rows, sums are empty: nothing is read but the offsets and C. (Kernels look rows up whatever k is.) */
+static void no_operands_of_empty_sums(skl_grouped_gemm *g) {
+  if (g->rows && g->a_rows == 0) g->k = 0;
+  if (g->k == 0) g->a = NULL, g->rows = NULL, g->b = NULL;
+}
+
 static void grouped(skl_grouped_gemm g, const char *who) {
-  const size_t k = g.k;
-  const void *given[5] = {g.offsets, g.a, g.rows, k ? g.b : NULL, g.c};
   int where;
   if (g.m == 0 || g.n == 0 || g.groups == 0) return; /* nothing is addressed */
-  if (!rows_ok(&g) || (k && !g.b)) {
+  if (!rows_ok(&g) || (g.k && !g.b)) {
     bad_argument(who);
     return;
   }
-  where = skl_classify(given, 5, who);
+  no_operands_of_empty_sums(&g);
+  {
+    const void *given[5] = {g.offsets, g.a, g.rows, g.b, g.c};
+    where = skl_classify(given, 5, who);
+  }
   if (where < 0) return;
   if (where == 1) {
     skl_hip_launch_gemm_grouped(&g);
@@ -131,7 +139,7 @@ static void grouped(skl_grouped_gemm g, const char *who) {
     skl_grouped_gemm d;
     memset(&s, 0, sizeof s);
     stage_rows(&s, &g, &d);
-    d.b = k ? stage(&s, g.b, ((g.groups - 1) * g.gsb + (k - 1) * g.rsb + (g.n - 1) * g.csb + 1) * 2) : NULL;
+    d.b = g.k ? stage(&s, g.b, ((g.groups - 1) * g.gsb + (g.k - 1) * g.rsb + (g.n - 1) * g.csb + 1) * 2) : NULL;
     if (!s.failed && skl_hip_launch_gemm_grouped(&d) == 0) skl_hip_memcpy_d2h(g.c, d.c, bytes_of_c(&g));
     unstage(&s);
   }
@@ -142,7 +150,7 @@ static skl_grouped_gemm grouped_problem(int dt, int c_single, size_t groups, con
   skl_grouped_gemm g;
   memset(&g, 0, sizeof g);
   g.dt = dt, g.c_single = c_single, g.groups = groups, g.offsets = offsets, g.m = m, g.n = n, g.k = k;
-  g.a = k ? a : NULL, g.rsa = rsa, g.rows = k ? rows : NULL, g.a_rows = a_rows, g.c = c, g.rsc = rsc; /* k == 0: kernels look rows up all the same */
+  g.a = a, g.rsa = rsa, g.rows = rows, g.a_rows = a_rows, g.c = c, g.rsc = rsc;
   g.alpha = alpha_of(alpha), g.beta = beta_of(beta);
   return g;
 }
@@ -165,16 +173,19 @@ SKL_GROUPED(skl_gemm_grouped_f16_f16rc_f16_gfx950, SKL_DT_F16, skl_f16_t, 0, skl
 /* ------------------------------------------------------------------------ */
 
 static void groupedk(skl_groupedk_gemm g, const char *who) {
-  const size_t total = g.total;
-  const void *given[6] = {g.offsets, total ? g.a : NULL, total ? g.b : NULL, total ? g.rows_a : NULL, total ? g.rows_b : NULL, g.c};
   int where;
   if (g.m == 0 || g.n == 0 || g.groups == 0) return; /* nothing is addressed */
-  if (!groups_ok(g.groups, g.offsets) || g.m > MOST_ROWS || g.n > MOST_ROWS || total > MOST_ROWS || g.a_rows > MOST_ROWS || g.b_rows > MOST_ROWS || !g.c ||
-      (g.m > 1 && g.rsc < g.n) || (g.groups > 1 && g.gsc < span(g.m, g.rsc, g.n)) || (total && ((!g.a && !(g.rows_a && g.a_rows == 0)) || (!g.b && !(g.rows_b && g.b_rows == 0))))) {
+  if (!groups_ok(g.groups, g.offsets) || g.m > MOST_ROWS || g.n > MOST_ROWS || g.total > MOST_ROWS || g.a_rows > MOST_ROWS || g.b_rows > MOST_ROWS || !g.c ||
+      (g.m > 1 && g.rsc < g.n) || (g.groups > 1 && g.gsc < span(g.m, g.rsc, g.n)) || (g.total && ((!g.a && !(g.rows_a && g.a_rows == 0)) || (!g.b && !(g.rows_b && g.b_rows == 0))))) {
     bad_argument(who);
     return;
   }
-  where = skl_classify(given, 6, who);
+  if ((g.rows_a && g.a_rows == 0) || (g.rows_b && g.b_rows == 0)) g.total = 0; /* an operand of no rows: every sum is empty */
+  if (g.total == 0) g.a = g.b = NULL, g.rows_a = g.rows_b = NULL;
+  {
+    const void *given[6] = {g.offsets, g.a, g.b, g.rows_a, g.rows_b, g.c};
+    where = skl_classify(given, 6, who);
+  }
   if (where < 0) return;
   if (where == 1) {
     skl_hip_launch_gemm_groupedk(&g);
@@ -186,10 +197,10 @@ static void groupedk(skl_groupedk_gemm g, const char *who) {
     staged s;
     memset(&s, 0, sizeof s);
     d.offsets = (const int32_t *)stage(&s, g.offsets, (g.groups + 1) * sizeof(int32_t));
-    d.a = total ? stage(&s, g.a, span(g.rows_a ? g.a_rows : total, g.rsa, g.m) * 2) : NULL;
-    d.b = total ? stage(&s, g.b, span(g.rows_b ? g.b_rows : total, g.rsb, g.n) * 2) : NULL;
-    d.rows_a = (const int32_t *)stage(&s, g.rows_a, total * sizeof(int32_t));
-    d.rows_b = (const int32_t *)stage(&s, g.rows_b, total * sizeof(int32_t));
+    d.a = stage(&s, g.a, span(g.rows_a ? g.a_rows : g.total, g.rsa, g.m) * 2);
+    d.b = stage(&s, g.b, span(g.rows_b ? g.b_rows : g.total, g.rsb, g.n) * 2);
+    d.rows_a = (const int32_t *)stage(&s, g.rows_a, g.total * sizeof(int32_t));
+    d.rows_b = (const int32_t *)stage(&s, g.rows_b, g.total * sizeof(int32_t));
     d.c = stage(&s, g.c, nc);
     if (!s.failed && skl_hip_launch_gemm_groupedk(&d) == 0) skl_hip_memcpy_d2h(g.c, d.c, nc);
     unstage(&s);
@@ -225,18 +236,18 @@ static int u4_ok(const skl_gfx950_u4_t *b, size_t groups, size_t n, size_t k) {
 }
 
 static void grouped_u4(skl_grouped_gemm g, const skl_gfx950_u4_t *b, const char *who) {
-  const size_t k = g.k;
   skl_grouped_u4 u;
   int where;
   if (g.m == 0 || g.n == 0 || g.groups == 0) return; /* nothing is addressed */
-  if (!rows_ok(&g) || (k && !u4_ok(b, g.groups, g.n, k))) {
+  if (!rows_ok(&g) || (g.k && !u4_ok(b, g.groups, g.n, g.k))) {
     bad_argument(who);
     return;
   }
+  no_operands_of_empty_sums(&g);
   memset(&u, 0, sizeof u);
   u.g = g;
-  if (k) {
-    u.group_k = b->group_k < k ? b->group_k : k;
+  if (g.k) {
+    u.group_k = b->group_k < g.k ? b->group_k : g.k;
     u.codes = b->codes, u.ld = b->ld, u.expert = b->expert;
     u.scales = b->scales, u.zeros = b->zeros, u.ld_scales = b->ld_scales, u.expert_scales = b->expert_scales;
   }
@@ -254,9 +265,9 @@ static void grouped_u4(skl_grouped_gemm g, const skl_gfx950_u4_t *b, const char 
     staged s;
     memset(&s, 0, sizeof s);
     stage_rows(&s, &g, &d.g);
-    if (k) {
-      const size_t blocks = (k + u.group_k - 1) / u.group_k, places = span(g.groups, u.expert_scales, span(g.n, u.ld_scales, blocks));
-      d.codes = (const uint8_t *)stage(&s, u.codes, span(g.groups, u.expert / 2, span(g.n, u.ld / 2, (k + 1) / 2)));
+    if (g.k) {
+      const size_t blocks = (g.k + u.group_k - 1) / u.group_k, places = span(g.groups, u.expert_scales, span(g.n, u.ld_scales, blocks));
+      d.codes = (const uint8_t *)stage(&s, u.codes, span(g.groups, u.expert / 2, span(g.n, u.ld / 2, (g.k + 1) / 2)));
       d.scales = stage(&s, u.scales, places * 2);
       d.zeros = (const uint8_t *)stage(&s, u.zeros, places);
     }

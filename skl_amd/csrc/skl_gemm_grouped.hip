@@ -146,9 +146,7 @@ __global__ void __launch_bounds__(256, 2) gemm_grouped_kernel(GroupedArgs p) {
     if (at.none) return;
     e = at.e, first = at.first, rows = at.rows, col0 = at.tile_n * kEdge;
   }
-  // an operand without rows counts as zeros
-  const bool none = (p.rows_a && p.a_rows == 0) || (OVER && p.rows_b && p.b_rows == 0);
-  const unsigned k = none ? 0u : OVER ? rows : p.k;
+  const unsigned k = OVER ? rows : p.k;
   const uint16_t *const b = OVER ? p.b : p.b + (size_t)e * p.gsb;
   TA ta;
   TB tb;

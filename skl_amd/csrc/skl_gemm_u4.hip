@@ -196,8 +196,7 @@ __global__ void __launch_bounds__(WAVES * 64, MIN) gemm_u4_stream_kernel(U4Args 
   for (int f = 0; f < F; ++f) code_at[f] = (16 * f + l < cols ? 16 * f + l : cols - 1) * (unsigned)(p.ld / 2);  // (ld below 2^25, see the launch)
   const size_t scale_base = (size_t)e * p.expert_scales + (size_t)col0 * p.ld_scales;
   const bool read_c = !skl_beta_is_zero<float>(p.beta);
-  const unsigned limit = p.rows ? p.a_rows : p.m;  // an A without rows: nothing to multiply
-  const unsigned chunks = limit == 0 ? 0 : (p.k + kChunk - 1) / kChunk;
+  const unsigned limit = p.rows ? p.a_rows : p.m, chunks = (p.k + kChunk - 1) / kChunk;
 
   struct Codes {
     v4i v[F];

@@ -21,7 +21,7 @@ extern "C" {
 int skl_hip_launch_group_rows(size_t count, const int32_t *ids, size_t per_row, size_t groups, int32_t *offsets, int32_t *order, int32_t *rows,
                               int32_t *place);
 
-/* C (m x n, row-major) = alpha * A[rows] * B_e + beta * C, by groups of rows. m, n > 0; k may be 0. */
+/* C (m x n, row-major) = alpha * A[rows] * B_e + beta * C, by groups of rows. m, n > 0; k may be 0, with a, rows and b NULL; an A that `rows` points into has a row. */
 typedef struct {
   int dt;       /* SKL_DT_BF16 or SKL_DT_F16 */
   int c_single; /* C is fp32, else as A */
@@ -40,7 +40,7 @@ typedef struct {
 } skl_grouped_gemm;
 int skl_hip_launch_gemm_grouped(const skl_grouped_gemm *g);
 
-/* C_e (m x n) = alpha * A[rows_a]^T B[rows_b] + beta * C_e, the sum over group e's rows. m, n > 0. */
+/* C_e (m x n) = alpha * A[rows_a]^T B[rows_b] + beta * C_e, the sum over group e's rows. m, n > 0; total may be 0, likewise; operands have rows otherwise. */
 typedef struct {
   int dt, c_single;
   size_t groups;

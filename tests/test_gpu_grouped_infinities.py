@@ -1,0 +1,56 @@
+"""Products grouped by expert where the values that rows meet are infinite: the same result whatever layout, alignment and kernel the operands have. All sums are of whole numbers
+of few bits or not finite, so every result is exact."""
+import numpy as np
+import pytest
+
+import grouped_support as gs
+import skl_amd
+from skl_amd import DeviceBuffer, U4Weights
+from test_gpu_gemm_grouped import strided
+
+pytestmark = pytest.mark.gpu
+
+INF = {"bf16": 0x7F80, "f16": 0x7C00}
+
+
+def download(lib, buf, *shape):
+    assert lib.skl_hip_synchronize() == 0
+    skl_amd.check_error()
+    return buf.download(np.float32).reshape(shape)
+
+
+# On 16-byte boundaries, where the streaming kernels run, and off them.
+@pytest.mark.parametrize("pad", (8, 1))
+@pytest.mark.parametrize("kind", ("bf16", "f16"))
+def test_an_operand_without_rows(gpu, kind, pad):
+    """An index into an A (or B) of no rows: nothing is multiplied, C = beta C, infinities in the other operand or not."""
+    m, n, k = 70, 72, 64
+    index, offsets = DeviceBuffer.from_array(np.zeros(m, np.int32)), DeviceBuffer.from_array(np.array([0, 30, 65], np.int32))
+    other = DeviceBuffer.from_array(np.full((2 * n + m) * (n + pad), INF[kind], np.uint16))
+    c = DeviceBuffer(4 * 2 * 72 * n)
+    old = np.full(2 * 72 * n, 4.0, np.float32)
+    grouped, over = (getattr(gpu, f"skl_gemm_grouped_{kind}_{kind}rc_f32_gfx950"), getattr(gpu, f"skl_gemm_groupedk_{kind}c_{kind}_f32_gfx950"))
+    for strides in ((1, k + pad), (n + pad, 1)):
+        c.upload(old)
+        grouped(2, offsets, m, n, k, 1.0, None, k + pad, index, 0, other, *strides, n * (k + pad), 0.5, c, n)
+        got = download(gpu, c, 2 * 72, n)
+        assert np.all(got[:65] == 2.0) and np.all(got[65:] == 4.0), strides
+    for rows in (("a",), ("b",), ("a", "b")):
+        c.upload(old)
+        a = (None, k + pad, index, 0) if "a" in rows else (other, k + pad, None, 0)
+        b = (None, n + pad, index, 0) if "b" in rows else (other, n + pad, None, 0)
+        over(2, offsets, k, n, m, 1.0, *a, *b, 0.5, c, n, 72 * n)
+        got = download(gpu, c, 2, 72, n)
+        assert np.all(got[:, :k] == 2.0) and np.all(got[:, k:] == 4.0), rows
+
+
+@pytest.mark.parametrize("shift", (0, 1))
+@pytest.mark.parametrize("m", (1, 3, 40))
+def test_an_operand_without_rows_and_4_bit_weights(gpu, m, shift):
+    n, k = 40, 64
+    index = DeviceBuffer.from_array(np.zeros(m, np.int32))
+    codes, scales = DeviceBuffer.from_array(np.full(n * k // 2 + 16, 0x33, np.uint8)), DeviceBuffer.from_array(np.full(n * 2, INF["bf16"], np.uint16))
+    c = DeviceBuffer.from_array(np.full(m * n, 4.0, np.float32))
+    w = U4Weights(group_k=32, codes=codes.offset(shift), ld=k, expert=0, scales=scales, zeros=None, ld_scales=2, expert_scales=0)
+    gpu.skl_gemm_grouped_bf16_u4c_f32_gfx950(1, None, m, n, k, 1.0, None, k, index, 0, w, 0.5, c, n)
+    assert np.all(download(gpu, c, m, n) == 2.0)
