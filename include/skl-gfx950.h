@@ -496,7 +496,7 @@ void skl_group_rows_gfx950(size_t count, const int32_t *ids, size_t per_row, siz
 /* C[i][j] = alpha * sum_p A[r(i)][p] * B_e[p][j] + beta * C[i][j] for the rows i of every group e; r(i) = rows[i], or i where rows is NULL.
  * A is row-major, `a_rows` rows (rows == NULL: m) rsa apart; B_e(p, j) at b[e * gsb + p * rsb + j * csb], any strides; C is row-major, m rows rsc apart. With
  * weights W_e [out][in] a layer's output takes rsb = 1, csb = in; the gradient of its input, dX = dY W_e, takes rsb = in, csb = 1 (k = out, n = in).
- * Rows of C in no group are left as they were. A row whose index is outside [0, a_rows) counts as zeros; the same index may come any number of times.
+ * Rows of C in no group are left as they were. A row whose index is outside [0, a_rows) counts as zeros, which an infinity in B makes NaN; the same index may come any number of times.
  * offsets have to ascend; they are cut off at 0 and m, nothing outside C's m rows is written whatever they are, and which of its rows are written is open where
  * they do not ascend. offsets may be NULL with groups == 1: all m rows are the group. groups is 1 to 4096; m, n, k and a_rows are at most 2^30.
  * Products are exact, sums in fp32 on the matrix cores, the result rounded once where C has 16 bits. The order of a sum depends on k and the layouts and, through the
@@ -548,7 +548,7 @@ typedef struct skl_gfx950_u4 {
 } skl_gfx950_u4_t;
 /* C = alpha * A * B_e + beta * C with such a B, the rest as in skl_gemm_grouped_bf16_bf16rc_f32_gfx950; groups == 1 and offsets == NULL is an ordinary layer. q - z is
  * an integer that bf16 and f16 hold, its products with A are exact, they are summed in fp32 over at most 128 values of one group, and those sums are scaled and added up in fp32.
- * (An infinite scale thus meets the sum, not each product: no NaN from a code that equals its zero point.)
+ * (An infinite scale thus meets the sum, not each product: no NaN from a code that equals its zero point. A row whose index is outside A has none that a scale could meet: 0 whatever the scales are.)
  * Made for few rows: an expert's codes are read once for up to 4, 16 or 32 of its rows, by how many there are on average; more rows take more passes over them. */
 void skl_gemm_grouped_bf16_u4c_f32_gfx950(size_t groups, const int32_t *offsets, size_t m, size_t n, size_t k, float alpha, const skl_bf16_t *a, size_t rsa,
                                           const int32_t *rows, size_t a_rows, const skl_gfx950_u4_t *b, float beta, float *c, size_t rsc);

@@ -88,7 +88,8 @@ __global__ void __launch_bounds__(256) gemm_u4_any_kernel(U4Args p) {
       const unsigned at = row0 + 4 * part + i;
       if (at >= r.rows) continue;
       TC *const to = c + (size_t)at * p.rsc;
-      *to = skl_grouped_result(sum[i], to, p.alpha, p.beta, read_c);
+      const bool outside = p.rows && (unsigned)p.rows[r.first + at] >= p.a_rows;  // no scale meets its zeros: 0, if it is infinite, too
+      *to = skl_grouped_result(outside ? 0.0f : sum[i], to, p.alpha, p.beta, read_c);
     }
   }
 }
@@ -323,7 +324,7 @@ __global__ void __launch_bounds__(WAVES * 64, MIN) gemm_u4_stream_kernel(U4Args 
 #pragma unroll
       for (unsigned w = 0; w < kWaves; ++w) v = __fadd_rn(v, sums[w][row][c]);
       const unsigned out = range.first + row0 + row;
-      if (p.rows && (unsigned)p.rows[out] >= limit) v = 0.0f;
+      if (p.rows && (unsigned)p.rows[out] >= limit) v = 0.0f;  // what was computed is A's first row's
       const size_t at = (size_t)out * p.rsc + col0 + c;
       if (c_single) {
         float *const to = reinterpret_cast<float *>(p.c) + at;

@@ -54,3 +54,45 @@ def test_an_operand_without_rows_and_4_bit_weights(gpu, m, shift):
     w = U4Weights(group_k=32, codes=codes.offset(shift), ld=k, expert=0, scales=scales, zeros=None, ld_scales=2, expert_scales=0)
     gpu.skl_gemm_grouped_bf16_u4c_f32_gfx950(1, None, m, n, k, 1.0, None, k, index, 0, w, 0.5, c, n)
     assert np.all(download(gpu, c, m, n) == 2.0)
+
+
+@pytest.mark.parametrize("pad", (8, 1))
+@pytest.mark.parametrize("m", (2, 30, 300))
+def test_a_row_outside_meets_infinite_weights(gpu, m, pad):
+    """A row whose index is outside A is a row of zeros: NaN where a weight is infinite, 0 elsewhere."""
+    n, k = 72, 64
+    index, outside = np.arange(m) % 5, np.arange(1, m, 3)
+    index[outside] = np.resize([-1, 5, 2 ** 31 - 1, -2 ** 31], len(outside))
+    w = np.ones((n, k), np.float32)
+    w[::4, 7] = np.inf
+    a, b = strided(gs.bits(np.ones((5, k)), "bf16"), k + pad, 0), strided(gs.bits(w, "bf16"), k + pad, 0)
+    da, db, di, c = DeviceBuffer.from_array(a), DeviceBuffer.from_array(b), DeviceBuffer.from_array(index.astype(np.int32)), DeviceBuffer(4 * m * n)
+    gpu.skl_gemm_grouped_bf16_bf16rc_f32_gfx950(1, None, m, n, k, 1.0, da, k + pad, di, 5, db, 1, k + pad, 0, 0.0, c, n)
+    got = download(gpu, c, m, n)
+    want = np.full((m, n), 64.0)
+    want[:, ::4], want[outside] = np.inf, 0.0
+    want[outside, ::4] = np.nan
+    assert np.array_equal(got, want, equal_nan=True)
+
+
+@pytest.mark.parametrize("shift", (0, 1))
+@pytest.mark.parametrize("kind", ("bf16", "f16"))
+@pytest.mark.parametrize("k,group_k", [(64, 32), (192, 64), (256, 128), (96, 96)])
+@pytest.mark.parametrize("m,n", [(1, 40), (2, 33), (30, 72), (300, 40)])
+def test_a_row_outside_meets_infinite_scales(gpu, m, n, k, group_k, kind, shift):
+    """With 4-bit weights, whose scales meet sums, such a row has none: 0, infinite scales or not - from the stream over the codes and, with codes off 16-byte boundaries, from the kernel
+    for any layout."""
+    blocks = -(-k // group_k)
+    index, outside = np.arange(m) % 5, np.arange(min(1, m - 1), m, 3)
+    index[outside] = np.resize([-1, 5, 2 ** 31 - 1, -2 ** 31], len(outside))
+    scales = np.ones((n, blocks), np.float32)
+    scales[::4, blocks // 2] = np.inf
+    codes = np.concatenate([np.zeros(shift, np.uint8), gs.u4_store(np.full((n, k), 9, np.uint8), k)])
+    da, di, dc, ds = (DeviceBuffer.from_array(v) for v in (gs.bits(np.ones((5, k)), kind), index.astype(np.int32), codes, gs.bits(scales, kind)))
+    c = DeviceBuffer(4 * m * n)
+    w = U4Weights(group_k=group_k, codes=dc.offset(shift), ld=k, expert=0, scales=ds, zeros=None, ld_scales=blocks, expert_scales=0)
+    getattr(gpu, f"skl_gemm_grouped_{kind}_u4c_f32_gfx950")(1, None, m, n, k, 1.0, da, k, di, 5, w, 0.0, c, n)
+    got = download(gpu, c, m, n)
+    want = np.full((m, n), float(k))
+    want[:, ::4], want[outside] = np.inf, 0.0
+    assert np.array_equal(got, want)
