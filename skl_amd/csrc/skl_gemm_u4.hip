@@ -62,11 +62,11 @@ __global__ void __launch_bounds__(256) gemm_u4_any_kernel(U4Args p) {
       there = there && row < p.a_rows;
     }
     const uint16_t *const a = p.a + (size_t)(there ? row : 0u) * p.rsa;
-    v4f sum = {0, 0, 0, 0};
-    for (unsigned k0 = 0; k0 < p.k; k0 += 32) {
-      const unsigned block = k0 / p.group_k;  // the same for all 32
+    v4f sum = {0, 0, 0, 0}, part_sum = {0, 0, 0, 0};
+    for (unsigned k0 = 0, block = 0, end = p.group_k; k0 < p.k; k0 += 32) {  // end: of the group that all 32 are in
       Frag x, w;
       const int zero = p.zeros ? (int)p.zeros[first_scale + block] : 8;
+      const float scale = skl_widen(p.scales[first_scale + block], is_bf16<T>);
 #pragma unroll
       for (unsigned i = 0; i < 8; ++i) {
         const unsigned at = k0 + 8 * part + i;
@@ -76,10 +76,11 @@ __global__ void __launch_bounds__(256) gemm_u4_any_kernel(U4Args p) {
         const unsigned byte = in ? p.codes[(first_code + at) / 2] : 0u;
         w[i] = (T)(float)(in ? (int)((at & 1) ? byte >> 4 : byte & 15u) - zero : 0);
       }
-      const v4f part_sum = product<T>(__builtin_bit_cast(v4i, x), __builtin_bit_cast(v4i, w), v4f{0, 0, 0, 0});
-      const float scale = skl_widen(p.scales[first_scale + block], is_bf16<T>);
+      part_sum = product<T>(__builtin_bit_cast(v4i, x), __builtin_bit_cast(v4i, w), part_sum);
+      if (k0 + 32 < p.k && (k0 + 32) % 128 != 0 && k0 + 32 != end) continue;  // a scale meets what it meets in the stream below
 #pragma unroll
-      for (int i = 0; i < 4; ++i) sum[i] = __builtin_fmaf(part_sum[i], scale, sum[i]);
+      for (int i = 0; i < 4; ++i) sum[i] = __builtin_fmaf(part_sum[i], scale, sum[i]), part_sum[i] = 0.0f;
+      if (k0 + 32 == end) ++block, end += p.group_k;
     }
     if (col0 + l >= p.n) continue;
     TC *const c = reinterpret_cast<TC *>(p.c) + (size_t)r.first * p.rsc + col;

@@ -96,3 +96,23 @@ def test_a_row_outside_meets_infinite_scales(gpu, m, n, k, group_k, kind, shift)
     want = np.full((m, n), float(k))
     want[:, ::4], want[outside] = np.inf, 0.0
     assert np.array_equal(got, want)
+
+
+@pytest.mark.parametrize("shift", (0, 1))
+@pytest.mark.parametrize("kind", ("bf16", "f16"))
+@pytest.mark.parametrize("k,group_k", [(128, 128), (64, 64), (384, 384), (100, 200), (512, 256)])
+@pytest.mark.parametrize("m", (1, 3, 20))
+def test_an_infinite_scale_meets_the_sum_of_128_values(gpu, m, k, group_k, kind, shift):
+    """Every other 32 codes equal their zero point, so that their products are zeros: what an infinite scale meets is the sum of up to 128 values of the group, which is not."""
+    n, blocks = 33, -(-k // group_k)
+    q = np.full((n, k), 8, np.uint8)
+    q[:, 32:64], q[:, 96:128] = 9, 11
+    q[:, 128:] = 10
+    q[1::2] = 16 - q[1::2]
+    codes = np.concatenate([np.zeros(shift, np.uint8), gs.u4_store(q, k)])
+    da, dc, ds = (DeviceBuffer.from_array(v) for v in (gs.bits(np.ones((m, k)), kind), codes, np.full((n, blocks), INF[kind], np.uint16)))
+    c = DeviceBuffer(4 * m * n)
+    w = U4Weights(group_k=group_k, codes=dc.offset(shift), ld=k, expert=0, scales=ds, zeros=None, ld_scales=blocks, expert_scales=0)
+    getattr(gpu, f"skl_gemm_grouped_{kind}_u4c_f32_gfx950")(1, None, m, n, k, 1.0, da, k, None, 0, w, 0.0, c, n)
+    got = download(gpu, c, m, n)
+    assert np.all(got[:, 0::2] == np.inf) and np.all(got[:, 1::2] == -np.inf)
