@@ -517,7 +517,8 @@ void skl_gemm_grouped_f16_f16rc_f16_gfx950(size_t groups, const int32_t *offsets
 
 /* C_e[i][j] = alpha * sum_r A[ra(r)][i] * B[rb(r)][j] + beta * C_e[i][j], the sum over the rows r of group e: the gradient of such a layer's weights,
  * dW_e = dY^T X with A = dY, B = X. A has m columns and B n, both row-major; ra(r) = rows_a[r], or r where rows_a is NULL, likewise rb; of `total` rows in all
- * (offsets are cut off at 0 and total; rows_a == NULL: A has them all). C_e(i, j) at c[e * gsc + i * rsc + j]. An empty group makes C_e = beta * C_e, and so does an index into an operand of no rows. Everything else as above:
+ * (offsets are cut off at 0 and total; rows_a == NULL: A has them all). C_e(i, j) at c[e * gsc + i * rsc + j]: with more than one group the matrices one behind the other,
+ * gsc at least (m - 1) * rsc + n, or their rows side by side, gsc at least n and rsc at least (groups - 1) * gsc + n; others are refused. An empty group makes C_e = beta * C_e, and so does an index into an operand of no rows. Everything else as above:
  * a row whose index is outside [0, a_rows) or [0, b_rows) counts as zeros, offsets may be NULL with groups == 1, total is at most 2^30. A sum is taken in the order of its
  * rows' places; where C has few values and groups many rows, in parts, by m, n, groups and total and by whether the stream holds scratch memory. */
 void skl_gemm_groupedk_bf16c_bf16_f32_gfx950(size_t groups, const int32_t *offsets, size_t m, size_t n, size_t total, float alpha, const skl_bf16_t *a,

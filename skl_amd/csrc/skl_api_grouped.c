@@ -172,11 +172,16 @@ SKL_GROUPED(skl_gemm_grouped_f16_f16rc_f16_gfx950, SKL_DT_F16, skl_f16_t, 0, skl
 /* products summed over groups of rows                                       */
 /* ------------------------------------------------------------------------ */
 
+/* The groups' matrices lie one behind the other, or their rows side by side. */
+static int results_apart(const skl_groupedk_gemm *g) {
+  return g->groups == 1 || g->gsc >= span(g->m, g->rsc, g->n) || (g->gsc >= g->n && g->rsc >= span(g->groups, g->gsc, g->n));
+}
+
 static void groupedk(skl_groupedk_gemm g, const char *who) {
   int where;
   if (g.m == 0 || g.n == 0 || g.groups == 0) return; /* nothing is addressed */
   if (!groups_ok(g.groups, g.offsets) || g.m > MOST_ROWS || g.n > MOST_ROWS || g.total > MOST_ROWS || g.a_rows > MOST_ROWS || g.b_rows > MOST_ROWS || !g.c ||
-      (g.m > 1 && g.rsc < g.n) || (g.groups > 1 && g.gsc < span(g.m, g.rsc, g.n)) || (g.total && ((!g.a && !(g.rows_a && g.a_rows == 0)) || (!g.b && !(g.rows_b && g.b_rows == 0))))) {
+      (g.m > 1 && g.rsc < g.n) || !results_apart(&g) || (g.total && ((!g.a && !(g.rows_a && g.a_rows == 0)) || (!g.b && !(g.rows_b && g.b_rows == 0))))) {
     bad_argument(who);
     return;
   }
