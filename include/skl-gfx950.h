@@ -498,7 +498,8 @@ void skl_group_rows_gfx950(size_t count, const int32_t *ids, size_t per_row, siz
  * weights W_e [out][in] a layer's output takes rsb = 1, csb = in; the gradient of its input, dX = dY W_e, takes rsb = in, csb = 1 (k = out, n = in).
  * Rows of C in no group are left as they were. A row whose index is outside [0, a_rows) counts as zeros, which an infinity in B makes NaN; the same index may come any number of times.
  * offsets have to ascend; they are cut off at 0 and m, nothing outside C's m rows is written whatever they are, and which of its rows are written is open where
- * they do not ascend. offsets may be NULL with groups == 1: all m rows are the group. groups is 1 to 4096; m, n, k and a_rows are at most 2^30.
+ * they do not ascend. offsets may be NULL with groups == 1: all m rows are the group. groups is 1 to 4096; m, n, k and a_rows are at most 2^30. A call with m, n
+ * or groups == 0 does nothing.
  * Products are exact, sums in fp32 on the matrix cores, the result rounded once where C has 16 bits. The order of a sum depends on k and the layouts and, through the
  * tiles chosen, on groups, m and n, not on the offsets' values: the same call gives the same bits. k == 0, or an index into an A of no rows (a_rows == 0): C = beta * C on the groups'
  * rows, neither A, B nor rows is read. beta == 0 leaves C unread (an old C counts as +0) unless skl_hip_set_beta_zero_mode asks for the reference's evaluation. C overlaps neither A nor B. */
@@ -538,7 +539,8 @@ void skl_gemm_groupedk_f16c_f16_f16_gfx950(size_t groups, const int32_t *offsets
  *   (q - z) * s,   q   4-bit number e * expert + j * ld + p of `codes`, 0 to 15, two to a byte, the first in the low half,
  *                  s   scales[e * expert_scales + j * ld_scales + p / group_k], of A's type,
  *                  z   zeros at the same place, 0 to 255; zeros == NULL: 8.
- * group_k is a multiple of 32, or k or more; k need not be a multiple of it. ld and expert are even (where there is more than one row, or matrix). */
+ * group_k is a multiple of 32, or k or more; k need not be a multiple of it. ld and expert are even (where there is more than one row, or matrix); with more than one row, ld is at
+ * least k and ld_scales at least the number of groups of a row. */
 typedef struct skl_gfx950_u4 {
   size_t group_k;
   const uint8_t *codes;
@@ -550,7 +552,8 @@ typedef struct skl_gfx950_u4 {
 /* C = alpha * A * B_e + beta * C with such a B, the rest as in skl_gemm_grouped_bf16_bf16rc_f32_gfx950; groups == 1 and offsets == NULL is an ordinary layer. q - z is
  * an integer that bf16 and f16 hold, its products with A are exact, they are summed in fp32 over at most 128 values of one group, and those sums are scaled and added up in fp32.
  * (An infinite scale thus meets the sum, not each product: no NaN from a code that equals its zero point. A row whose index is outside A has none that a scale could meet: 0 whatever the scales are.)
- * Made for few rows: an expert's codes are read once for up to 4, 16 or 32 of its rows, by how many there are on average; more rows take more passes over them. */
+ * Made for few rows: an expert's codes are read once for up to 4, 16 or 32 of its rows, by how many there are on average; more rows take more passes over them, one after the other: the time of a
+ * prompt's products is that of its passes. */
 void skl_gemm_grouped_bf16_u4c_f32_gfx950(size_t groups, const int32_t *offsets, size_t m, size_t n, size_t k, float alpha, const skl_bf16_t *a, size_t rsa,
                                           const int32_t *rows, size_t a_rows, const skl_gfx950_u4_t *b, float beta, float *c, size_t rsc);
 void skl_gemm_grouped_bf16_u4c_bf16_gfx950(size_t groups, const int32_t *offsets, size_t m, size_t n, size_t k, float alpha, const skl_bf16_t *a, size_t rsa,
