@@ -98,7 +98,7 @@ __global__ void __launch_bounds__(256) gemm_u4_any_kernel(U4Args p) {
 // ---------------------------------------------------------------------------
 // The stream over the codes: rows of codes and of A on 16-byte boundaries, k a multiple of 32, group_k 32, 64 or a multiple of 128 (one group of all k
 // among them).
-// A workgroup of eight waves takes 16 F columns and all of k, in chunks: a wave UNITS units of 128 k of each, half a line of each column's codes, which go
+// A workgroup of four or eight waves takes 16 F columns and all of k, in chunks: a wave UNITS units of 128 k of each, half a line of each column's codes, which go
 // to registers a chunk ahead. ROWS rows of A and the columns' scales go to LDS, where all waves read them; in the end the waves' sums meet there.
 // ---------------------------------------------------------------------------
 

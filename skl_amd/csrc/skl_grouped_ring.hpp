@@ -1,5 +1,5 @@
 // skl_grouped_ring.hpp - the streaming kernel's way (skl_gemm_mfma_impl.hpp) with products grouped by expert: operands go from memory to LDS without registers, slices
-// of 64 bytes of K in a ring of four stages, the next slice's reads and a later one's requests dealt out behind the products of this one. What is different: which
+// of 64 bytes of K in a ring of four to eight stages, the next slice's reads and a later one's requests dealt out behind the products of this one. What is different: which
 // rows a tile has is known on the GPU alone, an operand's rows may come through an index, C has two types.
 //
 // A tile is 256, 128 or 64 rows by BN columns. What whole tiles of 256 rows leave of a group goes into the smallest tile that holds it: a group of

@@ -9,7 +9,7 @@
 #include "../../include/skl-hip.h"
 
 // The streaming kernels (skl_grouped_ring.hpp), and what they take: operands and the distances of their lines on 16-byte boundaries, whole 16 bytes of what lies
-// side by side along k, offsets in 32 bits.
+// side by side along k, offsets in 32 bits. Across k they read whole 16 bytes, too, of which those behind an operand's last column go nowhere.
 int skl_launch_grouped_ring_bf16(const skl_grouped_gemm &g);
 int skl_launch_grouped_ring_f16(const skl_grouped_gemm &g);
 int skl_launch_groupedk_ring_bf16(const skl_groupedk_gemm &g);
@@ -63,7 +63,7 @@ __device__ __forceinline__ SklRange skl_group_range(const int32_t *offsets, unsi
 }
 
 // Which tile of which group a workgroup takes. A group's rows are lines of MOST; the last one, if it is a small tile - for MOST == 256 of up to 128 rows -, comes behind everybody's others, so that
-// what ends last ends soon. Both kinds go group after group, up to eight lines of a group column by column so that B comes once for them, and are dealt out to the eight dies in runs, so that a die's
+// what ends last ends soon. Both kinds go group after group, up to eight lines of a group column by column so that a column of B serves them together, and are dealt out to the eight dies in runs, so that a die's
 // workgroups share operands. (Last lines of more than 128 rows behind the whole ones, too, read B once more: 8 groups of 14336 x 4096 with 8192 rows 926 us against 870, 64 of 2048 x 1408 with 32768
 // 270 against 250; all of a group's lines together and the dies' runs cut by cost 869 and 259, of 4096 x 4096 16 groups with 32768 rows 940 against 900.) Lane l counts for groups
 // l * each .. + each - 1.
